@@ -11,8 +11,10 @@ Public names mirror what the reference exports from its package root through laz
     DiscreteGroupedGemmDswigluSm100, discrete_grouped_gemm_dswiglu_wrapper_sm100
     GroupedGemmWgradSm100, grouped_gemm_wgrad_wrapper_sm100      (weight gradient: the experts split K)
 
-plus what the reference does not have: ``quantize_mxfp8`` (activation quantiser), the routing
-helpers of ``moe`` and the expert-parallel layer ``ExpertParallelMoE``.
+plus what the reference does not have: ``quantize_mxfp8`` (activation quantiser), the dense 16-bit operators
+``gated_ffn`` and ``linear`` with their backward passes (shared experts, projections, the router's), the gate
+``router_topk`` with its backward pass, the routing helpers of ``moe`` and the expert-parallel layer
+``ExpertParallelMoE``.
 """
 
 __version__ = "0.1.0"
@@ -36,6 +38,12 @@ _LAZY = {
     "quantize_mxfp8": "ops",
     "quantize_mxfp8_out": "ops",
     "empty_sf": "ops",
+    "gated_ffn": "dense",
+    "gated_ffn_backward": "dense",
+    "linear": "dense",
+    "linear_backward": "dense",
+    "router_topk": "moe",
+    "router_topk_backward": "moe",
     "route": "moe",
     "scatter_rows": "moe",
     "combine_rows": "moe",

@@ -13,8 +13,9 @@ from . import _build
 
 E_NULL, E_SHAPE, E_ALIGN, E_UNSUPPORTED, E_WORKSPACE, E_DEVICE = -1, -2, -3, -4, -5, -6
 DTYPE_BF16, DTYPE_E4M3, DTYPE_F16, DTYPE_F32, DTYPE_E5M2, DTYPE_E2M1 = 0, 1, 2, 3, 4, 5
-ACT_SWIGLU, ACT_GEGLU = 0, 1
+ACT_SWIGLU, ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4, 5
 ABI_VERSION = 7  # b200moe_abi_version() of the header these declarations mirror
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 FLAG_DISCRETE_COL_SFD = 1
 FLAG_TILE_SINGLE = 2
 FLAG_TILE_PAIR = 4
@@ -72,6 +73,12 @@ class GemmArgs(Structure):
     ]
 
 
+class DenseArgs(Structure):
+    _fields_ = [(name, c_void_p) for name in ("x", "w0", "w1", "bias", "residual", "dy", "y", "pre0", "pre1", "dx", "dw0", "dw1", "dbias", "workspace")] + [
+        (name, c_int64) for name in ("workspace_bytes", "m", "n", "k", "ld_x", "ld_w0", "ld_w1", "ld_residual", "ld_dy", "ld_y", "ld_pre0", "ld_pre1")
+    ] + [(name, c_int32) for name in ("dtype", "y_dtype", "bias_dtype", "act", "wait_limit_ms")]  # fmt: skip
+
+
 _SIGNATURES = {
     "b200moe_fc1_swiglu": (ctypes.c_int, [POINTER(GemmArgs), c_void_p]),
     "b200moe_fc2_quant": (ctypes.c_int, [POINTER(GemmArgs), c_void_p]),
@@ -117,6 +124,19 @@ _SIGNATURES = {
     "b200moe_peer_free": (ctypes.c_int, [c_void_p]),
     "b200moe_gather_rows": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "b200moe_combine_rows": (ctypes.c_int, [c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p, c_void_p]),
+    "b200moe_gated_ffn": (ctypes.c_int, [POINTER(DenseArgs), c_void_p]),
+    "b200moe_gated_ffn_backward": (ctypes.c_int, [POINTER(DenseArgs), c_void_p]),
+    "b200moe_linear": (ctypes.c_int, [POINTER(DenseArgs), c_void_p]),
+    "b200moe_linear_backward": (ctypes.c_int, [POINTER(DenseArgs), c_void_p]),
+    "b200moe_dense_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32]),
+    "b200moe_router_topk": (
+        ctypes.c_int,
+        [c_void_p, c_int32, c_int64, c_int32, c_int64, c_void_p, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p],
+    ),
+    "b200moe_router_topk_backward": (
+        ctypes.c_int,
+        [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p],
+    ),
     "b200moe_last_error": (c_char_p, []),
     "b200moe_device_status": (ctypes.c_int, [ctypes.c_int]),
     "b200moe_abi_version": (ctypes.c_int, []),

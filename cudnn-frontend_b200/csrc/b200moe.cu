@@ -2,3 +2,5 @@
 #include "quantize.cu"
 #include "grouped_gemm.cu"
 #include "routing.cu"
+#include "dense.cu"
+#include "router.cu"

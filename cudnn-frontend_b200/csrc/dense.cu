@@ -1,0 +1,941 @@
+// Dense 16-bit operators next to the grouped GEMMs: the gated feed-forward block of a shared or dense
+// expert and the projection with its epilogue, forward and backward.
+//
+//   gated:  h  = act(x Wg^T) * (x Wu^T)          dg, du from dh;  dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x
+//   linear: y  = act(x W^T + b) + r              dz = dy act'(z); dx = dz W;  dW = dz^T x;  db = column sums of dz
+//
+// Every product is one tcgen05 kernel (kind::f16, float32 accumulators in TMEM, operands staged by TMA in
+// 128-byte-swizzled shared memory).  The operand whose reduction dimension is contiguous is "K-major", the other
+// one "MN-major": both are read as they lie in memory, so nothing is ever transposed.
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
+
+#include "b200moe.h"
+#include "common.cuh"
+
+namespace b200moe {
+
+constexpr int DENSE_BK = 64;                          // elements of the reduction per stage: one 128-byte swizzle row
+constexpr int DENSE_SLAB = DENSE_BK * 128;            // an MN-major slab: 64 columns x 64 rows of the reduction
+constexpr int DENSE_A_BYTES = 128 * DENSE_BK * 2;     // 128 operand rows
+constexpr int DENSE_MAX_SPLIT = 8;                    // portable cluster size
+constexpr int ST_DENSE_EMPTY = 401, ST_DENSE_FULL = 402, ST_DENSE_ACC = 403, ST_DENSE_DRAIN = 404;
+
+// epilogues
+constexpr int DENSE_GLU = 0;     // gate and up accumulators -> activation product
+constexpr int DENSE_LINEAR = 1;  // bias, activation, residual
+constexpr int DENSE_STORE = 2;   // the accumulator as it is (gradients)
+
+struct DenseParams {
+  int rows, cols;            // valid rows (operand A side) and columns (operand B side) of the result
+  int row_tiles, col_tiles;  // of one result; with `stacked` there are 2 * row_tiles
+  int tile_cols;             // accumulator columns of a tile (per accumulator)
+  int k_tiles;               // stages over the whole reduction (both chains)
+  int chain_tiles;           // stages of one chain: beyond them the second pair of tensor maps is read
+  int split;                 // CTAs of a cluster that share a tile's reduction
+  int stages, stage_bytes;
+  int a_mn, b_mn;            // operand is MN-major
+  int stacked;               // row tiles beyond row_tiles belong to the second A operand and the second output
+  uint32_t idesc;
+  uint32_t tmem_cols;
+  int act;
+  int f16;                   // 16-bit type of the operands and of 16-bit outputs
+  int out_f32;
+  int bias_f32;
+  int vec_store;             // output rows may be written 16 bytes at a time
+  void* out[2];
+  void* pre[2];              // gate / up, or the pre-activation: written when not NULL
+  const void* bias;
+  const void* residual;
+  int64_t ld_out, ld_res, ld_pre[2];
+  uint64_t wait_limit_ns;
+};
+
+struct DenseMaps {
+  CUtensorMap a[2], b[2];
+};
+
+// Instruction descriptor of kind::f16: [4,6) D = float32, [7,10) / [10,13) A / B = fp16 (0) or bf16 (1), bit 15 / 16 A / B
+// MN-major, [17,23) N >> 3, [24,29) M >> 4
+static uint32_t dense_idesc(int m, int n, bool f16, bool a_mn, bool b_mn) {
+  const uint32_t t = f16 ? 0u : 1u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+template <bool kPair>
+__device__ __forceinline__ void mma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 32 lanes x 16 consecutive columns -> 16 registers per thread
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// later uses of v[] stay behind the tcgen05.wait::ld that precedes this call
+__device__ __forceinline__ void reg_fence16(float* v) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
+  return f16 ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store16(void* p, int64_t i, float v, bool f16) {
+  if (f16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ float2 unpack16x2(uint32_t w, bool f16) {
+  return f16 ? __half22float2(*reinterpret_cast<__half2*>(&w)) : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+}
+
+// ---------------------------------------------------------------------------------------
+// Activations.  sigmoid(v) = 1 / (1 + 2^(-v log2 e)) on the approximate exponential and reciprocal (about 2^-22
+// relative each): the results are rounded to 16 bits, where that is a 2^-10th of a step.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.0f + ex2_approx(v * -1.4426950408889634f)); }
+
+// SwiGLU: gate sigmoid(gate) up.  GeGLU as the grouped GEMM defines it: gate <= 7, -7 <= up <= 7,
+// (up + 1) gate sigmoid(1.702 gate).  The limits pass NaN on (a comparison, not fminf).
+__device__ __forceinline__ float glu_f(float g, float u, int act) {
+  if (act == B200MOE_ACT_GEGLU) {
+    g = g > 7.0f ? 7.0f : g;
+    u = u > 7.0f ? 7.0f : (u < -7.0f ? -7.0f : u);
+    return g * sigmoid_f(1.702f * g) * (u + 1.0f);
+  }
+  return g * sigmoid_f(g) * u;
+}
+// gradients with respect to gate and up; a limited value has none
+__device__ __forceinline__ void glu_grad_f(float dh, float g, float u, int act, float& dg, float& du) {
+  if (act == B200MOE_ACT_GEGLU) {
+    const bool g_in = !(g > 7.0f), u_in = !(u > 7.0f || u < -7.0f);
+    g = g_in ? g : 7.0f;
+    u = u > 7.0f ? 7.0f : (u < -7.0f ? -7.0f : u);
+    const float s = sigmoid_f(1.702f * g);
+    dg = g_in ? dh * (u + 1.0f) * s * (1.0f + 1.702f * g * (1.0f - s)) : 0.0f;
+    du = u_in ? dh * g * s : 0.0f;
+  } else {
+    const float s = sigmoid_f(g);
+    dg = dh * u * s * (1.0f + g * (1.0f - s));
+    du = dh * g * s;
+  }
+}
+__device__ __forceinline__ float act_f(float z, int act) {
+  switch (act) {
+    case B200MOE_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case B200MOE_ACT_SILU: return z * sigmoid_f(z);
+    case B200MOE_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);  // erfc keeps the negative tail's digits
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_grad_f(float z, int act) {
+  switch (act) {
+    case B200MOE_ACT_RELU: return z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);
+    case B200MOE_ACT_SILU: {
+      const float s = sigmoid_f(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case B200MOE_ACT_GELU: return 0.5f * erfcf(z * -0.70710678118654752f) + z * 0.3989422804014327f * ex2_approx(z * z * -0.72134752044448171f);
+    default: return 1.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// One tile per CTA.  The tile's reduction may be shared by the CTAs of a cluster: each walks its part of the
+// k-tiles, sends its partial sums to the owners of the columns through distributed shared memory, and every CTA
+// finishes its share of the columns.  Sums are added in the order of the ranks, so a result does not depend on timing.
+//
+// kDual: two A tiles per stage (gate and up weights) against one B tile.  kTrans: the rows of the tile are output
+// features and its columns are tokens, element (r, c) goes to out[c * ld + r] (32 lanes = 32 neighbouring
+// features); otherwise element (r, c) goes to out[r * ld + c].
+//
+// kSeg: the accumulator is drained into registers every kSegTiles stages and added there with float32
+// round-to-nearest.  The tensor core's own accumulation rounds towards zero: over K = 7168 that leaves a bias of
+// 7e-6 of the result (measured), 4e-7 over the 512 elements of a segment.  Used for float32 outputs; a 16-bit
+// output's rounding (2^-9) hides it.
+//
+// warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-5 epilogue (one per TMEM lane quarter)
+// ---------------------------------------------------------------------------------------
+constexpr int DENSE_THREADS = 192;
+constexpr int kSegTiles = 8;
+constexpr int kSegCols = 64;
+
+template <bool kDual, bool kTrans, int kEpi, bool kSeg>
+__global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const DenseParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_bars[2 * 16 + 4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  constexpr int kAcc = kDual ? 2 : 1;
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t bars = smem_u32(s_bars);
+  const int stages = p.stages;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (16 + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (32 + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (34 + b); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitCtx wc = {&s_abort, p.wait_limit_ns};
+
+  const int rank = (int)(blockIdx.x % (unsigned)p.split);
+  int tile = (int)(blockIdx.x / (unsigned)p.split);
+  const int all_row_tiles = p.row_tiles * (p.stacked ? 2 : 1);
+  int row_tile = tile % all_row_tiles;
+  const int col_tile = tile / all_row_tiles;
+  const int which = row_tile >= p.row_tiles ? 1 : 0;  // stacked: second operand and output
+  row_tile -= which * p.row_tiles;
+  const int row0 = row_tile * 128, col0 = col_tile * p.tile_cols;
+  const int C = p.tile_cols;
+  const int kt0 = (int)((int64_t)p.k_tiles * rank / p.split), kt1 = (int)((int64_t)p.k_tiles * (rank + 1) / p.split);
+  const int nk = kt1 - kt0;  // at least 1: split <= k_tiles
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 4);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&s_tmem), p.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0) {
+    // ---- producer -----------------------------------------------------------------------
+    const int a_bytes = kAcc * DENSE_A_BYTES;
+    const bool second_a = which != 0;
+    int issued = 0;
+    for (; issued < nk; ++issued) {
+      const int s = issued % stages;
+      const uint32_t phase = (uint32_t)(issued / stages) & 1u;
+      if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(s), phase ^ 1u, wc, ST_DENSE_EMPTY))) break;
+      if (elect_one()) {
+        const uint32_t fb = full_bar(s), dst = ring + (uint32_t)s * p.stage_bytes;
+        int kt = kt0 + issued, chain = 0;
+        if (kt >= p.chain_tiles) {
+          kt -= p.chain_tiles;
+          chain = 1;
+        }
+        const int kc = kt * DENSE_BK;
+        mbar_arrive_expect_tx(fb, (uint32_t)p.stage_bytes);
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a) {
+          const CUtensorMap* m = &maps.a[kDual ? a : ((chain | (second_a ? 1 : 0)) ? 1 : 0)];
+          const uint32_t d = dst + a * DENSE_A_BYTES;
+          if (p.a_mn) {
+            tma_load_2d(d, m, fb, row0, kc);
+            tma_load_2d(d + DENSE_SLAB, m, fb, row0 + 64, kc);
+          } else {
+            tma_load_2d(d, m, fb, kc, row0);
+          }
+        }
+        const CUtensorMap* m = &maps.b[chain];
+        if (p.b_mn) {
+          for (int q = 0; q < C / 64; ++q) tma_load_2d(dst + a_bytes + q * DENSE_SLAB, m, fb, col0 + 64 * q, kc);
+        } else {
+          tma_load_2d(dst + a_bytes, m, fb, kc, col0);
+        }
+      }
+      __syncwarp();
+    }
+    if (issued < nk) {
+      // a wait gave up: the copies already issued still write this CTA's shared memory, so they are waited for
+      // (with a limit) before the CTA may end
+      for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full_bar(i % stages), (uint32_t)(i / stages) & 1u, wc, ST_DENSE_DRAIN);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---- MMA issuer ---------------------------------------------------------------------
+    constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // SBO 1024, version 1, 128-byte swizzle
+    // K-major: 16 elements = 32 bytes further per MMA inside the swizzle row.  MN-major: 16 rows of 128 bytes; the
+    // leading byte offset is the distance of two slabs.  (In a cluster the shared-memory address of a CTA carries its
+    // rank above the 18 bits of the offset: only the 14-bit field goes into the descriptor.)
+    const uint32_t a_lo0 = ((ring >> 4) & 0x3FFFu) | (p.a_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
+    const uint32_t b_lo0 = (((ring + kAcc * DENSE_A_BYTES) >> 4) & 0x3FFFu) | (p.b_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
+    const uint32_t a_step = p.a_mn ? (16u * 128u) >> 4 : 2u, b_step = p.b_mn ? (16u * 128u) >> 4 : 2u;
+    auto desc = [](uint32_t lo) { return ((uint64_t)HI << 32) | lo; };
+    bool ok = true;
+    int seg = 0;
+    for (int i = 0; i < nk && ok; ++i) {
+      const int s = i % stages;
+      const int in_seg = kSeg ? i % kSegTiles : i;
+      const uint32_t acc = tmem + (kSeg ? (uint32_t)((seg & 1) * kAcc * C) : 0u);
+      if (kSeg && in_seg == 0 && seg >= 2) {
+        // the epilogue has taken the segment that used this accumulator
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_empty_bar(seg & 1), (uint32_t)((seg >> 1) - 1) & 1u, wc, ST_DENSE_ACC))) { ok = false; break; }
+        tc_fence_after();
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), (uint32_t)(i / stages) & 1u, wc, ST_DENSE_FULL))) { ok = false; break; }
+      const bool seg_end = i + 1 == nk || (kSeg && in_seg == kSegTiles - 1);
+      if (elect_one()) {
+        const uint32_t off = ((uint32_t)s * p.stage_bytes) >> 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int a = 0; a < kAcc; ++a)
+            mma_f16_ss<false>(acc + a * C, desc(a_lo0 + off + a * (DENSE_A_BYTES >> 4) + j * a_step), desc(b_lo0 + off + j * b_step), p.idesc,
+                              (in_seg | j) != 0);
+        }
+        tc_commit(empty_bar(s));
+        if (seg_end) tc_commit(acc_full_bar(kSeg ? seg & 1 : 0));
+      }
+      __syncwarp();
+      if (seg_end) ++seg;
+    }
+    __syncwarp();
+  }
+
+  // ---- epilogue -------------------------------------------------------------------------
+  const bool f16 = p.f16 != 0;
+  const int quarter = warp & 3;
+  const int r_in_tile = quarter * 32 + lane;
+  const int row = row0 + r_in_tile;
+  const bool row_ok = row < p.rows;
+  const int valid = min(C, p.cols - col0);
+  float sums[kSeg ? kSegCols : 1];
+  bool ok = true;
+  if (warp >= 2) {
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    if constexpr (kSeg) {
+#pragma unroll
+      for (int j = 0; j < kSegCols; ++j) sums[j] = 0.0f;
+      const int segs = (nk + kSegTiles - 1) / kSegTiles;
+      for (int sg = 0; sg < segs; ++sg) {
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_full_bar(sg & 1), (uint32_t)(sg >> 1) & 1u, wc, ST_DENSE_ACC))) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kSegCols; c += 16) {
+          if (c < C) {
+            float v[16];
+            tmem_ld_32x16(tmem + lanes + (uint32_t)((sg & 1) * C + c), v);
+            tmem_ld_wait();
+            reg_fence16(v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[c + j] += v[j];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty_bar(sg & 1));
+      }
+    } else {
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_full_bar(0), 0, wc, ST_DENSE_ACC));
+      tc_fence_after();
+    }
+  }
+
+  // columns of this CTA's accumulators in chunks of 16: f(first column, values of accumulator 0, of accumulator 1)
+  auto each_chunk = [&](auto f) {
+    if constexpr (kSeg) {
+#pragma unroll
+      for (int c = 0; c < kSegCols; c += 16)
+        if (c < valid) f(c, sums + c, sums + c);
+    } else {
+      const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c = 0; c < valid; c += 16) {
+        float v0[16], v1[16];
+        __syncwarp();
+        tmem_ld_32x16(base + c, v0);
+        if (kDual) tmem_ld_32x16(base + C + c, v1);
+        tmem_ld_wait();
+        reg_fence16(v0);
+        if (kDual) reg_fence16(v1);
+        f(c, v0, v1);
+      }
+    }
+  };
+
+  float bias = 0.0f;
+  if (kEpi == DENSE_LINEAR && warp >= 2 && p.bias && row_ok)
+    bias = p.bias_f32 ? reinterpret_cast<const float*>(p.bias)[row] : load16(p.bias, row, f16);
+  // kTrans: one element (feature = row, token = col0 + c); residual read by the caller
+  auto emit = [&](int c, float v0, float v1, float res) {
+    const int64_t o = (int64_t)(col0 + c) * p.ld_out + row;
+    float y;
+    if constexpr (kEpi == DENSE_GLU) {
+      if (p.pre[0]) {
+        store16(p.pre[0], (int64_t)(col0 + c) * p.ld_pre[0] + row, v0, f16);
+        store16(p.pre[1], (int64_t)(col0 + c) * p.ld_pre[1] + row, v1, f16);
+      }
+      y = glu_f(v0, v1, p.act);
+    } else {
+      const float z = v0 + bias;
+      if (p.pre[0]) store16(p.pre[0], (int64_t)(col0 + c) * p.ld_pre[0] + row, z, f16);
+      y = act_f(z, p.act) + res;
+    }
+    if (p.out_f32) reinterpret_cast<float*>(p.out[0])[o] = y;
+    else store16(p.out[0], o, y, f16);
+  };
+  auto residual_at = [&](int c) -> float {
+    if (kEpi == DENSE_LINEAR && p.residual) return load16(p.residual, (int64_t)(col0 + c) * p.ld_res + row, f16);
+    return 0.0f;
+  };
+
+  if (p.split > 1) {
+    const int slice = (valid + p.split - 1) / p.split;  // columns that one CTA of the cluster finishes
+    __syncwarp();
+    cluster_arrive();  // every CTA of the cluster has read its last operand stage: the rings may be overwritten
+    cluster_wait();
+    if (warp >= 2 && ok) {
+      each_chunk([&](int c0, const float* v0, const float* v1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int c = c0 + j;
+          if (c < valid) {
+            const int owner = c / slice;
+            const uint32_t a = map_to_cta(ring, (uint32_t)owner) + (uint32_t)((((rank * kAcc) * slice + (c - owner * slice)) * 128 + r_in_tile) * 4);
+            st_cluster_f32(a, v0[j]);
+            if (kDual) st_cluster_f32(a + (uint32_t)(slice * 512), v1[j]);
+          }
+        }
+      });
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2 && row_ok) {
+      const float* part = reinterpret_cast<const float*>(smem) + r_in_tile;
+      const int c0 = rank * slice, c1 = min(valid, c0 + slice);
+      for (int c = c0; c < c1; ++c) {
+        const float res = kTrans ? residual_at(c) : 0.0f;
+        float v0 = 0.0f, v1 = 0.0f;
+        for (int r = 0; r < p.split; ++r) {
+          v0 += part[((r * kAcc) * slice + (c - c0)) * 128];
+          if (kDual) v1 += part[((r * kAcc + 1) * slice + (c - c0)) * 128];
+        }
+        if constexpr (kTrans) emit(c, v0, v1, res);
+        else store16(p.out[which], (int64_t)row * p.ld_out + col0 + c, v0, f16);
+      }
+    }
+  } else if (warp >= 2 && ok) {
+    each_chunk([&](int c0, const float* v0, const float* v1) {
+      if constexpr (kTrans) {
+        if (!row_ok) return;
+        float res[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) res[j] = c0 + j < valid ? residual_at(c0 + j) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c0 + j < valid) emit(c0 + j, v0[j], v1[j], res[j]);
+      } else {
+        if (!row_ok) return;
+        const int64_t o = (int64_t)row * p.ld_out + col0 + c0;
+        if (p.vec_store && c0 + 16 <= valid) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = pack16x2_from_float(v0[2 * j], v0[2 * j + 1], f16);
+          uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out[which]) + o);
+          d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c0 + j < valid) store16(p.out[which], o + j, v0[j], f16);
+        }
+      }
+    });
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, p.tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Elementwise parts of the backward passes: one read of the incoming gradient and of the saved pre-activations, one
+// write of the operand that the two gradient products share, with its rows padded to 8 values so that TMA can read it.
+// ---------------------------------------------------------------------------------------
+constexpr int GRAD_COLS = 256;  // columns of a block: 32 lanes x 8
+
+// dg, du [m, ldo] from dh, gate, up [m, n]
+__global__ void __launch_bounds__(256)
+    glu_grad_kernel(const void* __restrict__ dh, const void* __restrict__ gate, const void* __restrict__ up, int64_t m, int n, int64_t ld_dh,
+                    int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int act, int f16, int vec) {
+  const int c = (int)blockIdx.x * GRAD_COLS + (threadIdx.x & 31) * 8;
+  if (c >= n) return;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < m; r += (int64_t)gridDim.y * 8) {
+    float d[8], g[8], u[8];
+    if (vec && c + 8 <= n) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dh) + r * ld_dh + c));
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(gate) + r * ld_gate + c));
+      const uint4 e = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(up) + r * ld_up + c));
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w}, ew[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = unpack16x2(aw[j], f16), q = unpack16x2(bw[j], f16), s = unpack16x2(ew[j], f16);
+        d[2 * j] = p.x, d[2 * j + 1] = p.y, g[2 * j] = q.x, g[2 * j + 1] = q.y, u[2 * j] = s.x, u[2 * j + 1] = s.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = c + j < n;
+        d[j] = in ? load16(dh, r * ld_dh + c + j, f16) : 0.0f;
+        g[j] = in ? load16(gate, r * ld_gate + c + j, f16) : 0.0f;
+        u[j] = in ? load16(up, r * ld_up + c + j, f16) : 0.0f;
+      }
+    }
+    uint32_t gw[4], uw[4];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float a0, a1, b0, b1;
+      glu_grad_f(d[j], g[j], u[j], act, a0, b0);
+      glu_grad_f(d[j + 1], g[j + 1], u[j + 1], act, a1, b1);
+      gw[j / 2] = pack16x2_from_float(a0, a1, f16);
+      uw[j / 2] = pack16x2_from_float(b0, b1, f16);
+    }
+    // (the padding columns of the last 8 are written too: they are part of the padded row)
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = make_uint4(gw[0], gw[1], gw[2], gw[3]);
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = make_uint4(uw[0], uw[1], uw[2], uw[3]);
+  }
+}
+
+// dz [m, ldo] = dy act'(z) (dz == NULL: dy is used as it is), and the column sums of the unrounded dz over the block's
+// rows: sums [gridDim.y][n].  Every sum has a fixed order: a warp's rows, then the warps, then (next kernel) the blocks.
+__global__ void __launch_bounds__(256)
+    act_grad_kernel(const void* __restrict__ dy, const void* __restrict__ z, int64_t m, int n, int64_t ld_dy, int64_t ld_z, void* __restrict__ dz,
+                    int64_t ldo, float* __restrict__ sums, int act, int f16, int dy_f32, int vec, int64_t rows_per_block) {
+  __shared__ float s_part[8][GRAD_COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = (int)blockIdx.x * GRAD_COLS + lane * 8;
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+  const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(m, r0 + rows_per_block);
+  if (c < n) {
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      float d[8];
+      const bool whole = vec && c + 8 <= n;
+      if (dy_f32) {
+        const float* src = reinterpret_cast<const float*>(dy) + r * ld_dy + c;
+        if (whole) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+          d[0] = a.x, d[1] = a.y, d[2] = a.z, d[3] = a.w, d[4] = b.x, d[5] = b.y, d[6] = b.z, d[7] = b.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] = c + j < n ? src[j] : 0.0f;
+        }
+      } else if (whole) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dy) + r * ld_dy + c));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = unpack16x2(w[j], f16);
+          d[2 * j] = p.x, d[2 * j + 1] = p.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = c + j < n ? load16(dy, r * ld_dy + c + j, f16) : 0.0f;
+      }
+      if (z) {
+        if (whole) {
+          const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(z) + r * ld_z + c));
+          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 p = unpack16x2(w[j], f16);
+            d[2 * j] *= act_grad_f(p.x, act), d[2 * j + 1] *= act_grad_f(p.y, act);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (c + j < n) d[j] *= act_grad_f(load16(z, r * ld_z + c + j, f16), act);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += d[j];
+      if (dz) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pack16x2_from_float(d[2 * j], d[2 * j + 1], f16);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + r * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  if (sums) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_part[warp][lane * 8 + j] = acc[j];
+    __syncthreads();
+    const int col = (int)blockIdx.x * GRAD_COLS + threadIdx.x;
+    if (col < n) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += s_part[w][threadIdx.x];
+      sums[(int64_t)blockIdx.y * n + col] = t;
+    }
+  }
+}
+
+// out[c] = sum over the blocks' partial sums, in order
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ sums, int blocks, int n, float* __restrict__ out) {
+  const int c = (int)blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  float t = 0.0f;
+  for (int b = 0; b < blocks; ++b) t += sums[(int64_t)b * n + c];
+  out[c] = t;
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+static int dense_encode(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int f16) {
+  uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
+  uint64_t strides[1] = {(uint64_t)ld * 2};
+  uint32_t box[2] = {(uint32_t)DENSE_BK, (uint32_t)box_rows};
+  return encode_map(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, 2, dims, strides, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// A matrix operand of a product, as it lies in memory: `outer` rows of `inner` contiguous values, pitch `ld`
+struct DenseOperand {
+  const void* base;
+  int64_t outer, inner, ld;
+};
+
+struct DenseGemm {
+  DenseOperand a[2], b[2];
+  bool dual = false;          // a[0], a[1] side by side against b[0]
+  bool chained = false;       // a[0] b[0] + a[1] b[1]
+  bool stacked = false;       // a[0] b[0] -> out[0], a[1] b[0] -> out[1]
+  bool a_mn = false, b_mn = false;
+  int64_t rows = 0, cols = 0, red = 0;  // result rows and columns, length of the reduction (of one chain)
+  bool trans = false;
+  int epi = DENSE_STORE;
+  bool segmented = false;
+};
+
+template <bool kDual, bool kTrans, int kEpi, bool kSeg>
+static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsigned grid, cudaStream_t stream) {
+  auto kern = dense_tile_kernel<kDual, kTrans, kEpi, kSeg>;
+  const int smem = p.stages * p.stage_bytes + 1024;
+  static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  int dev = 0;
+  B200_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024));
+    ready.fetch_or(1ull << (dev & 63));
+  }
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(DENSE_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, maps, p));
+  return B200MOE_OK;
+}
+
+// Shared part of every product: tiles, tensor maps, launch.  `p` arrives with its epilogue fields set.
+static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaStream_t stream) {
+  p.rows = (int)g.rows;
+  p.cols = (int)g.cols;
+  p.a_mn = g.a_mn;
+  p.b_mn = g.b_mn;
+  p.stacked = g.stacked;
+  int C = g.b_mn ? 128 : (g.cols <= 16 ? 16 : (g.cols <= 32 ? 32 : (g.cols <= 64 ? 64 : 128)));
+  if (g.segmented) C = std::min(C, kSegCols);
+  p.tile_cols = C;
+  p.row_tiles = (int)((g.rows + 127) / 128);
+  p.col_tiles = (int)((g.cols + C - 1) / C);
+  p.chain_tiles = (int)((g.red + DENSE_BK - 1) / DENSE_BK);
+  p.k_tiles = p.chain_tiles * (g.chained ? 2 : 1);
+  const int acc = g.dual ? 2 : 1;
+  p.stage_bytes = acc * DENSE_A_BYTES + C * 128;
+  p.stages = std::min(16, (110 * 1024) / p.stage_bytes);
+  const int64_t tiles = (int64_t)p.row_tiles * (g.stacked ? 2 : 1) * p.col_tiles;
+  p.split = 1;
+  if (C <= 64) {
+    while (p.split < DENSE_MAX_SPLIT && tiles * p.split * 2 <= 2 * di->sm_count && p.k_tiles >= p.split * 2 * 4) p.split *= 2;
+  }
+  const int cols = acc * C * (g.segmented ? 2 : 1);
+  p.tmem_cols = cols <= 32 ? 32 : (cols <= 64 ? 64 : (cols <= 128 ? 128 : 256));
+  p.idesc = dense_idesc(128, C, p.f16 != 0, g.a_mn, g.b_mn);
+  if (tiles * p.split > 0x7fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
+
+  DenseMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  const int na = (g.dual || g.chained || g.stacked) ? 2 : 1, nb = g.chained ? 2 : 1;
+  for (int i = 0; i < na; ++i) {
+    int rc = dense_encode(&maps.a[i], g.a[i].base, g.a[i].outer, g.a[i].inner, g.a[i].ld, g.a_mn ? 64 : 128, p.f16);
+    if (rc) return rc;
+  }
+  for (int i = 0; i < nb; ++i) {
+    int rc = dense_encode(&maps.b[i], g.b[i].base, g.b[i].outer, g.b[i].inner, g.b[i].ld, g.b_mn ? 64 : C, p.f16);
+    if (rc) return rc;
+  }
+  const unsigned grid = (unsigned)(tiles * p.split);
+  if (g.epi == DENSE_GLU) return dense_launch_tile<true, true, DENSE_GLU, false>(maps, p, grid, stream);
+  if (g.trans && g.segmented) return dense_launch_tile<false, true, DENSE_LINEAR, true>(maps, p, grid, stream);
+  if (g.trans) return dense_launch_tile<false, true, DENSE_LINEAR, false>(maps, p, grid, stream);
+  return dense_launch_tile<false, false, DENSE_STORE, false>(maps, p, grid, stream);
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// a TMA operand: 16-byte aligned base and pitch
+static int check_operand(const char* op, const char* name, const void* p, int64_t ld, int64_t inner) {
+  if (!p) return fail(B200MOE_E_NULL, "%s: %s is required", op, name);
+  if (ld < inner) return fail(B200MOE_E_SHAPE, "%s: the pitch of %s is below its row length", op, name);
+  if (!aligned16(p) || ld % 8 != 0) return fail(B200MOE_E_ALIGN, "%s: %s must start on a 16-byte boundary and have a pitch of a multiple of 8", op, name);
+  return B200MOE_OK;
+}
+
+static int dense_check_common(const char* op, const b200moe_dense_args* a, bool gated, DeviceInfo** di) {
+  if (!a) return fail(B200MOE_E_NULL, "args is NULL");
+  if (a->m < 0 || a->n < 1 || a->k < 1 || a->m > 0x7ffffff0 || a->n > 0x3ffffff0 || a->k > 0x3ffffff0)
+    return fail(B200MOE_E_SHAPE, "%s: m, n, k = %lld, %lld, %lld out of range", op, (long long)a->m, (long long)a->n, (long long)a->k);
+  if (a->k % 8 != 0) return fail(B200MOE_E_SHAPE, "%s: k = %lld must be a multiple of 8", op, (long long)a->k);
+  if (a->dtype != B200MOE_DTYPE_BF16 && a->dtype != B200MOE_DTYPE_F16) return fail(B200MOE_E_UNSUPPORTED, "%s: dtype %d", op, a->dtype);
+  if (gated ? (a->act != B200MOE_ACT_SWIGLU && a->act != B200MOE_ACT_GEGLU)
+            : (a->act != B200MOE_ACT_NONE && a->act != B200MOE_ACT_RELU && a->act != B200MOE_ACT_SILU && a->act != B200MOE_ACT_GELU))
+    return fail(B200MOE_E_UNSUPPORTED, "%s: act %d", op, a->act);
+  if (a->wait_limit_ms < 0) return fail(B200MOE_E_SHAPE, "%s: wait_limit_ms must not be negative", op);
+  int rc = check_operand(op, gated ? "w_gate" : "weight", a->w0, a->ld_w0, a->k);
+  if (!rc && gated) rc = check_operand(op, "w_up", a->w1, a->ld_w1, a->k);
+  if (!rc && a->m > 0) rc = check_operand(op, "x", a->x, a->ld_x, a->k);
+  if (rc) return rc;
+  rc = get_device_info(di);
+  if (rc) return rc;
+  if ((*di)->cc_major != 10) return fail(B200MOE_E_DEVICE, "%s: needs an sm_100 device, found compute capability %d.x", op, (*di)->cc_major);
+  return B200MOE_OK;
+}
+
+static void dense_params(DenseParams& p, const b200moe_dense_args* a) {
+  memset(&p, 0, sizeof(p));
+  p.f16 = a->dtype == B200MOE_DTYPE_F16;
+  p.act = a->act;
+  p.wait_limit_ns = a->wait_limit_ms > 0 ? (uint64_t)a->wait_limit_ms * 1000000ull : kWaitLimitNs;
+}
+
+static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated, cudaStream_t stream) {
+  DeviceInfo* di = nullptr;
+  int rc = dense_check_common(op, a, gated, &di);
+  if (rc) return rc;
+  if (a->m == 0) return B200MOE_OK;
+  if (!a->y) return fail(B200MOE_E_NULL, "%s: the output is required", op);
+  if (a->ld_y < a->n || (a->pre0 && a->ld_pre0 < a->n) || (a->pre1 && a->ld_pre1 < a->n)) return fail(B200MOE_E_SHAPE, "%s: an output's pitch is below n", op);
+  if (gated && (a->pre0 == nullptr) != (a->pre1 == nullptr)) return fail(B200MOE_E_NULL, "%s: gate and up go together", op);
+  if (gated ? a->y_dtype != a->dtype : (a->y_dtype != a->dtype && a->y_dtype != B200MOE_DTYPE_F32))
+    return fail(B200MOE_E_UNSUPPORTED, "%s: output dtype %d", op, a->y_dtype);
+  if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != B200MOE_DTYPE_F32) return fail(B200MOE_E_UNSUPPORTED, "%s: bias dtype %d", op, a->bias_dtype);
+  DenseParams p;
+  dense_params(p, a);
+  p.out[0] = a->y;
+  p.ld_out = a->ld_y;
+  p.pre[0] = a->pre0;
+  p.pre[1] = a->pre1;
+  p.ld_pre[0] = a->ld_pre0;
+  p.ld_pre[1] = a->ld_pre1;
+  DenseGemm g;
+  g.a[0] = {a->w0, a->n, a->k, a->ld_w0};
+  g.b[0] = {a->x, a->m, a->k, a->ld_x};
+  g.rows = a->n;
+  g.cols = a->m;
+  g.red = a->k;
+  g.trans = true;
+  if (gated) {
+    g.a[1] = {a->w1, a->n, a->k, a->ld_w1};
+    g.dual = true;
+    g.epi = DENSE_GLU;
+  } else {
+    g.epi = DENSE_LINEAR;
+    p.bias = a->bias;
+    p.bias_f32 = a->bias_dtype == B200MOE_DTYPE_F32;
+    p.residual = a->residual;
+    p.ld_res = a->ld_residual;
+    p.out_f32 = a->y_dtype == B200MOE_DTYPE_F32;
+    g.segmented = p.out_f32 != 0;
+  }
+  return dense_gemm(g, p, di, stream);
+}
+
+// blocks along the rows of act_grad_kernel, and the rows of each
+static int grad_row_blocks(int64_t m, int64_t n, int64_t* rows_per_block) {
+  const int64_t col_blocks = (n + GRAD_COLS - 1) / GRAD_COLS;
+  int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((m + 31) / 32, 148 * 8 / std::max<int64_t>(1, col_blocks)));
+  *rows_per_block = (m + blocks - 1) / std::max<int64_t>(1, blocks);
+  return (int)((m + *rows_per_block - 1) / *rows_per_block);
+}
+
+static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// dx = sum of dz_i w_i and dw_i = dz_i^T x
+static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, DeviceInfo* di, cudaStream_t stream) {
+  DenseParams p;
+  if (a->dx) {
+    dense_params(p, a);
+    p.act = B200MOE_ACT_NONE;
+    p.out[0] = a->dx;
+    p.ld_out = a->k;
+    DenseGemm g;
+    // rows = the k features of x: w [n, k] is MN-major; columns = tokens
+    g.a[0] = {a->w0, a->n, a->k, a->ld_w0};
+    g.b[0] = {dz[0], a->m, a->n, ld_dz};
+    if (count == 2) {
+      g.a[1] = {a->w1, a->n, a->k, a->ld_w1};
+      g.b[1] = {dz[1], a->m, a->n, ld_dz};
+      g.chained = true;
+    }
+    g.a_mn = true;
+    g.rows = a->k;
+    g.cols = a->m;
+    g.red = a->n;
+    g.trans = true;
+    g.epi = DENSE_LINEAR;
+    int rc = dense_gemm(g, p, di, stream);
+    if (rc) return rc;
+  }
+  if (a->dw0) {
+    dense_params(p, a);
+    p.out[0] = a->dw0;
+    p.out[1] = a->dw1;
+    p.ld_out = a->k;
+    p.vec_store = aligned16(a->dw0) && aligned16(a->dw1);
+    DenseGemm g;
+    g.a[0] = {dz[0], a->m, a->n, ld_dz};
+    g.b[0] = {a->x, a->m, a->k, a->ld_x};
+    if (count == 2) {
+      g.a[1] = {dz[1], a->m, a->n, ld_dz};
+      g.stacked = true;
+    }
+    g.a_mn = g.b_mn = true;
+    g.rows = a->n;
+    g.cols = a->k;
+    g.red = a->m;
+    int rc = dense_gemm(g, p, di, stream);
+    if (rc) return rc;
+  }
+  return B200MOE_OK;
+}
+
+static int zero_outputs(const b200moe_dense_args* a, bool gated, cudaStream_t stream) {
+  // no tokens: the weights' gradients are zero
+  if (a->dw0) B200_CUDA_CHECK(cudaMemsetAsync(a->dw0, 0, (size_t)a->n * a->k * 2, stream));
+  if (gated && a->dw1) B200_CUDA_CHECK(cudaMemsetAsync(a->dw1, 0, (size_t)a->n * a->k * 2, stream));
+  if (!gated && a->dbias) B200_CUDA_CHECK(cudaMemsetAsync(a->dbias, 0, (size_t)a->n * 4, stream));
+  return B200MOE_OK;
+}
+
+static int64_t dense_workspace(int64_t m, int64_t n, bool gated) {
+  const int64_t ldo = (n + 7) / 8 * 8;
+  if (m <= 0) return 0;
+  if (gated) return 2 * round256(m * ldo * 2);
+  int64_t rows_per_block;
+  return round256(m * ldo * 2) + round256((int64_t)grad_row_blocks(m, n, &rows_per_block) * n * 4);
+}
+
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_gated_ffn(const b200moe_dense_args* a, void* stream) { return dense_forward("gated_ffn", a, true, (cudaStream_t)stream); }
+
+extern "C" int b200moe_linear(const b200moe_dense_args* a, void* stream) { return dense_forward("linear", a, false, (cudaStream_t)stream); }
+
+extern "C" int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t gated) { return dense_workspace(m, n, gated != 0); }
+
+extern "C" int b200moe_gated_ffn_backward(const b200moe_dense_args* a, void* stream_v) {
+  const char* op = "gated_ffn_backward";
+  cudaStream_t stream = (cudaStream_t)stream_v;
+  DeviceInfo* di = nullptr;
+  int rc = dense_check_common(op, a, true, &di);
+  if (rc) return rc;
+  if ((a->dw0 == nullptr) != (a->dw1 == nullptr)) return fail(B200MOE_E_NULL, "%s: the two weights' gradients go together", op);
+  if (a->m == 0) return zero_outputs(a, true, stream);
+  if (!a->dy || !a->pre0 || !a->pre1) return fail(B200MOE_E_NULL, "%s: dh, gate and up are required", op);
+  if (a->ld_dy < a->n || a->ld_pre0 < a->n || a->ld_pre1 < a->n) return fail(B200MOE_E_SHAPE, "%s: a pitch is below n", op);
+  const int64_t ldo = (a->n + 7) / 8 * 8;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, true))
+    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, true));
+  void* dg = a->workspace;
+  void* du = (uint8_t*)a->workspace + round256(a->m * ldo * 2);
+  const int vec = aligned16(a->dy) && aligned16(a->pre0) && aligned16(a->pre1) && a->ld_dy % 8 == 0 && a->ld_pre0 % 8 == 0 && a->ld_pre1 % 8 == 0;
+  const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)std::min<int64_t>((a->m + 7) / 8, 32768));
+  glu_grad_kernel<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, dg, du, ldo, a->act,
+                                            a->dtype == B200MOE_DTYPE_F16, vec);
+  B200_CUDA_CHECK(cudaGetLastError());
+  const void* dz[2] = {dg, du};
+  return dense_grad_products(a, 2, dz, ldo, di, stream);
+}
+
+extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream_v) {
+  const char* op = "linear_backward";
+  cudaStream_t stream = (cudaStream_t)stream_v;
+  DeviceInfo* di = nullptr;
+  int rc = dense_check_common(op, a, false, &di);
+  if (rc) return rc;
+  if (a->y_dtype != a->dtype && a->y_dtype != B200MOE_DTYPE_F32) return fail(B200MOE_E_UNSUPPORTED, "%s: dtype %d of dy", op, a->y_dtype);
+  if (a->m == 0) return zero_outputs(a, false, stream);
+  const bool has_act = a->act != B200MOE_ACT_NONE;
+  if (!a->dy || (has_act && !a->pre0)) return fail(B200MOE_E_NULL, "%s: dy, and with an activation the pre-activation, are required", op);
+  if (a->ld_dy < a->n || (has_act && a->ld_pre0 < a->n)) return fail(B200MOE_E_SHAPE, "%s: a pitch is below n", op);
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, false))
+    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, false));
+  const bool dy_f32 = a->y_dtype == B200MOE_DTYPE_F32;
+  int64_t ldo = (a->n + 7) / 8 * 8;
+  // without an activation the gradient products read dy itself, where TMA can
+  const bool as_is = !has_act && !dy_f32 && aligned16(a->dy) && a->ld_dy % 8 == 0;
+  const void* dz = as_is ? a->dy : a->workspace;
+  if (!as_is || a->dbias) {
+    float* sums = a->dbias ? (float*)((uint8_t*)a->workspace + round256(a->m * ldo * 2)) : nullptr;
+    const int64_t dy_unit = dy_f32 ? 4 : 8;
+    const int vec = aligned16(a->dy) && a->ld_dy % dy_unit == 0 && (!has_act || (aligned16(a->pre0) && a->ld_pre0 % 8 == 0));
+    int64_t rows_per_block;
+    const int row_blocks = grad_row_blocks(a->m, a->n, &rows_per_block);
+    const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)row_blocks);
+    act_grad_kernel<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo,
+                                              sums, a->act, a->dtype == B200MOE_DTYPE_F16, dy_f32, vec, rows_per_block);
+    B200_CUDA_CHECK(cudaGetLastError());
+    if (sums) {
+      column_sum_kernel<<<(unsigned)((a->n + 255) / 256), 256, 0, stream>>>(sums, row_blocks, (int)a->n, a->dbias);
+      B200_CUDA_CHECK(cudaGetLastError());
+    }
+  }
+  const void* dzs[2] = {dz, nullptr};
+  return dense_grad_products(a, 1, dzs, as_is ? a->ld_dy : ldo, di, stream);
+}

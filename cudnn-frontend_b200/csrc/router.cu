@@ -1,0 +1,274 @@
+// The gate in front of the experts: top-k choice with its weights, and the gradient of the logits.
+//
+//   choice   the topk largest of l + 0 (or, with a selection bias b, of score(l) + b), ties to the lowest index;
+//            a logit of -inf is never chosen, and a slot that finds no expert gets id -1 and weight 0
+//   weights  w_j = scale * score_j, or normalised over the chosen ones scale * score_j / sum_i score_i, with
+//            score = softmax over the row, or sigmoid.  The bias decides the choice only.
+//
+// The normalised sigmoid is softmax over log sigmoid(l): the quotient of two numbers that may both underflow is
+// never formed.
+#include <type_traits>
+
+#include "b200moe.h"
+#include "common.cuh"
+
+namespace b200moe {
+
+constexpr int ROUTER_MAX_EXPERTS = 1024;
+constexpr int ROUTER_MAX_TOPK = 32;
+
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
+  if (dtype == B200MOE_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == B200MOE_DTYPE_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, float v, int dtype) {
+  if (dtype == B200MOE_DTYPE_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == B200MOE_DTYPE_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Keys that order like the values (NaN above everything, 0 and -0 equal); key 0 = never chosen
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  if (v == -INFINITY) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_key64(double v) {
+  if (v != v) return ~0ull;
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float o = __shfl_xor_sync(0xffffffffu, v, d);
+    v = (o != o || o > v) ? o : v;  // NaN stays
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+__device__ __forceinline__ float log_sigmoid_f(float v) { return fminf(v, 0.0f) - log1pf(expf(-fabsf(v))); }
+__device__ __forceinline__ float sigmoid_exact_f(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+// Weight of the choice that this lane holds (lanes without one: chosen = false); called by the whole warp.
+// row_max / row_sum: of the whole row, for the softmax that is not normalised over the choice.
+__device__ __forceinline__ float choice_weight(float logit, bool chosen, int sigmoid, int normalize, float scale, float row_max, float row_sum) {
+  if (normalize) {
+    const float a = chosen ? (sigmoid ? (logit != logit ? logit : log_sigmoid_f(logit)) : logit) : -INFINITY;
+    const float m = warp_max(a);
+    const float e = chosen ? expf(a - m) : 0.0f;
+    const float s = warp_sum(e);
+    return chosen ? scale * (e / s) : 0.0f;
+  }
+  if (!chosen) return 0.0f;
+  return scale * (sigmoid ? sigmoid_exact_f(logit) : expf(logit - row_max) / row_sum);
+}
+
+// One warp per row; lane l holds experts l, l + 32, ...
+template <int kPerLane, bool kBias>
+__global__ void __launch_bounds__(256)
+    router_topk_kernel(const void* __restrict__ logits, int dtype, int64_t rows, int experts, int64_t ld, const float* __restrict__ bias, int topk,
+                       int sigmoid, int normalize, float scale, float* __restrict__ weights, int32_t* __restrict__ ids) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  float v[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < experts ? load_any(logits, row * ld + e, dtype) : -INFINITY;
+  }
+  float row_max = -INFINITY, row_sum = 1.0f;
+  if (!sigmoid && !normalize) {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) row_max = (v[i] != v[i] || v[i] > row_max) ? v[i] : row_max;
+    row_max = warp_max(row_max);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) s += v[i] == -INFINITY ? 0.0f : expf(v[i] - row_max);
+    row_sum = warp_sum(s);
+  }
+  // 32-bit keys of the logits, or 64-bit keys of the biased scores: those decide between neighbours that differ in the
+  // last bits of a float32, so they are formed in 64 bits
+  using Key = typename std::conditional<kBias, uint64_t, uint32_t>::type;
+  Key key[kPerLane];
+  if constexpr (kBias) {
+    double wide[kPerLane], top = -INFINITY, sum = 0.0;
+    if (!sigmoid) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) top = fmax(top, (double)v[i]);
+      for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+    }
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      wide[i] = v[i] == -INFINITY ? 0.0 : (sigmoid ? 1.0 / (1.0 + exp(-(double)v[i])) : exp((double)v[i] - top));
+      sum += wide[i];
+    }
+    if (!sigmoid) sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int e = lane + 32 * i;
+      key[i] = v[i] == -INFINITY ? 0ull : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) key[i] = order_key(v[i]);
+  }
+  int my_id = -1;
+  float my_logit = -INFINITY;
+  for (int j = 0; j < topk; ++j) {
+    Key best = 0;
+    int at = 0;
+    float logit = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (key[i] > best) best = key[i], at = i, logit = v[i];
+    Key top;
+    if constexpr (kBias) {
+      const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+      const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+      top = (uint64_t)hi << 32 | lo;
+    } else {
+      top = __reduce_max_sync(0xffffffffu, best);
+    }
+    if (top == 0) break;  // nothing left that may be chosen
+    const int id = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * at : 0x7fffffff);
+    const float l = __shfl_sync(0xffffffffu, logit, id & 31);
+    if (lane == j) my_id = id, my_logit = l;
+    if (lane == (id & 31)) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i)
+        if (i == (id >> 5)) key[i] = 0;
+    }
+  }
+  const float w = choice_weight(my_logit, my_id >= 0, sigmoid, normalize, scale, row_max, row_sum);
+  if (lane < topk) {
+    weights[row * topk + lane] = w;
+    ids[row * topk + lane] = my_id;
+  }
+}
+
+// dlogits [rows, experts] from the gradient of the weights and the choice.  With c the chosen set and dw' = scale dw:
+//   softmax, normalised   dl_i = w_i (dw_i - sum_c w_j dw_j / scale)              (i in c, else 0)
+//   sigmoid, normalised   the same times 1 - sigmoid(l_i)
+//   sigmoid               dl_i = dw'_i s_i (1 - s_i)
+//   softmax               dl_e = p_e (dw'_e - sum_c p_j dw'_j)                   (every e; dw'_e = 0 outside c)
+// An expert that occurs twice gets the sum of both gradients.
+__global__ void __launch_bounds__(256)
+    router_grad_kernel(const float* __restrict__ dweights, const void* __restrict__ logits, int dtype, const int32_t* __restrict__ ids, int64_t rows,
+                       int experts, int64_t ld, int topk, int sigmoid, int normalize, float scale, void* __restrict__ dlogits) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  int id = lane < topk ? ids[row * topk + lane] : -1;
+  if (id >= experts) id = -1;
+  const bool chosen = id >= 0;
+  const float logit = chosen ? load_any(logits, row * ld + id, dtype) : -INFINITY;
+  const float dw = chosen ? dweights[row * topk + lane] : 0.0f;
+  const bool whole_row = !sigmoid && !normalize;
+  float row_max = -INFINITY, row_sum = 1.0f;
+  if (whole_row) {
+    for (int e = lane; e < experts; e += 32) {
+      const float v = load_any(logits, row * ld + e, dtype);
+      row_max = (v != v || v > row_max) ? v : row_max;
+    }
+    row_max = warp_max(row_max);
+    float s = 0.0f;
+    for (int e = lane; e < experts; e += 32) {
+      const float v = load_any(logits, row * ld + e, dtype);
+      s += v == -INFINITY ? 0.0f : expf(v - row_max);
+    }
+    row_sum = warp_sum(s);
+  }
+  const float w = choice_weight(logit, chosen, sigmoid, normalize, scale, row_max, row_sum);
+  const float dot = warp_sum(w * dw);
+  float g;
+  if (normalize) {
+    g = w * (dw - (scale != 0.0f ? dot / scale : 0.0f));
+    if (sigmoid) g *= sigmoid_exact_f(-logit);
+  } else {
+    g = w * dw;
+    if (sigmoid) g *= sigmoid_exact_f(-logit);
+  }
+  if (!chosen) g = 0.0f;
+  float total = 0.0f;
+  for (int j = 0; j < topk; ++j) {
+    const int other = __shfl_sync(0xffffffffu, id, j);
+    const float v = __shfl_sync(0xffffffffu, g, j);
+    if (other == id) total += v;
+  }
+  const int64_t base = row * experts;
+  for (int e = lane; e < experts; e += 32) {
+    float v = 0.0f;
+    if (whole_row) {
+      const float l = load_any(logits, row * ld + e, dtype);
+      if (l != -INFINITY) v = -(expf(l - row_max) / row_sum) * dot;
+    }
+    store_any(dlogits, base + e, v, dtype);
+  }
+  __syncwarp();  // the row is written before its chosen entries are
+  if (chosen) {
+    if (whole_row && logit != -INFINITY) total -= (expf(logit - row_max) / row_sum) * dot;
+    store_any(dlogits, base + id, total, dtype);
+  }
+}
+
+static int router_check(const char* op, const void* logits, int dtype, int64_t rows, int32_t experts, int64_t ld, int32_t topk, int32_t score) {
+  if (rows < 0 || experts < 1 || experts > ROUTER_MAX_EXPERTS || ld < experts)
+    return fail(B200MOE_E_SHAPE, "%s: rows %lld, experts %d (at most %d), pitch %lld", op, (long long)rows, experts, ROUTER_MAX_EXPERTS, (long long)ld);
+  if (topk < 1 || topk > experts || topk > ROUTER_MAX_TOPK) return fail(B200MOE_E_SHAPE, "%s: topk %d (1 to %d, at most the experts)", op, topk, ROUTER_MAX_TOPK);
+  if (dtype != B200MOE_DTYPE_F32 && dtype != B200MOE_DTYPE_BF16 && dtype != B200MOE_DTYPE_F16) return fail(B200MOE_E_UNSUPPORTED, "%s: dtype %d", op, dtype);
+  if (score != B200MOE_SCORE_SOFTMAX && score != B200MOE_SCORE_SIGMOID) return fail(B200MOE_E_UNSUPPORTED, "%s: score function %d", op, score);
+  if (rows > 0x3fffffff8ll) return fail(B200MOE_E_SHAPE, "%s: too many rows", op);
+  if (rows > 0 && !logits) return fail(B200MOE_E_NULL, "%s: logits are required", op);
+  return B200MOE_OK;
+}
+
+template <int kPerLane>
+static void router_launch(const void* logits, int dtype, int64_t rows, int experts, int64_t ld, const float* bias, int topk, int sigmoid, int normalize,
+                          float scale, float* weights, int32_t* ids, cudaStream_t stream) {
+  const unsigned grid = (unsigned)((rows + 7) / 8);
+  if (bias) router_topk_kernel<kPerLane, true><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, weights, ids);
+  else router_topk_kernel<kPerLane, false><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, weights, ids);
+}
+
+}  // namespace b200moe
+
+using namespace b200moe;
+
+extern "C" int b200moe_router_topk(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld, const float* bias, int32_t topk,
+                                   int32_t score, int32_t normalize, float scale, float* weights, int32_t* ids, void* stream_v) {
+  int rc = router_check("router_topk", logits, dtype, rows, experts, ld, topk, score);
+  if (rc || rows == 0) return rc;
+  if (!weights || !ids) return fail(B200MOE_E_NULL, "router_topk: weights and ids are required");
+  cudaStream_t stream = (cudaStream_t)stream_v;
+  const int sig = score == B200MOE_SCORE_SIGMOID;
+#define B200_ROUTER(V) router_launch<V>(logits, dtype, rows, experts, ld, bias, topk, sig, normalize != 0, scale, weights, ids, stream)
+  if (experts <= 32) B200_ROUTER(1);
+  else if (experts <= 64) B200_ROUTER(2);
+  else if (experts <= 128) B200_ROUTER(4);
+  else if (experts <= 256) B200_ROUTER(8);
+  else if (experts <= 512) B200_ROUTER(16);
+  else B200_ROUTER(32);
+#undef B200_ROUTER
+  B200_CUDA_CHECK(cudaGetLastError());
+  return B200MOE_OK;
+}
+
+extern "C" int b200moe_router_topk_backward(const float* dweights, const void* logits, int32_t dtype, const int32_t* ids, int64_t rows, int32_t experts,
+                                            int64_t ld, int32_t topk, int32_t score, int32_t normalize, float scale, void* dlogits, void* stream_v) {
+  int rc = router_check("router_topk_backward", logits, dtype, rows, experts, ld, topk, score);
+  if (rc || rows == 0) return rc;
+  if (!dweights || !ids || !dlogits) return fail(B200MOE_E_NULL, "router_topk_backward: dweights, ids and dlogits are required");
+  router_grad_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream_v>>>(dweights, logits, dtype, ids, rows, experts, ld, topk,
+                                                                                     score == B200MOE_SCORE_SIGMOID, normalize != 0, scale, dlogits);
+  B200_CUDA_CHECK(cudaGetLastError());
+  return B200MOE_OK;
+}

@@ -1,0 +1,182 @@
+"""Dense 16-bit operators that stand next to the grouped GEMMs of an MoE layer.
+
+``gated_ffn`` is the block of a shared (or dense) expert, the counterpart of the grouped FC1
+(:mod:`.grouped_gemm_glu`) for weights that every token passes: both projections, the activation and the
+product in one kernel.  ``linear`` is the projection behind it or the router's, with bias, activation and
+residual in its epilogue.  Both have their backward pass.  The reference has no counterpart.
+
+All functions take bf16 or fp16 tensors ``[rows, cols]`` with contiguous rows (any pitch that is a multiple
+of 8 elements, 16-byte aligned, for what a tensor map reads: ``x`` and the weights), sum in float32 and round
+once.  They allocate their outputs and launch on ``stream`` (default: the current stream of the tensors' device); when
+another stream is passed, outputs and workspace belong to that stream.  They are not recorded by autograd:
+the backward functions are called explicitly, as with the grouped GEMMs.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .ops import on_stream
+
+_TYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_GLU = {"swiglu": _lib.ACT_SWIGLU, "geglu": _lib.ACT_GEGLU}
+_ACT = {None: _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
+
+
+def _check_x(x: torch.Tensor) -> Tuple[int, int]:
+    if not x.is_cuda:
+        raise ValueError("all tensors must live on a CUDA device")
+    if x.dtype not in _TYPES:
+        raise NotImplementedError(f"x dtype {x.dtype} is not built (bf16 and fp16 are)")
+    if x.dim() != 2:
+        raise ValueError(f"x must be a 2-D tensor [tokens, k], got shape {tuple(x.shape)}")
+    return x.shape
+
+
+def _pitch(name: str, t: torch.Tensor, shape, dtype, device) -> int:
+    """Row pitch of a ``shape`` tensor with contiguous rows."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} lives on {t.device}, x on {device}")
+    rows, cols = shape
+    if cols > 1 and rows > 0 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    # the pitch of a single row is free: the next multiple of 8
+    return t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
+
+
+def _weight(name: str, w: torch.Tensor, k: int, x: torch.Tensor) -> int:
+    if w.dim() != 2 or w.shape[1] != k:
+        raise ValueError(f"{name} must have shape [n, {k}], got {tuple(w.shape)}")
+    return _pitch(name, w, tuple(w.shape), x.dtype, x.device)
+
+
+def _launch(fn: str, args: _lib.DenseArgs, stream: int) -> None:
+    _lib.check(getattr(_lib.load(), fn)(ctypes.byref(args), stream))
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_func: str = "swiglu", return_preact: bool = False, stream=None):
+    """``act(x w_gate^T) * (x w_up^T)``: ``x [tokens, k]``, weights ``[n, k]`` -> ``h [tokens, n]``, and with
+    ``return_preact`` also ``gate`` and ``up`` (what :func:`gated_ffn_backward` reads).
+
+    ``act_func`` as in the grouped FC1: ``"swiglu"`` = ``gate * sigmoid(gate) * up``, ``"geglu"`` = the reference's
+    GeGLU, ``gate <= 7``, ``-7 <= up <= 7``, ``(up + 1) * gate * sigmoid(1.702 * gate)`` (gate and up are returned
+    without the limits)."""
+    m, k = _check_x(x)
+    if act_func not in _GLU:
+        raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
+    ld_x = _pitch("x", x, (m, k), x.dtype, x.device)
+    ld_g, ld_u = _weight("w_gate", w_gate, k, x), _weight("w_up", w_up, k, x)
+    if w_up.shape != w_gate.shape:
+        raise ValueError("w_gate and w_up must have equal shapes")
+    n = w_gate.shape[0]
+    with on_stream(x.device, stream) as s:
+        h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        gate = up = None
+        if return_preact:
+            gate, up = torch.empty_like(h), torch.empty_like(h)
+        t = _TYPES[x.dtype]
+        _launch("b200moe_gated_ffn", _lib.DenseArgs(
+            x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), y=h.data_ptr(), pre0=gate.data_ptr() if return_preact else None,
+            pre1=up.data_ptr() if return_preact else None, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g, ld_w1=ld_u, ld_y=n, ld_pre0=n, ld_pre1=n,
+            dtype=t, y_dtype=t, act=_GLU[act_func]), s)  # fmt: skip
+    return (h, gate, up) if return_preact else h
+
+
+def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
+                       act_func: str = "swiglu", stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+    """Backward pass of :func:`gated_ffn` from ``dh [tokens, n]`` and the saved ``gate`` and ``up``: returns
+    ``(dx, dw_gate, dw_up)``.  A value that GeGLU limits has no gradient."""
+    m, k = _check_x(x)
+    if act_func not in _GLU:
+        raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
+    ld_x = _pitch("x", x, (m, k), x.dtype, x.device)
+    ld_g, ld_u = _weight("w_gate", w_gate, k, x), _weight("w_up", w_up, k, x)
+    if w_up.shape != w_gate.shape:
+        raise ValueError("w_gate and w_up must have equal shapes")
+    n = w_gate.shape[0]
+    lds = [_pitch(name, v, (m, n), x.dtype, x.device) for name, v in (("dh", dh), ("gate", gate), ("up", up))]
+    with on_stream(x.device, stream) as s:
+        dx = torch.empty((m, k), dtype=x.dtype, device=x.device)
+        dw_gate, dw_up = torch.empty((n, k), dtype=x.dtype, device=x.device), torch.empty((n, k), dtype=x.dtype, device=x.device)
+        need = _lib.load().b200moe_dense_workspace_bytes(m, n, 1)
+        work = torch.empty(need, dtype=torch.uint8, device=x.device)
+        t = _TYPES[x.dtype]
+        _launch("b200moe_gated_ffn_backward", _lib.DenseArgs(
+            x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), dy=dh.data_ptr(), pre0=gate.data_ptr(), pre1=up.data_ptr(), dx=dx.data_ptr(),
+            dw0=dw_gate.data_ptr(), dw1=dw_up.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g,
+            ld_w1=ld_u, ld_dy=lds[0], ld_pre0=lds[1], ld_pre1=lds[2], dtype=t, y_dtype=t, act=_GLU[act_func]), s)  # fmt: skip
+    return dx, dw_gate, dw_up
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act_func: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, return_preact: bool = False, stream=None):  # fmt: skip
+    """``act(x weight^T + bias) + residual``: ``x [tokens, k]``, ``weight [n, k]``, ``bias [n]`` (x's type or float32),
+    ``residual [tokens, n]`` (x's type; a pitch of 0, one row for every token, included) -> ``[tokens, n]`` of
+    ``out_dtype`` (x's type, or float32, which is then exact to float32 rounding).  ``act_func``: ``None``, ``"relu"``,
+    ``"silu"`` or ``"gelu"`` (the error-function form).  With ``return_preact`` the result is ``(y, x weight^T + bias)``,
+    the second in x's type, for :func:`linear_backward`."""
+    m, k = _check_x(x)
+    if act_func not in _ACT:
+        raise ValueError(f"act_func must be None, 'relu', 'silu' or 'gelu', got {act_func!r}")
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise NotImplementedError(f"out_dtype {out_dtype} is not built for {x.dtype} inputs (their own type and float32 are)")
+    ld_x = _pitch("x", x, (m, k), x.dtype, x.device)
+    ld_w = _weight("weight", weight, k, x)
+    n = weight.shape[0]
+    if bias is not None:
+        if tuple(bias.shape) != (n,) or bias.device != x.device or (n > 1 and bias.stride(0) != 1):
+            raise ValueError(f"bias must be a contiguous [{n}] tensor on {x.device}")
+        if bias.dtype not in (x.dtype, torch.float32):
+            raise NotImplementedError(f"bias dtype {bias.dtype} is not built for {x.dtype} inputs (their own type and float32 are)")
+    ld_r = 0 if residual is None else _pitch("residual", residual, (m, n), x.dtype, x.device)
+    with on_stream(x.device, stream) as s:
+        y = torch.empty((m, n), dtype=out_dtype, device=x.device)
+        z = torch.empty((m, n), dtype=x.dtype, device=x.device) if return_preact else None
+        t = _TYPES[x.dtype]
+        _launch("b200moe_linear", _lib.DenseArgs(
+            x=x.data_ptr(), w0=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
+            residual=None if residual is None else residual.data_ptr(), y=y.data_ptr(), pre0=z.data_ptr() if return_preact else None, m=m, n=n, k=k,
+            ld_x=ld_x, ld_w0=ld_w, ld_residual=ld_r, ld_y=n, ld_pre0=n, dtype=t, y_dtype=_lib.DTYPE_F32 if out_dtype == torch.float32 else t,
+            bias_dtype=t if bias is None or bias.dtype == x.dtype else _lib.DTYPE_F32, act=_ACT[act_func]), s)  # fmt: skip
+    return (y, z) if return_preact else y
+
+
+def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, preact: Optional[torch.Tensor] = None, act_func: Optional[str] = None,
+                    bias_grad: bool = False, stream=None) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:  # fmt: skip
+    """Backward pass of :func:`linear` from ``dy [tokens, n]`` (x's type or float32): returns ``(dx, dweight, dbias)``,
+    ``dbias`` float32 or ``None``.  ``preact`` is the saved pre-activation (needed with an activation).  The residual's
+    gradient is ``dy`` itself."""
+    m, k = _check_x(x)
+    if act_func not in _ACT:
+        raise ValueError(f"act_func must be None, 'relu', 'silu' or 'gelu', got {act_func!r}")
+    ld_x = _pitch("x", x, (m, k), x.dtype, x.device)
+    ld_w = _weight("weight", weight, k, x)
+    n = weight.shape[0]
+    if dy.dtype not in (x.dtype, torch.float32):
+        raise NotImplementedError(f"dy dtype {dy.dtype} is not built for {x.dtype} inputs (their own type and float32 are)")
+    ld_dy = _pitch("dy", dy, (m, n), dy.dtype, x.device)
+    ld_z = 0
+    if act_func is not None:
+        if preact is None:
+            raise ValueError("preact is required with an activation")
+        ld_z = _pitch("preact", preact, (m, n), x.dtype, x.device)
+    with on_stream(x.device, stream) as s:
+        dx, dw = torch.empty((m, k), dtype=x.dtype, device=x.device), torch.empty((n, k), dtype=x.dtype, device=x.device)
+        db = torch.empty((n,), dtype=torch.float32, device=x.device) if bias_grad else None
+        need = _lib.load().b200moe_dense_workspace_bytes(m, n, 0)
+        work = torch.empty(need, dtype=torch.uint8, device=x.device)
+        t = _TYPES[x.dtype]
+        _launch("b200moe_linear_backward", _lib.DenseArgs(
+            x=x.data_ptr(), w0=weight.data_ptr(), dy=dy.data_ptr(), pre0=None if act_func is None else preact.data_ptr(), dx=dx.data_ptr(),
+            dw0=dw.data_ptr(), dbias=None if db is None else db.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x,
+            ld_w0=ld_w, ld_dy=ld_dy, ld_pre0=ld_z, dtype=t, y_dtype=_lib.DTYPE_F32 if dy.dtype == torch.float32 else t, act=_ACT[act_func]), s)  # fmt: skip
+    return dx, dw, db

@@ -12,7 +12,69 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _stream_ptr
+from .ops import _stream_ptr, on_stream
+
+_LOGIT_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _check_logits(logits: torch.Tensor, score_func: str) -> int:
+    """Row pitch of the router's logits."""
+    if not logits.is_cuda or logits.dim() != 2:
+        raise ValueError("logits must be a 2-D CUDA tensor [tokens, experts]")
+    if logits.dtype not in _LOGIT_TYPES:
+        raise NotImplementedError(f"logits dtype {logits.dtype} is not built (float32, bf16 and fp16 are)")
+    if score_func not in _SCORES:
+        raise ValueError(f"score_func must be 'softmax' or 'sigmoid', got {score_func!r}")
+    t, e = logits.shape
+    if e > 1 and t > 0 and logits.stride(1) != 1:
+        raise ValueError("logits must have contiguous rows")
+    return logits.stride(0) if t > 1 else e
+
+
+def router_topk(logits: torch.Tensor, topk: int, score_func: str = "softmax", normalize: bool = True, bias: Optional[torch.Tensor] = None,
+                scale: float = 1.0, stream=None) -> Tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+    """The gate in front of :func:`route`: ``logits [T, E]`` -> ``(weights [T, topk] float32, ids [T, topk] int32)``.
+
+    Chosen are the ``topk`` largest logits of a row or, with ``bias [E]`` float32, the largest ``score + bias``
+    (decided in 64 bits), in falling order and ties to the lowest index.  A logit of -inf is never chosen; a slot left
+    without an expert gets id -1, which :func:`route` skips, and weight 0.  NaN sorts above everything.  The weights are
+    ``scale * score`` with ``score_func`` softmax over the row or sigmoid, with ``normalize`` divided by the sum of the
+    chosen scores; the bias decides the choice only.  ``E <= 1024``, ``topk <= 32``."""
+    ld = _check_logits(logits, score_func)
+    t, e = logits.shape
+    if bias is not None and (tuple(bias.shape) != (e,) or bias.dtype != torch.float32 or bias.device != logits.device or (e > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"bias must be a contiguous float32 [{e}] tensor on {logits.device}")
+    with on_stream(logits.device, stream) as s:
+        weights = torch.empty((t, topk), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((t, topk), dtype=torch.int32, device=logits.device)
+        rc = _lib.load().b200moe_router_topk(
+            logits.data_ptr(), _LOGIT_TYPES[logits.dtype], t, e, ld, None if bias is None else bias.data_ptr(), topk, _SCORES[score_func], int(normalize),
+            scale, weights.data_ptr(), ids.data_ptr(), s,
+        )  # fmt: skip
+        _lib.check(rc)
+    return weights, ids
+
+
+def router_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, score_func: str = "softmax", normalize: bool = True,
+                         scale: float = 1.0, stream=None) -> torch.Tensor:  # fmt: skip
+    """Backward pass of :func:`router_topk`: ``dweights [T, topk]`` float32 (what the gated GEMMs return as the gradient of
+    the gate probabilities) -> ``dlogits [T, E]`` of the logits' type.  Slots with id -1 have no part; the choice itself has no
+    gradient."""
+    ld = _check_logits(logits, score_func)
+    t, e = logits.shape
+    if ids.dim() != 2 or ids.shape[0] != t or ids.dtype != torch.int32 or ids.device != logits.device or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 [{t}, topk] tensor on {logits.device}")
+    if dweights.shape != ids.shape or dweights.dtype != torch.float32 or dweights.device != logits.device or not dweights.is_contiguous():
+        raise ValueError(f"dweights must be a contiguous float32 tensor of the ids' shape on {logits.device}")
+    with on_stream(logits.device, stream) as s:
+        dlogits = torch.empty((t, e), dtype=logits.dtype, device=logits.device)
+        rc = _lib.load().b200moe_router_topk_backward(
+            dweights.data_ptr(), logits.data_ptr(), _LOGIT_TYPES[logits.dtype], ids.data_ptr(), t, e, ld, ids.shape[1], _SCORES[score_func], int(normalize),
+            scale, dlogits.data_ptr(), s,
+        )  # fmt: skip
+        _lib.check(rc)
+    return dlogits
 
 
 def route(expert_ids: torch.Tensor, num_experts: int, m_aligned: int = 128, stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -41,6 +41,11 @@ extern "C" {
 
 #define B200MOE_ACT_SWIGLU 0
 #define B200MOE_ACT_GEGLU 1
+/* activations of b200moe_linear */
+#define B200MOE_ACT_NONE 2
+#define B200MOE_ACT_RELU 3
+#define B200MOE_ACT_SILU 4
+#define B200MOE_ACT_GELU 5 /* z/2 erfc(-z/sqrt 2) */
 
 /* flags */
 #define B200MOE_FLAG_DISCRETE_COL_SFD 1 /* per-expert column scale-factor blocks */
@@ -361,6 +366,87 @@ int b200moe_peer_alloc(int64_t bytes, void** ptr, void* handle64);
 int b200moe_peer_open(const void* handle64, void** ptr);
 int b200moe_peer_close(void* ptr);
 int b200moe_peer_free(void* ptr);
+
+/*
+ * Dense 16-bit operators next to the grouped GEMMs (no reference counterpart): the gated feed-forward block of a
+ * shared or dense expert, and the projection with its epilogue, each with its backward pass.
+ *
+ *   b200moe_gated_ffn           y = act(g) * u with g = x w0^T, u = x w1^T (act SWIGLU / GEGLU as in b200moe_fc1_swiglu,
+ *                               without prob); pre0, pre1 (outputs, both or none) receive g and u
+ *   b200moe_gated_ffn_backward  dy = gradient of y; pre0, pre1 (inputs) = g, u:
+ *                               dx = dg w0 + du w1, dw0 = dg^T x, dw1 = du^T x (dx, or dw0 and dw1, may be NULL)
+ *   b200moe_linear              y = act(z) + residual with z = x w0^T + bias; pre0 (output, optional) receives z
+ *   b200moe_linear_backward     dz = dy act'(pre0) (pre0 is not read with ACT_NONE); dx = dz w0, dw0 = dz^T x,
+ *                               dbias [n] float32 = column sums of dz (each may be NULL)
+ *
+ * x [m, k], w0 / w1 [n, k], y / dy / residual / pre0 / pre1 [m, n], dx [m, k], dw0 / dw1 [n, k].  Rows are contiguous; ld_* is
+ * the pitch of a row in elements (dx, dw0, dw1 are dense).  x, w0 and w1 must start on 16-byte boundaries with pitches of a multiple
+ * of 8, and k must be a multiple of 8; m and n may be anything, m == 0 included (the weights' gradients are then zero).
+ * dtype: B200MOE_DTYPE_BF16 or _F16, of every 16-bit tensor.  y_dtype: dtype, or (linear) B200MOE_DTYPE_F32, of y and
+ * dy.  bias_dtype: dtype or F32.  The backward passes need b200moe_dense_workspace_bytes(m, n, gated) bytes, 16-byte
+ * aligned; what it holds before and after a call means nothing.  Products are summed in float32; results do not depend on
+ * timing.
+ */
+typedef struct b200moe_dense_args {
+  const void* x;
+  const void* w0;
+  const void* w1;
+  const void* bias;
+  const void* residual;
+  const void* dy;
+  void* y;
+  void* pre0;
+  void* pre1;
+  void* dx;
+  void* dw0;
+  void* dw1;
+  float* dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int64_t ld_x;
+  int64_t ld_w0;
+  int64_t ld_w1;
+  int64_t ld_residual;
+  int64_t ld_dy;
+  int64_t ld_y;
+  int64_t ld_pre0;
+  int64_t ld_pre1;
+  int32_t dtype;
+  int32_t y_dtype;
+  int32_t bias_dtype;
+  int32_t act;
+  int32_t wait_limit_ms; /* as in b200moe_gemm_args */
+} b200moe_dense_args;
+int b200moe_gated_ffn(const b200moe_dense_args* args, void* stream);
+int b200moe_gated_ffn_backward(const b200moe_dense_args* args, void* stream);
+int b200moe_linear(const b200moe_dense_args* args, void* stream);
+int b200moe_linear_backward(const b200moe_dense_args* args, void* stream);
+int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t gated);
+
+/*
+ * The gate in front of the experts (no reference counterpart; the ids go to b200moe_route, the weights to the GEMMs' prob).
+ *
+ * b200moe_router_topk: logits [rows, experts] (dtype F32 / BF16 / F16, row pitch ld) -> ids [rows, topk] int32 and
+ *   weights [rows, topk] f32.  Chosen are the topk largest logits of a row, or with bias [experts] f32 the topk largest
+ *   score(l) + bias (formed in 64 bits), in falling order, ties to the lowest index.  A logit of -inf is never chosen; a
+ *   slot left without an expert gets id -1 (which b200moe_route skips) and weight 0.  NaN sorts above everything.  Weights:
+ *   scale * score of the chosen (the bias has no part in it), with normalize divided by the chosen scores' sum; score =
+ *   softmax over the row or sigmoid.
+ * b200moe_router_topk_backward: dlogits [rows, experts] (dense, dtype) from dweights [rows, topk] f32, the logits and
+ *   the ids; entries with an id outside [0, experts) have no part.  The choice itself has no gradient.
+ * experts <= 1024, topk <= 32.
+ */
+#define B200MOE_SCORE_SOFTMAX 0
+#define B200MOE_SCORE_SIGMOID 1
+int b200moe_router_topk(const void* logits, int32_t dtype, int64_t rows, int32_t experts, int64_t ld, const float* bias,
+                        int32_t topk, int32_t score, int32_t normalize, float scale, float* weights, int32_t* ids,
+                        void* stream);
+int b200moe_router_topk_backward(const float* dweights, const void* logits, int32_t dtype, const int32_t* ids,
+                                 int64_t rows, int32_t experts, int64_t ld, int32_t topk, int32_t score,
+                                 int32_t normalize, float scale, void* dlogits, void* stream);
 
 /* Last error text of the calling thread ("" if none).  Never NULL. */
 const char* b200moe_last_error(void);
