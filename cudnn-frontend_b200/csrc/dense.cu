@@ -481,6 +481,344 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
 }
 
 // ---------------------------------------------------------------------------------------
+// Large products: a persistent kernel of CTA pairs, one pair per two SMs.  A tile is 256 x 256 (cta_group::2: each CTA
+// holds 128 rows of A, 128 columns of B and the accumulator of its 128 rows), its two accumulators of 256 columns fill
+// TMEM, so the epilogue of one tile runs beside the products of the next.  Rows are tokens (or, for a weight's gradient,
+// the weight's rows), so a thread of the epilogue holds 32 neighbouring columns of one output row.
+//
+// DENSE_GLU: the pair's first CTA loads 128 rows of the gate weights as its half of B, the second the same rows of the up
+// weights: accumulator columns [0, 128) are the gate, [128, 256) the up projection of the same 128 features.
+//
+// A launch walks one or two jobs (the two gradient products of a backward pass share a launch: the tiles of the second fill
+// the last wave of the first).  Tiles are dealt out in rounds; where the last round of job 0 leaves pairs idle, they
+// begin job 1 `early` rounds sooner.
+//
+// warps: 0 producer, 1 MMA issuer (first CTA) and TMEM owner, 2-9 epilogue (TMEM lane quarter x column half)
+// ---------------------------------------------------------------------------------------
+constexpr int PAIR_THREADS = 320;
+constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_STAGE_BYTES = 2 * DENSE_A_BYTES;
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
+constexpr int PAIR_EPI_WARPS = 8;
+constexpr int ST_PAIR_EMPTY = 411, ST_PAIR_FULL = 412, ST_PAIR_ACC_EMPTY = 413, ST_PAIR_ACC_FULL = 414, ST_PAIR_DRAIN = 415;
+
+struct PairJob {
+  int rows, cols;
+  int row_tiles, col_tiles;   // row_tiles of one result; twice as many with `stacked`
+  int k_tiles, chain_tiles;
+  int a_mn, b_mn, stacked;
+  int tiles;
+  int raster;                 // row tiles of a raster group: the group's rows of A stay in L2 while its columns pass
+  uint32_t idesc;
+  int vec;                    // output (and residual, pre-activation) rows may be accessed 16 bytes at a time
+  void* out[2];
+  int64_t ld_out;
+};
+
+struct PairParams {
+  PairJob job[2];
+  int jobs;
+  int full_rounds, rest;      // job 0: every pair takes full_rounds tiles, the first `rest` pairs one more
+  int early, early_tiles;     // rounds (and tiles) of job 1 that the other pairs take before all join
+  int act, f16, out_f32, bias_f32;
+  void* pre[2];
+  int64_t ld_pre[2];
+  const void* bias;
+  const void* residual;
+  int64_t ld_res;
+  uint64_t wait_limit_ns;
+};
+
+struct PairMaps {
+  DenseMaps job[2];
+};
+
+struct PairTile {
+  int job, row_tile, col_tile, which;
+};
+
+// the i-th tile of a pair; false when it has no more
+__device__ __forceinline__ bool pair_tile(const PairParams& p, int pair, int pairs, int i, PairTile& t) {
+  int idx;
+  const int mine = p.full_rounds + (pair < p.rest ? 1 : 0);
+  if (i < mine) {
+    t.job = 0;
+    idx = pair + i * pairs;
+  } else {
+    if (p.jobs < 2) return false;
+    t.job = 1;
+    i -= mine;
+    const int early = p.rest > 0 && pair >= p.rest ? p.early : 0;
+    if (i < early) {
+      idx = i * (pairs - p.rest) + pair - p.rest;
+      if (idx >= p.early_tiles) return false;
+    } else {
+      idx = p.early_tiles + (i - early) * pairs + pair;
+      if (idx >= p.job[1].tiles) return false;
+    }
+  }
+  const PairJob& j = p.job[t.job];
+  const int rows = j.row_tiles * (j.stacked ? 2 : 1);
+  const int group = idx / (j.raster * j.col_tiles);
+  const int in = idx - group * j.raster * j.col_tiles;
+  const int height = min(j.raster, rows - group * j.raster);
+  t.col_tile = in / height;
+  t.row_tile = group * j.raster + in - t.col_tile * height;
+  t.which = t.row_tile >= j.row_tiles ? 1 : 0;
+  t.row_tile -= t.which * j.row_tiles;
+  return true;
+}
+
+// the activation on 32 values: one uniform branch, so that v[] stays in registers
+__device__ __forceinline__ void act_x32(float* v, int act) {
+  if (act == B200MOE_ACT_RELU) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_RELU);
+  } else if (act == B200MOE_ACT_SILU) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_SILU);
+  } else if (act == B200MOE_ACT_GELU) {
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_GELU);
+  }
+}
+
+// 32 values to 16-bit memory
+__device__ __forceinline__ void store16x32(void* base, int64_t o, const float* v, int count, bool f16, bool vec) {
+  uint16_t* d = reinterpret_cast<uint16_t*>(base) + o;
+  if (vec && count >= 32) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float* w = v + 8 * q;
+      reinterpret_cast<uint4*>(d)[q] = make_uint4(pack16x2_from_float(w[0], w[1], f16), pack16x2_from_float(w[2], w[3], f16),
+                                                  pack16x2_from_float(w[4], w[5], f16), pack16x2_from_float(w[6], w[7], f16));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < count) store16(base, o + j, v[j], f16);
+  }
+}
+
+template <int kEpi>
+__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
+    dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t s_bars[2 * PAIR_STAGES + 4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t bars = smem_u32(s_bars);
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (PAIR_STAGES + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (2 * PAIR_STAGES + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * PAIR_STAGES + 2 + b); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitCtx wc = {&s_abort, p.wait_limit_ns};
+  const int rank = (int)cluster_ctarank();
+  const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PAIR_STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 2 * PAIR_EPI_WARPS);
+    }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&s_tmem), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();  // both CTAs' barriers exist before either is signalled
+  cluster_wait();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0) {
+    // ---- producer: this CTA's halves of A and B; every copy is credited to the first CTA's barrier --------------
+    const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    bool ok = true;
+    PairTile t;
+    for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
+      const PairJob& j = p.job[t.job];
+      const DenseMaps& m = maps.job[t.job];
+      const int a0 = t.row_tile * 256 + rank * 128;
+      const int b0 = kEpi == DENSE_GLU ? t.col_tile * 128 : t.col_tile * 256 + rank * 128;
+      const bool a_mn = j.a_mn != 0, b_mn = j.b_mn != 0;
+      for (int kt = 0; kt < j.k_tiles; ++kt) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, wc, ST_PAIR_EMPTY))) { ok = false; break; }
+        if (elect_one()) {
+          const int chain = kt >= j.chain_tiles ? 1 : 0;
+          const int kc = (kt - chain * j.chain_tiles) * DENSE_BK;
+          const uint32_t fb = leader_full0 + 8u * stage;
+          const uint32_t da = ring + stage * PAIR_STAGE_BYTES, db = da + DENSE_A_BYTES;
+          const CUtensorMap* ma = &m.a[chain | t.which];
+          const CUtensorMap* mb = &m.b[kEpi == DENSE_GLU ? rank : chain];
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * PAIR_STAGE_BYTES);
+          if (a_mn) {
+            tma_load_2d_pair(da, ma, fb, a0, kc);
+            tma_load_2d_pair(da + DENSE_SLAB, ma, fb, a0 + 64, kc);
+          } else {
+            tma_load_2d_pair(da, ma, fb, kc, a0);
+          }
+          if (b_mn) {
+            tma_load_2d_pair(db, mb, fb, b0, kc);
+            tma_load_2d_pair(db + DENSE_SLAB, mb, fb, b0 + 64, kc);
+          } else {
+            tma_load_2d_pair(db, mb, fb, kc, b0);
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+      }
+    }
+    if (!ok && rank == 0) {
+      // a wait gave up: the copies of both CTAs are credited here; wait (with a limit) until they have landed.  The second
+      // CTA ends after the cluster barrier below, so its shared memory outlives them too.
+      for (int i = max(0, issued - PAIR_STAGES); i < issued; ++i) mbar_wait(full_bar(i % PAIR_STAGES), (uint32_t)(i / PAIR_STAGES) & 1u, wc, ST_PAIR_DRAIN);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---- MMA issuer -------------------------------------------------------------------------------------
+    if (rank == 0) {
+      constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);  // SBO 1024, version 1, 128-byte swizzle
+      const uint32_t a_base = (ring >> 4) & 0x3FFFu, b_base = ((ring + DENSE_A_BYTES) >> 4) & 0x3FFFu;
+      auto desc = [](uint32_t lo) { return ((uint64_t)HI << 32) | lo; };
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      PairTile t;
+      for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
+        const PairJob& j = p.job[t.job];
+        const uint32_t acc = tmem + (uint32_t)(i & 1) * 256u;
+        const uint32_t a_lo0 = a_base | (j.a_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
+        const uint32_t b_lo0 = b_base | (j.b_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
+        const uint32_t a_step = j.a_mn ? (16u * 128u) >> 4 : 2u, b_step = j.b_mn ? (16u * 128u) >> 4 : 2u;
+        const uint32_t idesc = j.idesc;
+        const int k_tiles = j.k_tiles;
+        if (i >= 2) {
+          if (!__all_sync(0xffffffffu, mbar_wait(acc_empty_bar(i & 1), (uint32_t)((i >> 1) - 1) & 1u, wc, ST_PAIR_ACC_EMPTY))) { ok = false; break; }
+          tc_fence_after();
+        }
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          bool landed = mbar_try_wait(full_bar(stage), phase);
+          if (!landed) landed = mbar_wait(full_bar(stage), phase, wc, ST_PAIR_FULL);
+          if (!__all_sync(0xffffffffu, landed)) { ok = false; break; }
+          if (elect_one()) {
+            const uint32_t a_lo = a_lo0 + stage * (PAIR_STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (PAIR_STAGE_BYTES >> 4);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mma_f16_ss<true>(acc, desc(a_lo + q * a_step), desc(b_lo + q * b_step), idesc, (kt | q) != 0);
+            tc_commit_pair(empty_bar(stage), 3);
+            if (kt + 1 == k_tiles) tc_commit_pair(acc_full_bar(i & 1), 3);
+          }
+          __syncwarp();
+          if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- epilogue ---------------------------------------------------------------------------------------
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const bool f16 = p.f16 != 0;
+    PairTile t;
+    for (int i = 0; pair_tile(p, pair, pairs, i, t); ++i) {
+      const PairJob& j = p.job[t.job];
+      const int row = t.row_tile * 256 + rank * 128 + quarter * 32 + lane;
+      const bool row_ok = row < j.rows;
+      const bool vec = j.vec != 0;
+      if (!__all_sync(0xffffffffu, mbar_wait<true>(acc_full_bar(i & 1), (uint32_t)(i >> 1) & 1u, wc, ST_PAIR_ACC_FULL))) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)(i & 1) * 256u + ((uint32_t)(quarter * 32) << 16);
+      constexpr int kChunks = kEpi == DENSE_GLU ? 2 : 4;
+#pragma unroll 1
+      for (int c = 0; c < kChunks; ++c) {
+        __syncwarp();
+        float v[32], u[kEpi == DENSE_GLU ? 32 : 1];
+        const int in_tile = half * (kChunks * 32) + c * 32;
+        tmem_ld_32x32(acc + in_tile, v);
+        if constexpr (kEpi == DENSE_GLU) tmem_ld_32x32(acc + 128 + in_tile, u);
+        const int col = t.col_tile * (kEpi == DENSE_GLU ? 128 : 256) + in_tile;
+        const int count = row_ok ? min(32, j.cols - col) : 0;  // columns of this chunk that exist
+        tmem_ld_wait();
+        reg_fence32(v);
+        if constexpr (kEpi == DENSE_GLU) reg_fence32(u);
+        if (c == kChunks - 1) {
+          // the accumulator is in registers: the issuer may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar(i & 1), 0));
+        }
+        if (count <= 0) continue;
+        const int64_t o = (int64_t)row * j.ld_out + col;
+        if constexpr (kEpi == DENSE_GLU) {
+          if (p.pre[0]) {
+            store16x32(p.pre[0], (int64_t)row * p.ld_pre[0] + col, v, count, f16, vec);
+            store16x32(p.pre[1], (int64_t)row * p.ld_pre[1] + col, u, count, f16, vec);
+          }
+#pragma unroll
+          for (int q = 0; q < 32; ++q) v[q] = glu_f(v[q], u[q], p.act);
+          store16x32(j.out[0], o, v, count, f16, vec);
+        } else if constexpr (kEpi == DENSE_LINEAR) {
+          if (p.bias) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              if (q < count) v[q] += p.bias_f32 ? __ldg(reinterpret_cast<const float*>(p.bias) + col + q) : load16(p.bias, col + q, f16);
+          }
+          if (p.pre[0]) store16x32(p.pre[0], (int64_t)row * p.ld_pre[0] + col, v, count, f16, vec);
+          act_x32(v, p.act);
+          if (p.residual) {
+            const int64_t ro = (int64_t)row * p.ld_res + col;
+            if (vec && count >= 32) {
+              const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.residual) + ro);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint4 w = __ldg(src + q);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack16x2(ws[e], f16);
+                  v[8 * q + 2 * e] += f.x;
+                  v[8 * q + 2 * e + 1] += f.y;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 32; ++q)
+                if (q < count) v[q] += load16(p.residual, ro + q, f16);
+            }
+          }
+          store16x32(j.out[0], o, v, count, f16, vec);
+        } else {
+          store16x32(j.out[t.which], o, v, count, f16, vec);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();  // the other CTA's arrivals and the issuer's products reach this CTA until both are here
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
 // Elementwise parts of the backward passes: one read of the incoming gradient and of the saved pre-activations, one
 // write of the operand that the two gradient products share, with its rows padded to 8 values so that TMA can read it.
 // ---------------------------------------------------------------------------------------
@@ -717,6 +1055,82 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+template <int kEpi>
+static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pairs, cudaStream_t stream) {
+  auto kern = dense_pair_kernel<kEpi>;
+  static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+  int dev = 0;
+  B200_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
+    ready.fetch_or(1ull << (dev & 63));
+  }
+  kern<<<(unsigned)(2 * pairs), PAIR_THREADS, PAIR_SMEM, stream>>>(maps, p);
+  B200_CUDA_CHECK(cudaGetLastError());
+  return B200MOE_OK;
+}
+
+// One launch of the pair kernel over one or two products of the same epilogue; operand A's rows are the result's rows.
+// `p` arrives with its epilogue fields and each job's outputs, pitch and `vec` set.
+static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceInfo* di, cudaStream_t stream) {
+  PairMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  p.jobs = jobs;
+  for (int i = 0; i < jobs; ++i) {
+    PairJob& j = p.job[i];
+    j.rows = (int)g[i].rows;
+    j.cols = (int)g[i].cols;
+    j.row_tiles = (int)((g[i].rows + 255) / 256);
+    const int tile_cols = g[i].dual ? 128 : 256;
+    j.col_tiles = (int)((g[i].cols + tile_cols - 1) / tile_cols);
+    j.chain_tiles = (int)((g[i].red + DENSE_BK - 1) / DENSE_BK);
+    j.k_tiles = j.chain_tiles * (g[i].chained ? 2 : 1);
+    j.a_mn = g[i].a_mn;
+    j.b_mn = g[i].b_mn;
+    j.stacked = g[i].stacked;
+    const int64_t tiles = (int64_t)j.row_tiles * (j.stacked ? 2 : 1) * j.col_tiles;
+    if (tiles > 0x3fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
+    j.tiles = (int)tiles;
+    j.raster = 16;
+    j.idesc = dense_idesc(256, 256, p.f16 != 0, g[i].a_mn, g[i].b_mn);
+    const int na = (g[i].chained || g[i].stacked) ? 2 : 1, nb = (g[i].chained || g[i].dual) ? 2 : 1;
+    for (int q = 0; q < na; ++q) {
+      int rc = dense_encode(&maps.job[i].a[q], g[i].a[q].base, g[i].a[q].outer, g[i].a[q].inner, g[i].a[q].ld, g[i].a_mn ? 64 : 128, p.f16);
+      if (rc) return rc;
+    }
+    for (int q = 0; q < nb; ++q) {
+      int rc = dense_encode(&maps.job[i].b[q], g[i].b[q].base, g[i].b[q].outer, g[i].b[q].inner, g[i].b[q].ld, g[i].b_mn ? 64 : 128, p.f16);
+      if (rc) return rc;
+    }
+  }
+  const int total = p.job[0].tiles + (jobs > 1 ? p.job[1].tiles : 0);
+  const int pairs = std::max(1, std::min(di->sm_count / 2, total));
+  p.full_rounds = p.job[0].tiles / pairs;
+  p.rest = p.job[0].tiles % pairs;
+  p.early = p.early_tiles = 0;
+  if (jobs > 1 && p.rest > 0) {
+    // a tile of job 0 lasts as long as this many of job 1
+    p.early = std::max(1, (p.job[0].k_tiles + p.job[1].k_tiles / 2) / p.job[1].k_tiles);
+    p.early_tiles = (int)std::min<int64_t>(p.job[1].tiles, (int64_t)p.early * (pairs - p.rest));
+  }
+  if (g[0].epi == DENSE_GLU) return dense_launch_pair<DENSE_GLU>(maps, p, pairs, stream);
+  if (g[0].epi == DENSE_LINEAR) return dense_launch_pair<DENSE_LINEAR>(maps, p, pairs, stream);
+  return dense_launch_pair<DENSE_STORE>(maps, p, pairs, stream);
+}
+
+static void pair_params(PairParams& p, const b200moe_dense_args* a) {
+  memset(&p, 0, sizeof(p));
+  p.f16 = a->dtype == B200MOE_DTYPE_F16;
+  p.act = a->act;
+  p.wait_limit_ns = a->wait_limit_ms > 0 ? (uint64_t)a->wait_limit_ms * 1000000ull : kWaitLimitNs;
+}
+
+// A product of more rows than the tile kernel holds in one tile, and whose 256 x 256 tiles occupy at least half of the SM
+// pairs, goes to the pair kernel.
+static bool pair_pays(int64_t rows, int64_t cols, int64_t tile_cols, const DeviceInfo* di) {
+  return rows > 128 && ((rows + 255) / 256) * ((cols + tile_cols - 1) / tile_cols) * 4 >= di->sm_count;
+}
+
 // a TMA operand: 16-byte aligned base and pitch
 static int check_operand(const char* op, const char* name, const void* p, int64_t ld, int64_t inner) {
   if (!p) return fail(B200MOE_E_NULL, "%s: %s is required", op, name);
@@ -763,6 +1177,35 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
   if (gated ? a->y_dtype != a->dtype : (a->y_dtype != a->dtype && a->y_dtype != B200MOE_DTYPE_F32))
     return fail(B200MOE_E_UNSUPPORTED, "%s: output dtype %d", op, a->y_dtype);
   if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != B200MOE_DTYPE_F32) return fail(B200MOE_E_UNSUPPORTED, "%s: bias dtype %d", op, a->bias_dtype);
+  if (a->y_dtype != B200MOE_DTYPE_F32 && pair_pays(a->m, a->n, gated ? 128 : 256, di)) {
+    PairParams q;
+    pair_params(q, a);
+    DenseGemm g;
+    g.a[0] = {a->x, a->m, a->k, a->ld_x};
+    g.b[0] = {a->w0, a->n, a->k, a->ld_w0};
+    g.b[1] = {a->w1, a->n, a->k, a->ld_w1};
+    g.dual = gated;
+    g.epi = gated ? DENSE_GLU : DENSE_LINEAR;
+    g.rows = a->m;
+    g.cols = a->n;
+    g.red = a->k;
+    q.job[0].out[0] = a->y;
+    q.job[0].ld_out = a->ld_y;
+    q.pre[0] = a->pre0;
+    q.pre[1] = a->pre1;
+    q.ld_pre[0] = a->ld_pre0;
+    q.ld_pre[1] = a->ld_pre1;
+    q.job[0].vec = aligned16(a->y) && a->ld_y % 8 == 0 && aligned16(a->pre0) && aligned16(a->pre1) && (!a->pre0 || a->ld_pre0 % 8 == 0) &&
+                   (!a->pre1 || a->ld_pre1 % 8 == 0);
+    if (!gated) {
+      q.bias = a->bias;
+      q.bias_f32 = a->bias_dtype == B200MOE_DTYPE_F32;
+      q.residual = a->residual;
+      q.ld_res = a->ld_residual;
+      if (a->residual && (!aligned16(a->residual) || a->ld_residual % 8 != 0)) q.job[0].vec = 0;
+    }
+    return dense_pair_gemm(&g, 1, q, di, stream);
+  }
   DenseParams p;
   dense_params(p, a);
   p.out[0] = a->y;
@@ -806,6 +1249,47 @@ static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // dx = sum of dz_i w_i and dw_i = dz_i^T x
 static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, DeviceInfo* di, cudaStream_t stream) {
+  {
+    // both products in one launch of the pair kernel where their tiles fill it
+    const int64_t dx_tiles = a->dx ? ((a->m + 255) / 256) * ((a->k + 255) / 256) : 0;
+    const int64_t dw_tiles = a->dw0 ? count * ((a->n + 255) / 256) * ((a->k + 255) / 256) : 0;
+    if ((dx_tiles + dw_tiles) * 4 >= di->sm_count && a->m >= 128) {
+      PairParams q;
+      pair_params(q, a);
+      DenseGemm g[2];
+      int jobs = 0;
+      if (a->dx) {
+        DenseGemm& x = g[jobs];
+        for (int i = 0; i < count; ++i) {
+          x.a[i] = {dz[i], a->m, a->n, ld_dz};
+          x.b[i] = {i ? a->w1 : a->w0, a->n, a->k, i ? a->ld_w1 : a->ld_w0};
+        }
+        x.chained = count == 2;
+        x.b_mn = true;
+        x.rows = a->m;
+        x.cols = a->k;
+        x.red = a->n;
+        q.job[jobs].out[0] = a->dx;
+        q.job[jobs].ld_out = a->k;
+        q.job[jobs++].vec = aligned16(a->dx);
+      }
+      if (a->dw0) {
+        DenseGemm& w = g[jobs];
+        for (int i = 0; i < count; ++i) w.a[i] = {dz[i], a->m, a->n, ld_dz};
+        w.b[0] = {a->x, a->m, a->k, a->ld_x};
+        w.stacked = count == 2;
+        w.a_mn = w.b_mn = true;
+        w.rows = a->n;
+        w.cols = a->k;
+        w.red = a->m;
+        q.job[jobs].out[0] = a->dw0;
+        q.job[jobs].out[1] = a->dw1;
+        q.job[jobs].ld_out = a->k;
+        q.job[jobs++].vec = aligned16(a->dw0) && aligned16(a->dw1);
+      }
+      return dense_pair_gemm(g, jobs, q, di, stream);
+    }
+  }
   DenseParams p;
   if (a->dx) {
     dense_params(p, a);

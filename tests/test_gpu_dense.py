@@ -51,7 +51,7 @@ def glu64(g, u, act):
 
 def act64(z, act):
     if act == "relu":
-        return z.clamp(min=0.0)
+        return torch.relu(z)  # no gradient at 0 (clamp has one there)
     if act == "silu":
         return z * torch.sigmoid(z)
     if act == "gelu":
@@ -63,6 +63,8 @@ def act64(z, act):
 SHAPES = [
     (1, 8, 1), (1, 4096, 640), (2, 64, 7), (7, 72, 129), (16, 520, 128), (17, 1000, 200), (33, 128, 64), (64, 2048, 127), (65, 192, 300),
     (128, 64, 256), (129, 1024, 1001), (300, 776, 520), (513, 1544, 260), (1030, 512, 777),
+    # enough 256 x 256 tiles for the kernel of CTA pairs, forward and backward: fewer tiles than pairs, several rounds, odd edges
+    (1300, 520, 2100), (130, 1544, 3001), (2049, 264, 1290), (2600, 72, 3100), (4096, 136, 2304),
 ]  # fmt: skip
 
 
