@@ -58,7 +58,9 @@ def __getattr__(name):
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
     import importlib
 
-    return getattr(importlib.import_module(f"{__name__}.{mod}"), name)
+    value = getattr(importlib.import_module(f"{__name__}.{mod}"), name)
+    globals()[name] = value  # the next access finds it without this function
+    return value
 
 
 def __dir__():

@@ -36,6 +36,7 @@ struct DenseParams {
   int chain_tiles;           // stages of one chain: beyond them the second pair of tensor maps is read
   int split;                 // CTAs of a cluster that share a tile's reduction
   int stages, stage_bytes;
+  int reduce_offset;         // where the partial sums meet, from the start of the ring
   int a_mn, b_mn;            // operand is MN-major
   int stacked;               // row tiles beyond row_tiles belong to the second A operand and the second output
   uint32_t idesc;
@@ -170,29 +171,33 @@ __device__ __forceinline__ float act_grad_f(float z, int act) {
 // k-tiles, sends its partial sums to the owners of the columns through distributed shared memory, and every CTA
 // finishes its share of the columns.  Sums are added in the order of the ranks, so a result does not depend on timing.
 //
-// kDual: two A tiles per stage (gate and up weights) against one B tile.  kTrans: the rows of the tile are output
-// features and its columns are tokens, element (r, c) goes to out[c * ld + r] (32 lanes = 32 neighbouring
-// features); otherwise element (r, c) goes to out[r * ld + c].
+// DENSE_GLU: the 128 operand rows of a tile are 64 rows of the gate weights and the same 64 rows of the up weights, so the
+// two projections of a feature land in lanes r and r + 64 and meet in shared memory, where the partial sums go anyway.
+//
+// kTrans: the rows of the tile are output features and its columns are tokens, element (r, c) goes to
+// out[c * ld + r] (32 lanes = 32 neighbouring features); otherwise element (r, c) goes to out[r * ld + c].
 //
 // kSeg: the accumulator is drained into registers every kSegTiles stages and added there with float32
 // round-to-nearest.  The tensor core's own accumulation rounds towards zero: over K = 7168 that leaves a bias of
 // 7e-6 of the result (measured), 4e-7 over the 512 elements of a segment.  Used for float32 outputs; a 16-bit
 // output's rounding (2^-9) hides it.
 //
-// warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-5 epilogue (one per TMEM lane quarter)
+// warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (TMEM lane quarter x every other 16 columns)
 // ---------------------------------------------------------------------------------------
-constexpr int DENSE_THREADS = 192;
+constexpr int DENSE_THREADS = 320;
+constexpr int DENSE_SMEM = 112 * 1024;  // per CTA, two CTAs to an SM
 constexpr int kSegTiles = 8;
 constexpr int kSegCols = 64;
 
-template <bool kDual, bool kTrans, int kEpi, bool kSeg>
-__global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const DenseParams p) {
+template <bool kTrans, int kEpi, bool kSeg>
+__global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t s_bars[2 * 16 + 4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
-  constexpr int kAcc = kDual ? 2 : 1;
+  constexpr bool kGlu = kEpi == DENSE_GLU;
+  constexpr int kTileRows = kGlu ? 64 : 128;
   const uint32_t ring = smem_u32(smem);
   const uint32_t bars = smem_u32(s_bars);
   const int stages = p.stages;
@@ -204,14 +209,14 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
   const WaitCtx wc = {&s_abort, p.wait_limit_ns};
 
   const int rank = (int)(blockIdx.x % (unsigned)p.split);
-  int tile = (int)(blockIdx.x / (unsigned)p.split);
+  const int tile = (int)(blockIdx.x / (unsigned)p.split);
   const int all_row_tiles = p.row_tiles * (p.stacked ? 2 : 1);
   int row_tile = tile % all_row_tiles;
   const int col_tile = tile / all_row_tiles;
   const int which = row_tile >= p.row_tiles ? 1 : 0;  // stacked: second operand and output
   row_tile -= which * p.row_tiles;
-  const int row0 = row_tile * 128, col0 = col_tile * p.tile_cols;
   const int C = p.tile_cols;
+  const int row0 = row_tile * kTileRows, col0 = col_tile * C;
   const int kt0 = (int)((int64_t)p.k_tiles * rank / p.split), kt1 = (int)((int64_t)p.k_tiles * (rank + 1) / p.split);
   const int nk = kt1 - kt0;  // at least 1: split <= k_tiles
 
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full_bar(b), 1);
-      mbar_init(acc_empty_bar(b), 4);
+      mbar_init(acc_empty_bar(b), 8);
     }
     s_abort = 0;
     fence_mbar_init();
@@ -234,12 +239,12 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // (waited for before the first access to another CTA's shared memory: by then every CTA of the cluster has started)
+  if (p.split > 1) cluster_arrive();
   const uint32_t tmem = s_tmem;
 
   if (warp == 0) {
     // ---- producer -----------------------------------------------------------------------
-    const int a_bytes = kAcc * DENSE_A_BYTES;
-    const bool second_a = which != 0;
     int issued = 0;
     for (; issued < nk; ++issued) {
       const int s = issued % stages;
@@ -254,22 +259,23 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
         }
         const int kc = kt * DENSE_BK;
         mbar_arrive_expect_tx(fb, (uint32_t)p.stage_bytes);
-#pragma unroll
-        for (int a = 0; a < kAcc; ++a) {
-          const CUtensorMap* m = &maps.a[kDual ? a : ((chain | (second_a ? 1 : 0)) ? 1 : 0)];
-          const uint32_t d = dst + a * DENSE_A_BYTES;
+        if constexpr (kGlu) {
+          tma_load_2d(dst, &maps.a[0], fb, kc, row0);
+          tma_load_2d(dst + 64 * 128, &maps.a[1], fb, kc, row0);
+        } else {
+          const CUtensorMap* m = &maps.a[chain | which];
           if (p.a_mn) {
-            tma_load_2d(d, m, fb, row0, kc);
-            tma_load_2d(d + DENSE_SLAB, m, fb, row0 + 64, kc);
+            tma_load_2d(dst, m, fb, row0, kc);
+            tma_load_2d(dst + DENSE_SLAB, m, fb, row0 + 64, kc);
           } else {
-            tma_load_2d(d, m, fb, kc, row0);
+            tma_load_2d(dst, m, fb, kc, row0);
           }
         }
         const CUtensorMap* m = &maps.b[chain];
         if (p.b_mn) {
-          for (int q = 0; q < C / 64; ++q) tma_load_2d(dst + a_bytes + q * DENSE_SLAB, m, fb, col0 + 64 * q, kc);
+          for (int q = 0; q < C / 64; ++q) tma_load_2d(dst + DENSE_A_BYTES + q * DENSE_SLAB, m, fb, col0 + 64 * q, kc);
         } else {
-          tma_load_2d(dst + a_bytes, m, fb, kc, col0);
+          tma_load_2d(dst + DENSE_A_BYTES, m, fb, kc, col0);
         }
       }
       __syncwarp();
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     // leading byte offset is the distance of two slabs.  (In a cluster the shared-memory address of a CTA carries its
     // rank above the 18 bits of the offset: only the 14-bit field goes into the descriptor.)
     const uint32_t a_lo0 = ((ring >> 4) & 0x3FFFu) | (p.a_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
-    const uint32_t b_lo0 = (((ring + kAcc * DENSE_A_BYTES) >> 4) & 0x3FFFu) | (p.b_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
+    const uint32_t b_lo0 = (((ring + DENSE_A_BYTES) >> 4) & 0x3FFFu) | (p.b_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
     const uint32_t a_step = p.a_mn ? (16u * 128u) >> 4 : 2u, b_step = p.b_mn ? (16u * 128u) >> 4 : 2u;
     auto desc = [](uint32_t lo) { return ((uint64_t)HI << 32) | lo; };
     bool ok = true;
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     for (int i = 0; i < nk && ok; ++i) {
       const int s = i % stages;
       const int in_seg = kSeg ? i % kSegTiles : i;
-      const uint32_t acc = tmem + (kSeg ? (uint32_t)((seg & 1) * kAcc * C) : 0u);
+      const uint32_t acc = tmem + (kSeg ? (uint32_t)((seg & 1) * C) : 0u);
       if (kSeg && in_seg == 0 && seg >= 2) {
         // the epilogue has taken the segment that used this accumulator
         if (!__all_sync(0xffffffffu, mbar_wait(acc_empty_bar(seg & 1), (uint32_t)((seg >> 1) - 1) & 1u, wc, ST_DENSE_ACC))) { ok = false; break; }
@@ -306,12 +312,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
       if (elect_one()) {
         const uint32_t off = ((uint32_t)s * p.stage_bytes) >> 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int a = 0; a < kAcc; ++a)
-            mma_f16_ss<false>(acc + a * C, desc(a_lo0 + off + a * (DENSE_A_BYTES >> 4) + j * a_step), desc(b_lo0 + off + j * b_step), p.idesc,
-                              (in_seg | j) != 0);
-        }
+        for (int j = 0; j < 4; ++j) mma_f16_ss<false>(acc, desc(a_lo0 + off + j * a_step), desc(b_lo0 + off + j * b_step), p.idesc, (in_seg | j) != 0);
         tc_commit(empty_bar(s));
         if (seg_end) tc_commit(acc_full_bar(kSeg ? seg & 1 : 0));
       }
@@ -323,31 +324,30 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
 
   // ---- epilogue -------------------------------------------------------------------------
   const bool f16 = p.f16 != 0;
-  const int quarter = warp & 3;
+  const int quarter = warp & 3, half = (warp - 2) >> 2;  // this warp: TMEM lanes 32 quarter .. + 31, chunks half, half + 2, ...
   const int r_in_tile = quarter * 32 + lane;
-  const int row = row0 + r_in_tile;
-  const bool row_ok = row < p.rows;
   const int valid = min(C, p.cols - col0);
-  float sums[kSeg ? kSegCols : 1];
+  float sums[kSeg ? kSegCols / 2 : 1];
   bool ok = true;
   if (warp >= 2) {
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     if constexpr (kSeg) {
 #pragma unroll
-      for (int j = 0; j < kSegCols; ++j) sums[j] = 0.0f;
+      for (int j = 0; j < kSegCols / 2; ++j) sums[j] = 0.0f;
       const int segs = (nk + kSegTiles - 1) / kSegTiles;
       for (int sg = 0; sg < segs; ++sg) {
         if (!__all_sync(0xffffffffu, mbar_wait(acc_full_bar(sg & 1), (uint32_t)(sg >> 1) & 1u, wc, ST_DENSE_ACC))) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < kSegCols; c += 16) {
+        for (int q = 0; q < kSegCols / 32; ++q) {
+          const int c = half * 16 + q * 32;
           if (c < C) {
             float v[16];
             tmem_ld_32x16(tmem + lanes + (uint32_t)((sg & 1) * C + c), v);
             tmem_ld_wait();
             reg_fence16(v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sums[c + j] += v[j];
+            for (int j = 0; j < 16; ++j) sums[q * 16 + j] += v[j];
           }
         }
         tc_fence_before();
@@ -360,114 +360,129 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     }
   }
 
-  // columns of this CTA's accumulators in chunks of 16: f(first column, values of accumulator 0, of accumulator 1)
+  // this warp's chunks of 16 accumulator columns: f(first column, values)
   auto each_chunk = [&](auto f) {
     if constexpr (kSeg) {
 #pragma unroll
-      for (int c = 0; c < kSegCols; c += 16)
-        if (c < valid) f(c, sums + c, sums + c);
+      for (int q = 0; q < kSegCols / 32; ++q)
+        if (half * 16 + q * 32 < valid) f(half * 16 + q * 32, sums + q * 16);
     } else {
       const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < valid; c += 16) {
-        float v0[16], v1[16];
+      for (int c = half * 16; c < valid; c += 32) {
+        float v[16];
         __syncwarp();
-        tmem_ld_32x16(base + c, v0);
-        if (kDual) tmem_ld_32x16(base + C + c, v1);
+        tmem_ld_32x16(base + c, v);
         tmem_ld_wait();
-        reg_fence16(v0);
-        if (kDual) reg_fence16(v1);
-        f(c, v0, v1);
+        reg_fence16(v);
+        f(c, v);
       }
     }
   };
-
-  float bias = 0.0f;
-  if (kEpi == DENSE_LINEAR && warp >= 2 && p.bias && row_ok)
-    bias = p.bias_f32 ? reinterpret_cast<const float*>(p.bias)[row] : load16(p.bias, row, f16);
-  // kTrans: one element (feature = row, token = col0 + c); residual read by the caller
-  auto emit = [&](int c, float v0, float v1, float res) {
-    const int64_t o = (int64_t)(col0 + c) * p.ld_out + row;
+  // kTrans, one element: feature `row`, token col0 + c
+  auto bias_at = [&](int row) -> float {
+    if (kEpi != DENSE_LINEAR || !p.bias || row >= p.rows) return 0.0f;
+    return p.bias_f32 ? reinterpret_cast<const float*>(p.bias)[row] : load16(p.bias, row, f16);
+  };
+  auto residual_at = [&](int row, int c) -> float {
+    return kEpi == DENSE_LINEAR && p.residual ? load16(p.residual, (int64_t)(col0 + c) * p.ld_res + row, f16) : 0.0f;
+  };
+  auto emit = [&](int row, int c, float v0, float v1, float res) {
+    const int64_t t = col0 + c;
     float y;
-    if constexpr (kEpi == DENSE_GLU) {
+    if constexpr (kGlu) {
       if (p.pre[0]) {
-        store16(p.pre[0], (int64_t)(col0 + c) * p.ld_pre[0] + row, v0, f16);
-        store16(p.pre[1], (int64_t)(col0 + c) * p.ld_pre[1] + row, v1, f16);
+        store16(p.pre[0], t * p.ld_pre[0] + row, v0, f16);
+        store16(p.pre[1], t * p.ld_pre[1] + row, v1, f16);
       }
       y = glu_f(v0, v1, p.act);
     } else {
-      const float z = v0 + bias;
-      if (p.pre[0]) store16(p.pre[0], (int64_t)(col0 + c) * p.ld_pre[0] + row, z, f16);
-      y = act_f(z, p.act) + res;
+      if (p.pre[0]) store16(p.pre[0], t * p.ld_pre[0] + row, v0, f16);
+      y = act_f(v0, p.act) + res;
     }
-    if (p.out_f32) reinterpret_cast<float*>(p.out[0])[o] = y;
-    else store16(p.out[0], o, y, f16);
-  };
-  auto residual_at = [&](int c) -> float {
-    if (kEpi == DENSE_LINEAR && p.residual) return load16(p.residual, (int64_t)(col0 + c) * p.ld_res + row, f16);
-    return 0.0f;
+    if (p.out_f32) reinterpret_cast<float*>(p.out[0])[t * p.ld_out + row] = y;
+    else store16(p.out[0], t * p.ld_out + row, y, f16);
   };
 
-  if (p.split > 1) {
-    const int slice = (valid + p.split - 1) / p.split;  // columns that one CTA of the cluster finishes
-    __syncwarp();
-    cluster_arrive();  // every CTA of the cluster has read its last operand stage: the rings may be overwritten
-    cluster_wait();
+  const int split = p.split;
+  if (kGlu || split > 1) {
+    // partial sums meet in shared memory: [rank][column of the owner's slice][row].  With one CTA that is the ring, which the
+    // products have left; with several a region of its own, since another CTA's products may still read its ring.
+    const int slice = (valid + split - 1) / split;  // columns that one CTA of the cluster finishes
+    const uint32_t region = ring + p.reduce_offset;
+    if (split > 1) {
+      __syncwarp();
+      cluster_wait();  // (of the arrival at the start)
+    }
     if (warp >= 2 && ok) {
-      each_chunk([&](int c0, const float* v0, const float* v1) {
+      each_chunk([&](int c0, const float* v) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int c = c0 + j;
           if (c < valid) {
-            const int owner = c / slice;
-            const uint32_t a = map_to_cta(ring, (uint32_t)owner) + (uint32_t)((((rank * kAcc) * slice + (c - owner * slice)) * 128 + r_in_tile) * 4);
-            st_cluster_f32(a, v0[j]);
-            if (kDual) st_cluster_f32(a + (uint32_t)(slice * 512), v1[j]);
+            if (split == 1) {
+              st_shared_f32(region + (uint32_t)((c * 128 + r_in_tile) * 4), v[j]);
+            } else {
+              const int owner = c / slice;
+              st_cluster_f32(map_to_cta(region, (uint32_t)owner) + (uint32_t)(((rank * slice + c - owner * slice) * 128 + r_in_tile) * 4), v[j]);
+            }
           }
         }
       });
     }
     __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    if (warp >= 2 && row_ok) {
-      const float* part = reinterpret_cast<const float*>(smem) + r_in_tile;
-      const int c0 = rank * slice, c1 = min(valid, c0 + slice);
-      for (int c = c0; c < c1; ++c) {
-        const float res = kTrans ? residual_at(c) : 0.0f;
-        float v0 = 0.0f, v1 = 0.0f;
-        for (int r = 0; r < p.split; ++r) {
-          v0 += part[((r * kAcc) * slice + (c - c0)) * 128];
-          if (kDual) v1 += part[((r * kAcc + 1) * slice + (c - c0)) * 128];
+    if (split > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    if (warp >= 2) {
+      constexpr int kGroups = 256 / kTileRows;  // columns in flight
+      const int t = (int)threadIdx.x - 64;
+      const int r = t % kTileRows, row = row0 + r;
+      const int c_begin = rank * slice, c_end = min(valid, c_begin + slice);
+      if (row < p.rows) {
+        const float* part = reinterpret_cast<const float*>(smem + p.reduce_offset) + r;
+        const float bias = bias_at(row);
+        for (int c = c_begin + t / kTileRows; c < c_end; c += kGroups) {
+          const float res = residual_at(row, c);
+          float v0 = 0.0f, v1 = 0.0f;
+          for (int q = 0; q < split; ++q) {
+            v0 += part[(q * slice + c - c_begin) * 128];
+            if (kGlu) v1 += part[(q * slice + c - c_begin) * 128 + 64];
+          }
+          if constexpr (kTrans) emit(row, c, v0 + bias, v1, res);
+          else store16(p.out[which], (int64_t)row * p.ld_out + col0 + c, v0, f16);
         }
-        if constexpr (kTrans) emit(c, v0, v1, res);
-        else store16(p.out[which], (int64_t)row * p.ld_out + col0 + c, v0, f16);
       }
     }
   } else if (warp >= 2 && ok) {
-    each_chunk([&](int c0, const float* v0, const float* v1) {
+    const int row = row0 + r_in_tile;
+    const bool row_ok = row < p.rows;
+    const float bias = bias_at(row);
+    each_chunk([&](int c0, const float* v) {
+      if (!row_ok) return;
       if constexpr (kTrans) {
-        if (!row_ok) return;
         float res[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) res[j] = c0 + j < valid ? residual_at(c0 + j) : 0.0f;
+        for (int j = 0; j < 16; ++j) res[j] = c0 + j < valid ? residual_at(row, c0 + j) : 0.0f;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (c0 + j < valid) emit(c0 + j, v0[j], v1[j], res[j]);
+          if (c0 + j < valid) emit(row, c0 + j, v[j] + bias, 0.0f, res[j]);
       } else {
-        if (!row_ok) return;
         const int64_t o = (int64_t)row * p.ld_out + col0 + c0;
         if (p.vec_store && c0 + 16 <= valid) {
           uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = pack16x2_from_float(v0[2 * j], v0[2 * j + 1], f16);
+          for (int j = 0; j < 8; ++j) w[j] = pack16x2_from_float(v[2 * j], v[2 * j + 1], f16);
           uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out[which]) + o);
           d[0] = make_uint4(w[0], w[1], w[2], w[3]);
           d[1] = make_uint4(w[4], w[5], w[6], w[7]);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c0 + j < valid) store16(p.out[which], o + j, v0[j], f16);
+            if (c0 + j < valid) store16(p.out[which], o + j, v[j], f16);
         }
       }
     });
@@ -980,15 +995,15 @@ struct DenseGemm {
   bool segmented = false;
 };
 
-template <bool kDual, bool kTrans, int kEpi, bool kSeg>
+template <bool kTrans, int kEpi, bool kSeg>
 static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsigned grid, cudaStream_t stream) {
-  auto kern = dense_tile_kernel<kDual, kTrans, kEpi, kSeg>;
-  const int smem = p.stages * p.stage_bytes + 1024;
+  auto kern = dense_tile_kernel<kTrans, kEpi, kSeg>;
+  const int smem = DENSE_SMEM;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
   int dev = 0;
   B200_CUDA_CHECK(cudaGetDevice(&dev));
   if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024));
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM));
     ready.fetch_or(1ull << (dev & 63));
   }
   cudaLaunchConfig_t cfg;
@@ -1015,23 +1030,31 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   p.a_mn = g.a_mn;
   p.b_mn = g.b_mn;
   p.stacked = g.stacked;
-  int C = g.b_mn ? 128 : (g.cols <= 16 ? 16 : (g.cols <= 32 ? 32 : (g.cols <= 64 ? 64 : 128)));
-  if (g.segmented) C = std::min(C, kSegCols);
-  p.tile_cols = C;
-  p.row_tiles = (int)((g.rows + 127) / 128);
-  p.col_tiles = (int)((g.cols + C - 1) / C);
+  const int tile_rows = g.dual ? 64 : 128;
+  p.row_tiles = (int)((g.rows + tile_rows - 1) / tile_rows);
   p.chain_tiles = (int)((g.red + DENSE_BK - 1) / DENSE_BK);
   p.k_tiles = p.chain_tiles * (g.chained ? 2 : 1);
-  const int acc = g.dual ? 2 : 1;
-  p.stage_bytes = acc * DENSE_A_BYTES + C * 128;
-  p.stages = std::min(16, (110 * 1024) / p.stage_bytes);
-  const int64_t tiles = (int64_t)p.row_tiles * (g.stacked ? 2 : 1) * p.col_tiles;
+  // Columns of a tile: as many as there are, up to 128 (float32 sums in registers: 64); halved while that leaves SMs
+  // without a tile (down to 16, MN-major operands come in slabs of 64).
+  const int least = g.b_mn ? 64 : 16, most = g.segmented ? kSegCols : 128;
+  int C = least;
+  while (C < most && C < g.cols) C *= 2;
+  auto tiles_of = [&](int c) { return (int64_t)p.row_tiles * (g.stacked ? 2 : 1) * ((g.cols + c - 1) / c); };
+  while (C > least && tiles_of(C) < di->sm_count) C /= 2;
+  const int64_t tiles = tiles_of(C);
+  p.tile_cols = C;
+  p.col_tiles = (int)((g.cols + C - 1) / C);
+  // CTAs that share a tile's reduction: as many as find room on the GPU at once, each with at least 4 stages of work
   p.split = 1;
   if (C <= 64) {
     while (p.split < DENSE_MAX_SPLIT && tiles * p.split * 2 <= 2 * di->sm_count && p.k_tiles >= p.split * 2 * 4) p.split *= 2;
   }
-  const int cols = acc * C * (g.segmented ? 2 : 1);
-  p.tmem_cols = cols <= 32 ? 32 : (cols <= 64 ? 64 : (cols <= 128 ? 128 : 256));
+  p.stage_bytes = DENSE_A_BYTES + C * 128;
+  const int reduce_bytes = p.split > 1 ? (C + p.split - 1) * 512 : 0;
+  p.stages = std::min(16, (DENSE_SMEM - 1024 - reduce_bytes) / p.stage_bytes);
+  p.reduce_offset = p.split > 1 ? p.stages * p.stage_bytes : 0;
+  const int cols = C * (g.segmented ? 2 : 1);
+  p.tmem_cols = cols <= 32 ? 32 : (cols <= 64 ? 64 : 128);
   p.idesc = dense_idesc(128, C, p.f16 != 0, g.a_mn, g.b_mn);
   if (tiles * p.split > 0x7fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
 
@@ -1039,7 +1062,7 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   memset(&maps, 0, sizeof(maps));
   const int na = (g.dual || g.chained || g.stacked) ? 2 : 1, nb = g.chained ? 2 : 1;
   for (int i = 0; i < na; ++i) {
-    int rc = dense_encode(&maps.a[i], g.a[i].base, g.a[i].outer, g.a[i].inner, g.a[i].ld, g.a_mn ? 64 : 128, p.f16);
+    int rc = dense_encode(&maps.a[i], g.a[i].base, g.a[i].outer, g.a[i].inner, g.a[i].ld, g.a_mn || g.dual ? 64 : 128, p.f16);
     if (rc) return rc;
   }
   for (int i = 0; i < nb; ++i) {
@@ -1047,10 +1070,10 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
     if (rc) return rc;
   }
   const unsigned grid = (unsigned)(tiles * p.split);
-  if (g.epi == DENSE_GLU) return dense_launch_tile<true, true, DENSE_GLU, false>(maps, p, grid, stream);
-  if (g.trans && g.segmented) return dense_launch_tile<false, true, DENSE_LINEAR, true>(maps, p, grid, stream);
-  if (g.trans) return dense_launch_tile<false, true, DENSE_LINEAR, false>(maps, p, grid, stream);
-  return dense_launch_tile<false, false, DENSE_STORE, false>(maps, p, grid, stream);
+  if (g.epi == DENSE_GLU) return dense_launch_tile<true, DENSE_GLU, false>(maps, p, grid, stream);
+  if (g.trans && g.segmented) return dense_launch_tile<true, DENSE_LINEAR, true>(maps, p, grid, stream);
+  if (g.trans) return dense_launch_tile<true, DENSE_LINEAR, false>(maps, p, grid, stream);
+  return dense_launch_tile<false, DENSE_STORE, false>(maps, p, grid, stream);
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1103,6 +1126,12 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
       if (rc) return rc;
     }
   }
+  // time of a tile in stages; below 8 its epilogue takes longer than its products
+  auto cost = [&](int i) { return std::max(8, p.job[i].k_tiles); };
+  if (jobs > 1 && cost(1) > cost(0)) {  // long tiles first, the short ones fill the rest
+    std::swap(p.job[0], p.job[1]);
+    std::swap(maps.job[0], maps.job[1]);
+  }
   const int total = p.job[0].tiles + (jobs > 1 ? p.job[1].tiles : 0);
   const int pairs = std::max(1, std::min(di->sm_count / 2, total));
   p.full_rounds = p.job[0].tiles / pairs;
@@ -1110,7 +1139,7 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
   p.early = p.early_tiles = 0;
   if (jobs > 1 && p.rest > 0) {
     // a tile of job 0 lasts as long as this many of job 1
-    p.early = std::max(1, (p.job[0].k_tiles + p.job[1].k_tiles / 2) / p.job[1].k_tiles);
+    p.early = std::max(1, (cost(0) + cost(1) / 2) / cost(1));
     p.early_tiles = (int)std::min<int64_t>(p.job[1].tiles, (int64_t)p.early * (pairs - p.rest));
   }
   if (g[0].epi == DENSE_GLU) return dense_launch_pair<DENSE_GLU>(maps, p, pairs, stream);
