@@ -104,6 +104,12 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched with the attribute may start while its predecessor on the stream
+// drains, sets itself up, and waits here until the predecessor has ended and its writes are visible.  Nothing of global
+// memory is touched before the wait.  The trigger lets the successor start in the same way.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
   return f16 ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
@@ -231,6 +237,8 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     }
     s_abort = 0;
     fence_mbar_init();
+    prefetch_tensormap(&maps.a[0]);
+    prefetch_tensormap(&maps.b[0]);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(&s_tmem), p.tmem_cols);
@@ -242,6 +250,8 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
   // (waited for before the first access to another CTA's shared memory: by then every CTA of the cluster has started)
   if (p.split > 1) cluster_arrive();
   const uint32_t tmem = s_tmem;
+  pdl_wait();
+  pdl_trigger();
 
   if (warp == 0) {
     // ---- producer -----------------------------------------------------------------------
@@ -616,7 +626,7 @@ __device__ __forceinline__ void store16x32(void* base, int64_t o, const float* v
 }
 
 template <int kEpi>
-__global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
     dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -645,6 +655,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
     }
     s_abort = 0;
     fence_mbar_init();
+    prefetch_tensormap(&maps.job[0].a[0]);
+    prefetch_tensormap(&maps.job[0].b[0]);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&s_tmem), 512);
@@ -656,6 +668,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  pdl_wait();
+  pdl_trigger();
 
   if (warp == 0) {
     // ---- producer: this CTA's halves of A and B; every copy is credited to the first CTA's barrier --------------
@@ -843,6 +857,7 @@ constexpr int GRAD_COLS = 256;  // columns of a block: 32 lanes x 8
 __global__ void __launch_bounds__(256)
     glu_grad_kernel(const void* __restrict__ dh, const void* __restrict__ gate, const void* __restrict__ up, int64_t m, int n, int64_t ld_dh,
                     int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int act, int f16, int vec) {
+  pdl_trigger();
   const int c = (int)blockIdx.x * GRAD_COLS + (threadIdx.x & 31) * 8;
   if (c >= n) return;
   for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < m; r += (int64_t)gridDim.y * 8) {
@@ -887,6 +902,7 @@ __global__ void __launch_bounds__(256)
     act_grad_kernel(const void* __restrict__ dy, const void* __restrict__ z, int64_t m, int n, int64_t ld_dy, int64_t ld_z, void* __restrict__ dz,
                     int64_t ldo, float* __restrict__ sums, int act, int f16, int dy_f32, int vec, int64_t rows_per_block) {
   __shared__ float s_part[8][GRAD_COLS];
+  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = (int)blockIdx.x * GRAD_COLS + lane * 8;
   float acc[8];
@@ -959,6 +975,7 @@ __global__ void __launch_bounds__(256)
 
 // out[c] = sum over the blocks' partial sums, in order
 __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ sums, int blocks, int n, float* __restrict__ out) {
+  pdl_trigger();
   const int c = (int)blockIdx.x * 256 + threadIdx.x;
   if (c >= n) return;
   float t = 0.0f;
@@ -995,10 +1012,32 @@ struct DenseGemm {
   bool segmented = false;
 };
 
+// A launch in clusters that may start while its predecessor drains
+struct LaunchConfig {
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  LaunchConfig(unsigned grid, unsigned threads, size_t smem, int cluster, cudaStream_t stream) {
+    memset(&cfg, 0, sizeof(cfg));
+    memset(attr, 0, sizeof(attr));
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+  LaunchConfig(const LaunchConfig&) = delete;
+};
+
 template <bool kTrans, int kEpi, bool kSeg>
 static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsigned grid, cudaStream_t stream) {
   auto kern = dense_tile_kernel<kTrans, kEpi, kSeg>;
-  const int smem = DENSE_SMEM;
   static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
   int dev = 0;
   B200_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1006,20 +1045,8 @@ static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsign
     B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM));
     ready.fetch_or(1ull << (dev & 63));
   }
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(DENSE_THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, maps, p));
+  LaunchConfig c(grid, DENSE_THREADS, DENSE_SMEM, p.split, stream);
+  B200_CUDA_CHECK(cudaLaunchKernelEx(&c.cfg, kern, maps, p));
   return B200MOE_OK;
 }
 
@@ -1088,8 +1115,8 @@ static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pair
     B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
     ready.fetch_or(1ull << (dev & 63));
   }
-  kern<<<(unsigned)(2 * pairs), PAIR_THREADS, PAIR_SMEM, stream>>>(maps, p);
-  B200_CUDA_CHECK(cudaGetLastError());
+  LaunchConfig c((unsigned)(2 * pairs), PAIR_THREADS, PAIR_SMEM, 2, stream);
+  B200_CUDA_CHECK(cudaLaunchKernelEx(&c.cfg, kern, maps, p));
   return B200MOE_OK;
 }
 
