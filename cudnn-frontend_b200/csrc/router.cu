@@ -37,6 +37,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ uint64_t order_key64(double v) {
   if (v != v) return ~0ull;
+  if (v == -INFINITY) return 0ull;
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return b >> 63 ? ~b : b | (1ull << 63);
 }
@@ -72,18 +73,29 @@ __device__ __forceinline__ float choice_weight(float logit, bool chosen, int sig
 }
 
 // One warp per row; lane l holds experts l, l + 32, ...
+//
+// With more than 32 experts the choice goes by candidates: the topk-th largest of the lanes' own maxima is a lower bound of the
+// topk-th largest value, and what reaches it (about topk + 2 of 256) is packed one to a lane and ranked by
+// counting.  Of a biased sigmoid the lanes first hold a float32 score that is off by less than 2e-6 (1 + |score|), so the bound
+// is lowered by twice that, and only the candidates' scores are formed in 64 bits.  Rows with more than 32 candidates,
+// and biased softmax scores (whose sum over the row is needed in 64 bits), take the maxima one after the other.
 template <int kPerLane, bool kBias>
 __global__ void __launch_bounds__(256)
     router_topk_kernel(const void* __restrict__ logits, int dtype, int64_t rows, int experts, int64_t ld, const float* __restrict__ bias, int topk,
                        int sigmoid, int normalize, float scale, float* __restrict__ weights, int32_t* __restrict__ ids) {
+  __shared__ int2 s_choice[8][32];
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
+  int2* choice = s_choice[threadIdx.x >> 5];
   float v[kPerLane];
+  if (dtype == B200MOE_DTYPE_F32) {
+    const float* src = reinterpret_cast<const float*>(logits) + row * ld;
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const int e = lane + 32 * i;
-    v[i] = e < experts ? load_any(logits, row * ld + e, dtype) : -INFINITY;
+    for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < experts ? __ldg(src + lane + 32 * i) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < experts ? load_any(logits, row * ld + lane + 32 * i, dtype) : -INFINITY;
   }
   float row_max = -INFINITY, row_sum = 1.0f;
   if (!sigmoid && !normalize) {
@@ -95,57 +107,122 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < kPerLane; ++i) s += v[i] == -INFINITY ? 0.0f : expf(v[i] - row_max);
     row_sum = warp_sum(s);
   }
-  // 32-bit keys of the logits, or 64-bit keys of the biased scores: those decide between neighbours that differ in the
-  // last bits of a float32, so they are formed in 64 bits
-  using Key = typename std::conditional<kBias, uint64_t, uint32_t>::type;
-  Key key[kPerLane];
-  if constexpr (kBias) {
-    double wide[kPerLane], top = -INFINITY, sum = 0.0;
-    if (!sigmoid) {
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) top = fmax(top, (double)v[i]);
-      for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
-    }
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      wide[i] = v[i] == -INFINITY ? 0.0 : (sigmoid ? 1.0 / (1.0 + exp(-(double)v[i])) : exp((double)v[i] - top));
-      sum += wide[i];
-    }
-    if (!sigmoid) sum = warp_sum(sum);
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int e = lane + 32 * i;
-      key[i] = v[i] == -INFINITY ? 0ull : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) key[i] = order_key(v[i]);
-  }
   int my_id = -1;
   float my_logit = -INFINITY;
-  for (int j = 0; j < topk; ++j) {
-    Key best = 0;
-    int at = 0;
-    float logit = 0.0f;
+  bool done = false;
+  if (kPerLane > 1 && (!kBias || sigmoid)) {
+    uint32_t key[kPerLane], best = 0;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i)
-      if (key[i] > best) best = key[i], at = i, logit = v[i];
-    Key top;
-    if constexpr (kBias) {
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
-      const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-      top = (uint64_t)hi << 32 | lo;
-    } else {
-      top = __reduce_max_sync(0xffffffffu, best);
+    for (int i = 0; i < kPerLane; ++i) {
+      float order = v[i];
+      if (kBias) order = v[i] == -INFINITY ? v[i] : rcp_approx(1.0f + ex2_approx(v[i] * -1.4426950408889634f)) + __ldg(bias + lane + 32 * i);
+      key[i] = order_key(order);
+      best = max(best, key[i]);
     }
-    if (top == 0) break;  // nothing left that may be chosen
-    const int id = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * at : 0x7fffffff);
-    const float l = __shfl_sync(0xffffffffu, logit, id & 31);
-    if (lane == j) my_id = id, my_logit = l;
-    if (lane == (id & 31)) {
+    uint32_t bound = 0;
+    for (int j = 0; j < topk; ++j) {
+      bound = __reduce_max_sync(0xffffffffu, best);
+      if (best == bound) best = 0;
+    }
+    bool fits = true;
+    if (kBias && bound != 0) {
+      float b = __uint_as_float(bound & 0x80000000u ? bound ^ 0x80000000u : ~bound);
+      b -= 4e-6f * (1.0f + fabsf(b));
+      fits = fabsf(b) < INFINITY;  // neither NaN nor infinite
+      bound = order_key(b);
+    }
+    bound = max(bound, 1u);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const bool in = key[i] >= bound;
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      const int at = count + __popc(who & ((1u << lane) - 1));
+      if (in && at < 32) choice[at] = make_int2(lane + 32 * i, __float_as_int(v[i]));
+      count += __popc(who);
+    }
+    __syncwarp();
+    if (fits && count <= 32) {
+      const int2 mine = lane < count ? choice[lane] : make_int2(0x7fffffff, 0);
+      const float logit = __int_as_float(mine.y);
+      int place = 0;
+      if constexpr (kBias) {
+        uint64_t k = 0;
+        if (lane < count) k = order_key64(1.0 / (1.0 + exp(-(double)logit)) + (double)bias[mine.x]);
+        for (int q = 0; q < count; ++q) {
+          const uint64_t other = __shfl_sync(0xffffffffu, k, q);
+          const int id = __shfl_sync(0xffffffffu, mine.x, q);
+          place += other > k || (other == k && id < mine.x);
+        }
+      } else {
+        const uint32_t k = lane < count ? order_key(logit) : 0u;
+        for (int q = 0; q < count; ++q) {
+          const uint32_t other = __shfl_sync(0xffffffffu, k, q);
+          const int id = __shfl_sync(0xffffffffu, mine.x, q);
+          place += other > k || (other == k && id < mine.x);
+        }
+      }
+      __syncwarp();
+      if (lane < count) choice[place] = mine;  // the places are a permutation of the candidates
+      __syncwarp();
+      if (lane < min(count, topk)) {
+        my_id = choice[lane].x;
+        my_logit = __int_as_float(choice[lane].y);
+      }
+      done = true;
+    }
+  }
+  if (!done) {
+    // 32-bit keys of the logits, or 64-bit keys of the biased scores: those decide between neighbours that differ in the
+    // last bits of a float32, so they are formed in 64 bits
+    using Key = typename std::conditional<kBias, uint64_t, uint32_t>::type;
+    Key key[kPerLane];
+    if constexpr (kBias) {
+      double wide[kPerLane], top = -INFINITY, sum = 0.0;
+      if (!sigmoid) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) top = fmax(top, (double)v[i]);
+        for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+      }
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        wide[i] = v[i] == -INFINITY ? 0.0 : (sigmoid ? 1.0 / (1.0 + exp(-(double)v[i])) : exp((double)v[i] - top));
+        sum += wide[i];
+      }
+      if (!sigmoid) sum = warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = v[i] == -INFINITY ? 0ull : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) key[i] = order_key(v[i]);
+    }
+    for (int j = 0; j < topk; ++j) {
+      Key best = 0;
+      int at = 0;
+      float logit = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i)
-        if (i == (id >> 5)) key[i] = 0;
+        if (key[i] > best) best = key[i], at = i, logit = v[i];
+      Key top;
+      if constexpr (kBias) {
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        top = (uint64_t)hi << 32 | lo;
+      } else {
+        top = __reduce_max_sync(0xffffffffu, best);
+      }
+      if (top == 0) break;  // nothing left that may be chosen
+      const int id = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * at : 0x7fffffff);
+      const float l = __shfl_sync(0xffffffffu, logit, id & 31);
+      if (lane == j) my_id = id, my_logit = l;
+      if (lane == (id & 31)) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+          if (i == (id >> 5)) key[i] = 0;
+      }
     }
   }
   const float w = choice_weight(my_logit, my_id >= 0, sigmoid, normalize, scale, row_max, row_sum);
@@ -205,13 +282,17 @@ __global__ void __launch_bounds__(256)
     if (other == id) total += v;
   }
   const int64_t base = row * experts;
-  for (int e = lane; e < experts; e += 32) {
-    float v = 0.0f;
-    if (whole_row) {
+  if (whole_row) {
+    for (int e = lane; e < experts; e += 32) {
       const float l = load_any(logits, row * ld + e, dtype);
-      if (l != -INFINITY) v = -(expf(l - row_max) / row_sum) * dot;
+      store_any(dlogits, base + e, l != -INFINITY ? -(expf(l - row_max) / row_sum) * dot : 0.0f, dtype);
     }
-    store_any(dlogits, base + e, v, dtype);
+  } else if (experts % 8 == 0) {  // rows of a multiple of 16 bytes
+    const int vecs = experts * (dtype == B200MOE_DTYPE_F32 ? 4 : 2) / 16;
+    uint4* dst = reinterpret_cast<uint4*>(dlogits) + row * vecs;
+    for (int q = lane; q < vecs; q += 32) dst[q] = make_uint4(0, 0, 0, 0);
+  } else {
+    for (int e = lane; e < experts; e += 32) store_any(dlogits, base + e, 0.0f, dtype);
   }
   __syncwarp();  // the row is written before its chosen entries are
   if (chosen) {
@@ -267,6 +348,7 @@ extern "C" int b200moe_router_topk_backward(const float* dweights, const void* l
   int rc = router_check("router_topk_backward", logits, dtype, rows, experts, ld, topk, score);
   if (rc || rows == 0) return rc;
   if (!dweights || !ids || !dlogits) return fail(B200MOE_E_NULL, "router_topk_backward: dweights, ids and dlogits are required");
+  if ((uintptr_t)dlogits & 15) return fail(B200MOE_E_ALIGN, "router_topk_backward: dlogits must start on a 16-byte boundary");
   router_grad_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream_v>>>(dweights, logits, dtype, ids, rows, experts, ld, topk,
                                                                                      score == B200MOE_SCORE_SIGMOID, normalize != 0, scale, dlogits);
   B200_CUDA_CHECK(cudaGetLastError());

@@ -101,6 +101,35 @@ def test_far_sigmoids_keep_their_ratio():
     assert (w[0].cpu().double() - want).abs().max() < 2e-5  # one float32 step of the arguments, 2^-16
 
 
+def test_biased_choice_where_float32_cannot_decide():
+    """Scores that differ by less than a float32 step, many equal ones (more candidates than a warp has lanes), saturated
+    sigmoids, biases far above the scores and infinite ones: the choice is that of float64."""
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    e, k = 200, 8
+    rows = [torch.full((e,), 0.3, device="cuda"), 0.3 + 1e-7 * torch.randn((e,), device="cuda", generator=gen),
+            20 + 3 * torch.rand((e,), device="cuda", generator=gen), torch.randn((e,), device="cuda", generator=gen)]  # fmt: skip
+    logits = torch.stack(rows)
+    logits[3, 17] = float("inf")
+    small = 1e-7 * torch.randn((e,), device="cuda", generator=gen)
+    far = 1e4 * torch.randn((e,), device="cuda", generator=gen)
+    off = torch.zeros((e,), device="cuda")
+    off[:30], off[40] = -math.inf, math.inf
+    for bias in (torch.zeros((e,), device="cuda"), small, far, off, torch.full((e,), -math.inf, device="cuda")):
+        for score in ("sigmoid", "softmax"):
+            l = logits if score == "sigmoid" else logits[:3]  # (softmax of +inf is NaN)
+            _, ids = cf.router_topk(l, k, score_func=score, bias=bias)
+            s = torch.sigmoid(l.double()) if score == "sigmoid" else torch.softmax(l.double(), 1)
+            top, want = torch.sort(s + bias.double(), dim=1, descending=True, stable=True)
+            want = torch.where(top[:, :k] > -math.inf, want[:, :k], -1)
+            if score == "sigmoid":
+                assert torch.equal(ids.long(), want)
+            else:  # float64's own last bits may differ between two sums over a row: the scores agree, and so does the set of clear ones
+                got = torch.where(ids >= 0, (s + bias.double()).gather(1, ids.clamp(min=0).long()), -math.inf)
+                assert torch.allclose(got, top[:, :k], rtol=1e-14, atol=1e-15)
+
+
 def test_nan_stays_in_its_row():
     import cudnn_frontend_b200 as cf
 
