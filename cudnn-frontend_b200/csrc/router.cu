@@ -5,8 +5,8 @@
 //   weights  w_j = scale * score_j, or normalised over the chosen ones scale * score_j / sum_i score_i, with
 //            score = softmax over the row, or sigmoid.  The bias decides the choice only.
 //
-// The normalised sigmoid is softmax over log sigmoid(l): the quotient of two numbers that may both underflow is
-// never formed.
+// The normalised sigmoid is formed from u_i = e^(min(l_i, 0) - m) / (1 + e^-|l_i|) with m the largest min(l_j, 0) of the
+// choice: sigmoid(l_i) = e^m u_i, so the quotient of two numbers that may both underflow is never formed.
 #include <type_traits>
 
 #include "b200moe.h"
@@ -28,44 +28,50 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, float v, int dtype
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Keys that order like the values (NaN above everything, 0 and -0 equal); key 0 = never chosen
+// Keys that order like the values (NaN above everything, 0 and -0 equal: the addition turns -0 into 0 and any NaN into the
+// positive one); a key that is not above kNever, that of -inf, is never chosen
+constexpr uint32_t kNever = 0x007FFFFFu;
+constexpr uint64_t kNever64 = 0x000FFFFFFFFFFFFFull;
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  if (v == -INFINITY) return 0u;
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int32_t b = __float_as_int(v + 0.0f);
+  return (uint32_t)(b ^ ((b >> 31) | (int32_t)0x80000000));
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ uint64_t order_key64(double v) {
   if (v != v) return ~0ull;
-  if (v == -INFINITY) return 0ull;
-  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
-  return b >> 63 ? ~b : b | (1ull << 63);
+  const int64_t b = __double_as_longlong(v + 0.0);
+  return (uint64_t)(b ^ ((b >> 63) | (int64_t)(1ull << 63)));
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// over groups of kLanes lanes; NaN stays
+template <int kLanes = 32>
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const float o = __shfl_xor_sync(0xffffffffu, v, d);
-    v = (o != o || o > v) ? o : v;  // NaN stays
-  }
+  for (int d = kLanes / 2; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
-template <typename T>
+template <int kLanes = 32, typename T>
 __device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  for (int d = kLanes / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-__device__ __forceinline__ float log_sigmoid_f(float v) { return fminf(v, 0.0f) - log1pf(expf(-fabsf(v))); }
 __device__ __forceinline__ float sigmoid_exact_f(float v) { return 1.0f / (1.0f + expf(-v)); }
 
-// Weight of the choice that this lane holds (lanes without one: chosen = false); called by the whole warp.
-// row_max / row_sum: of the whole row, for the softmax that is not normalised over the choice.
+// Weight of the choice that this lane holds (lanes without one: chosen = false), the choices of a row in a group of kLanes
+// lanes; called by the whole warp.  row_max / row_sum: of the whole row, for the softmax that is not normalised over the choice.
+template <int kLanes>
 __device__ __forceinline__ float choice_weight(float logit, bool chosen, int sigmoid, int normalize, float scale, float row_max, float row_sum) {
   if (normalize) {
-    const float a = chosen ? (sigmoid ? (logit != logit ? logit : log_sigmoid_f(logit)) : logit) : -INFINITY;
-    const float m = warp_max(a);
-    const float e = chosen ? expf(a - m) : 0.0f;
-    const float s = warp_sum(e);
+    const float a = chosen ? (sigmoid && !(logit != logit) ? fminf(logit, 0.0f) : logit) : -INFINITY;
+    const float m = warp_max<kLanes>(a);
+    float e = chosen ? expf(a - m) : 0.0f;
+    if (sigmoid && chosen) e /= 1.0f + expf(-fabsf(logit));
+    const float s = warp_sum<kLanes>(e);
     return chosen ? scale * (e / s) : 0.0f;
   }
   if (!chosen) return 0.0f;
@@ -76,18 +82,21 @@ __device__ __forceinline__ float choice_weight(float logit, bool chosen, int sig
 //
 // With more than 32 experts the choice goes by candidates: the topk-th largest of the lanes' own maxima is a lower bound of the
 // topk-th largest value, and what reaches it (about topk + 2 of 256) is packed one to a lane and ranked by
-// counting.  Of a biased sigmoid the lanes first hold a float32 score that is off by less than 2e-6 (1 + |score|), so the bound
-// is lowered by twice that, and only the candidates' scores are formed in 64 bits.  Rows with more than 32 candidates,
-// and biased softmax scores (whose sum over the row is needed in 64 bits), take the maxima one after the other.
+// counting.  Of a biased sigmoid the lanes hold a float32 score that is off by less than 2e-6 (1 + |score|), so the bound
+// is lowered by twice that; where two candidates are nearer than that to one another, the scores of all of them are formed in
+// 64 bits.  Rows with more than 32 candidates, and biased softmax scores (whose sum over the row is needed in 64 bits),
+// take the maxima one after the other.
 template <int kPerLane, bool kBias>
 __global__ void __launch_bounds__(256)
     router_topk_kernel(const void* __restrict__ logits, int dtype, int64_t rows, int experts, int64_t ld, const float* __restrict__ bias, int topk,
                        int sigmoid, int normalize, float scale, float* __restrict__ weights, int32_t* __restrict__ ids) {
   __shared__ int2 s_choice[8][32];
+  __shared__ uint32_t s_order[8][32];
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
   int2* choice = s_choice[threadIdx.x >> 5];
+  uint32_t* order = s_order[threadIdx.x >> 5];
   float v[kPerLane];
   if (dtype == B200MOE_DTYPE_F32) {
     const float* src = reinterpret_cast<const float*>(logits) + row * ld;
@@ -100,7 +109,7 @@ __global__ void __launch_bounds__(256)
   float row_max = -INFINITY, row_sum = 1.0f;
   if (!sigmoid && !normalize) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) row_max = (v[i] != v[i] || v[i] > row_max) ? v[i] : row_max;
+    for (int i = 0; i < kPerLane; ++i) row_max = max_nan(row_max, v[i]);
     row_max = warp_max(row_max);
     float s = 0.0f;
 #pragma unroll
@@ -111,55 +120,62 @@ __global__ void __launch_bounds__(256)
   float my_logit = -INFINITY;
   bool done = false;
   if (kPerLane > 1 && (!kBias || sigmoid)) {
-    uint32_t key[kPerLane], best = 0;
+    uint32_t key[kPerLane], best = kNever;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      float order = v[i];
-      if (kBias) order = v[i] == -INFINITY ? v[i] : rcp_approx(1.0f + ex2_approx(v[i] * -1.4426950408889634f)) + __ldg(bias + lane + 32 * i);
-      key[i] = order_key(order);
+      float value = v[i];
+      if (kBias) value = v[i] == -INFINITY ? v[i] : rcp_approx(1.0f + ex2_approx(v[i] * -1.4426950408889634f)) + __ldg(bias + lane + 32 * i);
+      key[i] = order_key(value);
       best = max(best, key[i]);
     }
-    uint32_t bound = 0;
+    uint32_t bound = kNever;
     for (int j = 0; j < topk; ++j) {
       bound = __reduce_max_sync(0xffffffffu, best);
-      if (best == bound) best = 0;
+      if (best == bound) best = kNever;
     }
     bool fits = true;
-    if (kBias && bound != 0) {
-      float b = __uint_as_float(bound & 0x80000000u ? bound ^ 0x80000000u : ~bound);
-      b -= 4e-6f * (1.0f + fabsf(b));
+    if (kBias && bound > kNever) {
+      const float b = key_value(bound);
       fits = fabsf(b) < INFINITY;  // neither NaN nor infinite
-      bound = order_key(b);
+      bound = order_key(b - 4e-6f * (1.0f + fabsf(b)));
     }
-    bound = max(bound, 1u);
+    bound = max(bound, kNever + 1u);
     int count = 0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const bool in = key[i] >= bound;
       const unsigned who = __ballot_sync(0xffffffffu, in);
-      const int at = count + __popc(who & ((1u << lane) - 1));
-      if (in && at < 32) choice[at] = make_int2(lane + 32 * i, __float_as_int(v[i]));
+      if (in) {
+        const int at = count + __popc(who & ((1u << lane) - 1));
+        if (at < 32) {
+          choice[at] = make_int2(lane + 32 * i, __float_as_int(v[i]));
+          order[at] = key[i];
+        }
+      }
       count += __popc(who);
     }
     __syncwarp();
     if (fits && count <= 32) {
-      const int2 mine = lane < count ? choice[lane] : make_int2(0x7fffffff, 0);
-      const float logit = __int_as_float(mine.y);
+      const int2 mine = choice[lane];  // (lanes beyond the count hold what is not used)
+      const uint32_t k = order[lane];
       int place = 0;
-      if constexpr (kBias) {
-        uint64_t k = 0;
-        if (lane < count) k = order_key64(1.0 / (1.0 + exp(-(double)logit)) + (double)bias[mine.x]);
+      bool near = false;
+      const float score = key_value(k), margin = 4e-6f * (1.0f + fabsf(score));
+      for (int q = 0; q < count; ++q) {
+        const uint32_t other = order[q];
+        const int id = choice[q].x;
+        place += other > k || (other == k && id < mine.x);
+        // (a NaN or an infinity is near nothing and needs no digits)
+        if (kBias) near |= id != mine.x && fabsf(key_value(other) - score) <= margin;
+      }
+      if (kBias && __any_sync(0xffffffffu, near && lane < count)) {
+        uint64_t wide = 0;
+        if (lane < count) wide = order_key64(1.0 / (1.0 + exp(-(double)__int_as_float(mine.y))) + (double)bias[mine.x]);
+        place = 0;
         for (int q = 0; q < count; ++q) {
-          const uint64_t other = __shfl_sync(0xffffffffu, k, q);
-          const int id = __shfl_sync(0xffffffffu, mine.x, q);
-          place += other > k || (other == k && id < mine.x);
-        }
-      } else {
-        const uint32_t k = lane < count ? order_key(logit) : 0u;
-        for (int q = 0; q < count; ++q) {
-          const uint32_t other = __shfl_sync(0xffffffffu, k, q);
-          const int id = __shfl_sync(0xffffffffu, mine.x, q);
-          place += other > k || (other == k && id < mine.x);
+          const uint64_t other = __shfl_sync(0xffffffffu, wide, q);
+          const int id = choice[q].x;
+          place += other > wide || (other == wide && id < mine.x);
         }
       }
       __syncwarp();
@@ -193,14 +209,15 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
         const int e = lane + 32 * i;
-        key[i] = v[i] == -INFINITY ? 0ull : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
+        key[i] = v[i] == -INFINITY ? kNever64 : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) key[i] = order_key(v[i]);
     }
+    const Key never = kBias ? (Key)kNever64 : (Key)kNever;
     for (int j = 0; j < topk; ++j) {
-      Key best = 0;
+      Key best = never;
       int at = 0;
       float logit = 0.0f;
 #pragma unroll
@@ -214,18 +231,18 @@ __global__ void __launch_bounds__(256)
       } else {
         top = __reduce_max_sync(0xffffffffu, best);
       }
-      if (top == 0) break;  // nothing left that may be chosen
+      if (top <= never) break;  // nothing left that may be chosen
       const int id = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * at : 0x7fffffff);
       const float l = __shfl_sync(0xffffffffu, logit, id & 31);
       if (lane == j) my_id = id, my_logit = l;
       if (lane == (id & 31)) {
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i)
-          if (i == (id >> 5)) key[i] = 0;
+          if (i == (id >> 5)) key[i] = never;
       }
     }
   }
-  const float w = choice_weight(my_logit, my_id >= 0, sigmoid, normalize, scale, row_max, row_sum);
+  const float w = choice_weight<32>(my_logit, my_id >= 0, sigmoid, normalize, scale, row_max, row_sum);
   if (lane < topk) {
     weights[row * topk + lane] = w;
     ids[row * topk + lane] = my_id;
@@ -237,25 +254,28 @@ __global__ void __launch_bounds__(256)
 //   sigmoid, normalised   the same times 1 - sigmoid(l_i)
 //   sigmoid               dl_i = dw'_i s_i (1 - s_i)
 //   softmax               dl_e = p_e (dw'_e - sum_c p_j dw'_j)                   (every e; dw'_e = 0 outside c)
-// An expert that occurs twice gets the sum of both gradients.
+// An expert that occurs twice gets the sum of both gradients.  A row's choice sits in kLanes lanes, 32 / kLanes rows to a warp
+// (the whole-row softmax takes a warp for each); the rows of a warp are cleared as one piece.
+template <int kLanes>
 __global__ void __launch_bounds__(256)
     router_grad_kernel(const float* __restrict__ dweights, const void* __restrict__ logits, int dtype, const int32_t* __restrict__ ids, int64_t rows,
                        int experts, int64_t ld, int topk, int sigmoid, int normalize, float scale, void* __restrict__ dlogits) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  constexpr int kRows = 32 / kLanes;
   const int lane = threadIdx.x & 31;
-  int id = lane < topk ? ids[row * topk + lane] : -1;
+  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * kRows;
+  if (row0 >= rows) return;
+  const int64_t row = row0 + lane / kLanes;
+  const int j = lane % kLanes;
+  const bool mine = row < rows && j < topk;
+  int id = mine ? ids[row * topk + j] : -1;
   if (id >= experts) id = -1;
   const bool chosen = id >= 0;
   const float logit = chosen ? load_any(logits, row * ld + id, dtype) : -INFINITY;
-  const float dw = chosen ? dweights[row * topk + lane] : 0.0f;
-  const bool whole_row = !sigmoid && !normalize;
+  const float dw = chosen ? dweights[row * topk + j] : 0.0f;
+  const bool whole_row = kLanes == 32 && !sigmoid && !normalize;
   float row_max = -INFINITY, row_sum = 1.0f;
   if (whole_row) {
-    for (int e = lane; e < experts; e += 32) {
-      const float v = load_any(logits, row * ld + e, dtype);
-      row_max = (v != v || v > row_max) ? v : row_max;
-    }
+    for (int e = lane; e < experts; e += 32) row_max = max_nan(row_max, load_any(logits, row * ld + e, dtype));
     row_max = warp_max(row_max);
     float s = 0.0f;
     for (int e = lane; e < experts; e += 32) {
@@ -264,40 +284,40 @@ __global__ void __launch_bounds__(256)
     }
     row_sum = warp_sum(s);
   }
-  const float w = choice_weight(logit, chosen, sigmoid, normalize, scale, row_max, row_sum);
-  const float dot = warp_sum(w * dw);
-  float g;
-  if (normalize) {
-    g = w * (dw - (scale != 0.0f ? dot / scale : 0.0f));
-    if (sigmoid) g *= sigmoid_exact_f(-logit);
-  } else {
-    g = w * dw;
-    if (sigmoid) g *= sigmoid_exact_f(-logit);
-  }
+  const float w = choice_weight<kLanes>(logit, chosen, sigmoid, normalize, scale, row_max, row_sum);
+  const float dot = warp_sum<kLanes>(w * dw);
+  float g = normalize ? w * (dw - (scale != 0.0f ? dot / scale : 0.0f)) : w * dw;
+  if (sigmoid) g *= sigmoid_exact_f(-logit);
   if (!chosen) g = 0.0f;
-  float total = 0.0f;
-  for (int j = 0; j < topk; ++j) {
-    const int other = __shfl_sync(0xffffffffu, id, j);
-    const float v = __shfl_sync(0xffffffffu, g, j);
-    if (other == id) total += v;
+  float total = g;
+  const unsigned same = __match_any_sync(0xffffffffu, chosen ? (lane / kLanes) << 16 | id : -1 - lane);
+  if (__any_sync(0xffffffffu, __popc(same) > 1)) {
+    total = 0.0f;
+    for (int q = 0; q < kLanes; ++q) {
+      const int other = __shfl_sync(0xffffffffu, id, q, kLanes);
+      const float v = __shfl_sync(0xffffffffu, g, q, kLanes);
+      if (other == id) total += v;
+    }
   }
-  const int64_t base = row * experts;
   if (whole_row) {
     for (int e = lane; e < experts; e += 32) {
       const float l = load_any(logits, row * ld + e, dtype);
-      store_any(dlogits, base + e, l != -INFINITY ? -(expf(l - row_max) / row_sum) * dot : 0.0f, dtype);
+      store_any(dlogits, row * experts + e, l != -INFINITY ? -(expf(l - row_max) / row_sum) * dot : 0.0f, dtype);
     }
-  } else if (experts % 8 == 0) {  // rows of a multiple of 16 bytes
-    const int vecs = experts * (dtype == B200MOE_DTYPE_F32 ? 4 : 2) / 16;
-    uint4* dst = reinterpret_cast<uint4*>(dlogits) + row * vecs;
-    for (int q = lane; q < vecs; q += 32) dst[q] = make_uint4(0, 0, 0, 0);
   } else {
-    for (int e = lane; e < experts; e += 32) store_any(dlogits, base + e, 0.0f, dtype);
+    const int64_t size = dtype == B200MOE_DTYPE_F32 ? 4 : 2;
+    const int count = (int)min((int64_t)kRows, rows - row0) * experts;
+    uint8_t* dst = reinterpret_cast<uint8_t*>(dlogits) + row0 * experts * size;
+    if (experts % 8 == 0) {  // rows of a multiple of 16 bytes
+      for (int q = lane; q < count * (int)size / 16; q += 32) reinterpret_cast<uint4*>(dst)[q] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int q = lane; q < count; q += 32) store_any(dst, q, 0.0f, dtype);
+    }
   }
-  __syncwarp();  // the row is written before its chosen entries are
+  __syncwarp();  // the rows are written before their chosen entries are
   if (chosen) {
     if (whole_row && logit != -INFINITY) total -= (expf(logit - row_max) / row_sum) * dot;
-    store_any(dlogits, base + id, total, dtype);
+    store_any(dlogits, row * experts + id, total, dtype);
   }
 }
 
@@ -349,8 +369,16 @@ extern "C" int b200moe_router_topk_backward(const float* dweights, const void* l
   if (rc || rows == 0) return rc;
   if (!dweights || !ids || !dlogits) return fail(B200MOE_E_NULL, "router_topk_backward: dweights, ids and dlogits are required");
   if ((uintptr_t)dlogits & 15) return fail(B200MOE_E_ALIGN, "router_topk_backward: dlogits must start on a 16-byte boundary");
-  router_grad_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream_v>>>(dweights, logits, dtype, ids, rows, experts, ld, topk,
-                                                                                     score == B200MOE_SCORE_SIGMOID, normalize != 0, scale, dlogits);
+  const bool whole_row = score == B200MOE_SCORE_SOFTMAX && !normalize;
+  const int lanes = whole_row || topk > 16 ? 32 : (topk > 8 ? 16 : 8);
+  const unsigned grid = (unsigned)((rows + 8 * (32 / lanes) - 1) / (8 * (32 / lanes)));
+#define B200_ROUTER_GRAD(L)                                                                                                                       \
+  router_grad_kernel<L><<<grid, 256, 0, (cudaStream_t)stream_v>>>(dweights, logits, dtype, ids, rows, experts, ld, topk, score == B200MOE_SCORE_SIGMOID, \
+                                                                  normalize != 0, scale, dlogits)
+  if (lanes == 8) B200_ROUTER_GRAD(8);
+  else if (lanes == 16) B200_ROUTER_GRAD(16);
+  else B200_ROUTER_GRAD(32);
+#undef B200_ROUTER_GRAD
   B200_CUDA_CHECK(cudaGetLastError());
   return B200MOE_OK;
 }
