@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import on_stream
+from .ops import call_on
 
 _TYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _GLU = {"swiglu": _lib.ACT_SWIGLU, "geglu": _lib.ACT_GEGLU}
@@ -32,34 +32,33 @@ def _check_x(x: torch.Tensor) -> Tuple[int, int]:
         raise ValueError("all tensors must live on a CUDA device")
     if x.dtype not in _TYPES:
         raise NotImplementedError(f"x dtype {x.dtype} is not built (bf16 and fp16 are)")
-    if x.dim() != 2:
-        raise ValueError(f"x must be a 2-D tensor [tokens, k], got shape {tuple(x.shape)}")
-    return x.shape
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"x must be a 2-D tensor [tokens, k], got shape {tuple(shape)}")
+    return shape
 
 
 def _pitch(name: str, t: torch.Tensor, shape, dtype, device) -> int:
     """Row pitch of a ``shape`` tensor with contiguous rows."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} lives on {t.device}, x on {device}")
     rows, cols = shape
-    if cols > 1 and rows > 0 and t.stride(1) != 1:
+    pitch, step = t.stride()
+    if step != 1 and cols > 1 and rows > 0:
         raise ValueError(f"{name} must have contiguous rows")
     # the pitch of a single row is free: the next multiple of 8
-    return t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
+    return pitch if rows > 1 else (cols + 7) // 8 * 8
 
 
 def _weight(name: str, w: torch.Tensor, k: int, x: torch.Tensor) -> int:
-    if w.dim() != 2 or w.shape[1] != k:
-        raise ValueError(f"{name} must have shape [n, {k}], got {tuple(w.shape)}")
-    return _pitch(name, w, tuple(w.shape), x.dtype, x.device)
-
-
-def _launch(fn: str, args: _lib.DenseArgs, stream: int) -> None:
-    _lib.check(getattr(_lib.load(), fn)(ctypes.byref(args), stream))
+    shape = w.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"{name} must have shape [n, {k}], got {tuple(shape)}")
+    return _pitch(name, w, shape, x.dtype, x.device)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_func: str = "swiglu", return_preact: bool = False, stream=None):
@@ -77,17 +76,19 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_fun
     if w_up.shape != w_gate.shape:
         raise ValueError("w_gate and w_up must have equal shapes")
     n = w_gate.shape[0]
-    with on_stream(x.device, stream) as s:
-        h = torch.empty((m, n), dtype=x.dtype, device=x.device)
-        gate = up = None
-        if return_preact:
-            gate, up = torch.empty_like(h), torch.empty_like(h)
+
+    def launch(s):
+        h = x.new_empty((m, n))
+        gate, up = (torch.empty_like(h), torch.empty_like(h)) if return_preact else (None, None)
         t = _TYPES[x.dtype]
-        _launch("b200moe_gated_ffn", _lib.DenseArgs(
-            x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), y=h.data_ptr(), pre0=gate.data_ptr() if return_preact else None,
-            pre1=up.data_ptr() if return_preact else None, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g, ld_w1=ld_u, ld_y=n, ld_pre0=n, ld_pre1=n,
-            dtype=t, y_dtype=t, act=_GLU[act_func]), s)  # fmt: skip
-    return (h, gate, up) if return_preact else h
+        args = _lib.DenseArgs(x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), y=h.data_ptr(), m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g, ld_w1=ld_u,
+                              ld_y=n, ld_pre0=n, ld_pre1=n, dtype=t, y_dtype=t, act=_GLU[act_func])  # fmt: skip
+        if return_preact:
+            args.pre0, args.pre1 = gate.data_ptr(), up.data_ptr()
+        _lib.check(_lib.load().b200moe_gated_ffn(ctypes.byref(args), s))
+        return (h, gate, up) if return_preact else h
+
+    return call_on(x.device, stream, launch)
 
 
 def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
@@ -103,17 +104,21 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
         raise ValueError("w_gate and w_up must have equal shapes")
     n = w_gate.shape[0]
     lds = [_pitch(name, v, (m, n), x.dtype, x.device) for name, v in (("dh", dh), ("gate", gate), ("up", up))]
-    with on_stream(x.device, stream) as s:
-        dx = torch.empty((m, k), dtype=x.dtype, device=x.device)
-        dw_gate, dw_up = torch.empty((n, k), dtype=x.dtype, device=x.device), torch.empty((n, k), dtype=x.dtype, device=x.device)
-        need = _lib.load().b200moe_dense_workspace_bytes(m, n, 1)
-        work = torch.empty(need, dtype=torch.uint8, device=x.device)
+
+    def launch(s):
+        lib = _lib.load()
+        dx, dw_gate, dw_up = x.new_empty((m, k)), x.new_empty((n, k)), x.new_empty((n, k))
+        need = lib.b200moe_dense_workspace_bytes(m, n, 1)
+        work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
-        _launch("b200moe_gated_ffn_backward", _lib.DenseArgs(
+        args = _lib.DenseArgs(
             x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), dy=dh.data_ptr(), pre0=gate.data_ptr(), pre1=up.data_ptr(), dx=dx.data_ptr(),
             dw0=dw_gate.data_ptr(), dw1=dw_up.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g,
-            ld_w1=ld_u, ld_dy=lds[0], ld_pre0=lds[1], ld_pre1=lds[2], dtype=t, y_dtype=t, act=_GLU[act_func]), s)  # fmt: skip
-    return dx, dw_gate, dw_up
+            ld_w1=ld_u, ld_dy=lds[0], ld_pre0=lds[1], ld_pre1=lds[2], dtype=t, y_dtype=t, act=_GLU[act_func])  # fmt: skip
+        _lib.check(lib.b200moe_gated_ffn_backward(ctypes.byref(args), s))
+        return dx, dw_gate, dw_up
+
+    return call_on(x.device, stream, launch)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act_func: Optional[str] = None,
@@ -138,16 +143,24 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         if bias.dtype not in (x.dtype, torch.float32):
             raise NotImplementedError(f"bias dtype {bias.dtype} is not built for {x.dtype} inputs (their own type and float32 are)")
     ld_r = 0 if residual is None else _pitch("residual", residual, (m, n), x.dtype, x.device)
-    with on_stream(x.device, stream) as s:
-        y = torch.empty((m, n), dtype=out_dtype, device=x.device)
-        z = torch.empty((m, n), dtype=x.dtype, device=x.device) if return_preact else None
+
+    def launch(s):
+        y = x.new_empty((m, n), dtype=out_dtype)
         t = _TYPES[x.dtype]
-        _launch("b200moe_linear", _lib.DenseArgs(
-            x=x.data_ptr(), w0=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
-            residual=None if residual is None else residual.data_ptr(), y=y.data_ptr(), pre0=z.data_ptr() if return_preact else None, m=m, n=n, k=k,
-            ld_x=ld_x, ld_w0=ld_w, ld_residual=ld_r, ld_y=n, ld_pre0=n, dtype=t, y_dtype=_lib.DTYPE_F32 if out_dtype == torch.float32 else t,
-            bias_dtype=t if bias is None or bias.dtype == x.dtype else _lib.DTYPE_F32, act=_ACT[act_func]), s)  # fmt: skip
-    return (y, z) if return_preact else y
+        args = _lib.DenseArgs(x=x.data_ptr(), w0=weight.data_ptr(), y=y.data_ptr(), m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_w, ld_residual=ld_r, ld_y=n, ld_pre0=n,
+                              dtype=t, y_dtype=_lib.DTYPE_F32 if out_dtype == torch.float32 else t, bias_dtype=t, act=_ACT[act_func])  # fmt: skip
+        if bias is not None:
+            args.bias, args.bias_dtype = bias.data_ptr(), t if bias.dtype == x.dtype else _lib.DTYPE_F32
+        if residual is not None:
+            args.residual = residual.data_ptr()
+        z = None
+        if return_preact:
+            z = x.new_empty((m, n))
+            args.pre0 = z.data_ptr()
+        _lib.check(_lib.load().b200moe_linear(ctypes.byref(args), s))
+        return (y, z) if return_preact else y
+
+    return call_on(x.device, stream, launch)
 
 
 def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, preact: Optional[torch.Tensor] = None, act_func: Optional[str] = None,
@@ -169,14 +182,19 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
         if preact is None:
             raise ValueError("preact is required with an activation")
         ld_z = _pitch("preact", preact, (m, n), x.dtype, x.device)
-    with on_stream(x.device, stream) as s:
-        dx, dw = torch.empty((m, k), dtype=x.dtype, device=x.device), torch.empty((n, k), dtype=x.dtype, device=x.device)
-        db = torch.empty((n,), dtype=torch.float32, device=x.device) if bias_grad else None
-        need = _lib.load().b200moe_dense_workspace_bytes(m, n, 0)
-        work = torch.empty(need, dtype=torch.uint8, device=x.device)
+
+    def launch(s):
+        lib = _lib.load()
+        dx, dw = x.new_empty((m, k)), x.new_empty((n, k))
+        db = x.new_empty((n,), dtype=torch.float32) if bias_grad else None
+        need = lib.b200moe_dense_workspace_bytes(m, n, 0)
+        work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
-        _launch("b200moe_linear_backward", _lib.DenseArgs(
+        args = _lib.DenseArgs(
             x=x.data_ptr(), w0=weight.data_ptr(), dy=dy.data_ptr(), pre0=None if act_func is None else preact.data_ptr(), dx=dx.data_ptr(),
             dw0=dw.data_ptr(), dbias=None if db is None else db.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x,
-            ld_w0=ld_w, ld_dy=ld_dy, ld_pre0=ld_z, dtype=t, y_dtype=_lib.DTYPE_F32 if dy.dtype == torch.float32 else t, act=_ACT[act_func]), s)  # fmt: skip
-    return dx, dw, db
+            ld_w0=ld_w, ld_dy=ld_dy, ld_pre0=ld_z, dtype=t, y_dtype=_lib.DTYPE_F32 if dy.dtype == torch.float32 else t, act=_ACT[act_func])  # fmt: skip
+        _lib.check(lib.b200moe_linear_backward(ctypes.byref(args), s))
+        return dx, dw, db
+
+    return call_on(x.device, stream, launch)

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _stream_ptr, on_stream
+from .ops import _stream_ptr, call_on
 
 _LOGIT_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
@@ -20,16 +20,18 @@ _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
 def _check_logits(logits: torch.Tensor, score_func: str) -> int:
     """Row pitch of the router's logits."""
-    if not logits.is_cuda or logits.dim() != 2:
+    shape = logits.shape
+    if len(shape) != 2 or not logits.is_cuda:
         raise ValueError("logits must be a 2-D CUDA tensor [tokens, experts]")
     if logits.dtype not in _LOGIT_TYPES:
         raise NotImplementedError(f"logits dtype {logits.dtype} is not built (float32, bf16 and fp16 are)")
     if score_func not in _SCORES:
         raise ValueError(f"score_func must be 'softmax' or 'sigmoid', got {score_func!r}")
-    t, e = logits.shape
-    if e > 1 and t > 0 and logits.stride(1) != 1:
+    t, e = shape
+    pitch, step = logits.stride()
+    if step != 1 and e > 1 and t > 0:
         raise ValueError("logits must have contiguous rows")
-    return logits.stride(0) if t > 1 else e
+    return pitch if t > 1 else e
 
 
 def router_topk(logits: torch.Tensor, topk: int, score_func: str = "softmax", normalize: bool = True, bias: Optional[torch.Tensor] = None,
@@ -43,17 +45,21 @@ def router_topk(logits: torch.Tensor, topk: int, score_func: str = "softmax", no
     chosen scores; the bias decides the choice only.  ``E <= 1024``, ``topk <= 32``."""
     ld = _check_logits(logits, score_func)
     t, e = logits.shape
+    if topk < 0:
+        raise ValueError(f"topk must be positive, got {topk}")
     if bias is not None and (tuple(bias.shape) != (e,) or bias.dtype != torch.float32 or bias.device != logits.device or (e > 1 and bias.stride(0) != 1)):
         raise ValueError(f"bias must be a contiguous float32 [{e}] tensor on {logits.device}")
-    with on_stream(logits.device, stream) as s:
-        weights = torch.empty((t, topk), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((t, topk), dtype=torch.int32, device=logits.device)
+
+    def launch(s):
+        weights, ids = logits.new_empty((t, topk), dtype=torch.float32), logits.new_empty((t, topk), dtype=torch.int32)
         rc = _lib.load().b200moe_router_topk(
-            logits.data_ptr(), _LOGIT_TYPES[logits.dtype], t, e, ld, None if bias is None else bias.data_ptr(), topk, _SCORES[score_func], int(normalize),
+            logits.data_ptr(), _LOGIT_TYPES[logits.dtype], t, e, ld, None if bias is None else bias.data_ptr(), topk, _SCORES[score_func], bool(normalize),
             scale, weights.data_ptr(), ids.data_ptr(), s,
         )  # fmt: skip
         _lib.check(rc)
-    return weights, ids
+        return weights, ids
+
+    return call_on(logits.device, stream, launch)
 
 
 def router_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, score_func: str = "softmax", normalize: bool = True,
@@ -67,14 +73,17 @@ def router_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torc
         raise ValueError(f"ids must be a contiguous int32 [{t}, topk] tensor on {logits.device}")
     if dweights.shape != ids.shape or dweights.dtype != torch.float32 or dweights.device != logits.device or not dweights.is_contiguous():
         raise ValueError(f"dweights must be a contiguous float32 tensor of the ids' shape on {logits.device}")
-    with on_stream(logits.device, stream) as s:
-        dlogits = torch.empty((t, e), dtype=logits.dtype, device=logits.device)
+
+    def launch(s):
+        dlogits = logits.new_empty((t, e))
         rc = _lib.load().b200moe_router_topk_backward(
-            dweights.data_ptr(), logits.data_ptr(), _LOGIT_TYPES[logits.dtype], ids.data_ptr(), t, e, ld, ids.shape[1], _SCORES[score_func], int(normalize),
+            dweights.data_ptr(), logits.data_ptr(), _LOGIT_TYPES[logits.dtype], ids.data_ptr(), t, e, ld, ids.shape[1], _SCORES[score_func], bool(normalize),
             scale, dlogits.data_ptr(), s,
         )  # fmt: skip
         _lib.check(rc)
-    return dlogits
+        return dlogits
+
+    return call_on(logits.device, stream, launch)
 
 
 def route(expert_ids: torch.Tensor, num_experts: int, m_aligned: int = 128, stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

@@ -54,37 +54,20 @@ def _stream_ptr(stream) -> int:
     return int(stream)  # raw CUstream handle
 
 
-class on_stream:
-    """Enters ``device`` and ``stream`` (``None`` = the device's current stream; a torch stream or a raw CUstream
-    handle otherwise) and yields the raw handle.  What is allocated inside belongs to that stream, so neither outputs nor
-    a workspace that is dropped on return can be handed to another stream's work while the kernels still run."""
-
-    __slots__ = ("_device", "_stream", "_entered")
-
-    def __init__(self, device: torch.device, stream=None):
-        self._device, self._stream, self._entered = device, stream, ()
-
-    def __enter__(self) -> int:
-        stream = self._stream
-        if stream is None and self._device.index == torch.cuda.current_device():
-            return torch._C._cuda_getCurrentRawStream(self._device.index)  # (the public way builds a Stream object: 3 us)
-        guard = torch.cuda.device(self._device)
-        guard.__enter__()
-        self._entered = (guard,)
+def call_on(device: torch.device, stream, fn):
+    """``fn(raw stream handle)`` with ``device`` and ``stream`` current (``None`` = the device's current stream; a torch
+    stream or a raw CUstream handle otherwise).  What ``fn`` allocates belongs to that stream, so neither outputs nor a
+    workspace that is dropped on return can be handed to another stream's work while the kernels still run."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return fn(torch._C._cuda_getCurrentRawStream(device.index))  # (the public way builds a Stream object: 3 us)
+    with torch.cuda.device(device):
         if stream is None:
-            return torch.cuda.current_stream().cuda_stream
+            return fn(torch._C._cuda_getCurrentRawStream(device.index))
         if not isinstance(stream, torch.cuda.Stream):
             raw = int(stream)
-            stream = torch.cuda.ExternalStream(raw, device=self._device) if raw else torch.cuda.default_stream(self._device)
-        scope = torch.cuda.stream(stream)
-        scope.__enter__()
-        self._entered = (guard, scope)
-        return stream.cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        for scope in reversed(self._entered):
-            scope.__exit__(*exc)
-        self._entered = ()
+            stream = torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device)
+        with torch.cuda.stream(stream):
+            return fn(stream.cuda_stream)
 
 
 def _require_cuda(*tensors):
