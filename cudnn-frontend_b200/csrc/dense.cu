@@ -523,8 +523,10 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
 constexpr int PAIR_THREADS = 320;
 constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = 2 * DENSE_A_BYTES;
-constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE_BYTES + 1024;
 constexpr int PAIR_EPI_WARPS = 8;
+constexpr int PAIR_BOX = 32 * 32 * 2;  // a block of 32 rows x 32 columns of the output
+constexpr int PAIR_STAGING = PAIR_STAGES * PAIR_STAGE_BYTES;  // two blocks per epilogue warp
+constexpr int PAIR_SMEM = PAIR_STAGING + PAIR_EPI_WARPS * 2 * PAIR_BOX + 1024;
 constexpr int ST_PAIR_EMPTY = 411, ST_PAIR_FULL = 412, ST_PAIR_ACC_EMPTY = 413, ST_PAIR_ACC_FULL = 414, ST_PAIR_DRAIN = 415;
 
 struct PairJob {
@@ -535,7 +537,7 @@ struct PairJob {
   int tiles;
   int raster;                 // row tiles of a raster group: the group's rows of A stay in L2 while its columns pass
   uint32_t idesc;
-  int vec;                    // output (and residual, pre-activation) rows may be accessed 16 bytes at a time
+  int tma_store;              // the outputs (and pre-activations) have tensor maps: 16-byte aligned base and pitch
   void* out[2];
   int64_t ld_out;
 };
@@ -551,11 +553,14 @@ struct PairParams {
   const void* bias;
   const void* residual;
   int64_t ld_res;
+  int vec_res;                // residual rows may be read 16 bytes at a time
   uint64_t wait_limit_ns;
 };
 
 struct PairMaps {
   DenseMaps job[2];
+  CUtensorMap out[2][2];  // of each job: the outputs
+  CUtensorMap pre[2];
 };
 
 struct PairTile {
@@ -608,22 +613,61 @@ __device__ __forceinline__ void act_x32(float* v, int act) {
   }
 }
 
-// 32 values to 16-bit memory
-__device__ __forceinline__ void store16x32(void* base, int64_t o, const float* v, int count, bool f16, bool vec) {
-  uint16_t* d = reinterpret_cast<uint16_t*>(base) + o;
-  if (vec && count >= 32) {
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+// all but the thread's latest bulk copy have finished reading shared memory
+__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+__device__ __forceinline__ void st_shared_u32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// One warp's block of 32 rows x 32 columns to 16-bit memory: lane = row, v[] = its columns.  Stored from registers, every
+// instruction would touch 32 lines (7000 cycles for a tile of 128 x 256, measured as 87 us for 896 tiles); so the block goes
+// through shared memory (two blocks in turn, 64-byte swizzle: 16-byte writes without bank conflicts) and leaves as one bulk
+// copy, or, where the output has no tensor map, row by row with neighbouring lanes on neighbouring columns.
+struct BlockWriter {
+  uint32_t staging;  // this warp's two blocks
+  int turn;
+  int lane;
+  bool f16;
+  __device__ __forceinline__ void write(const float* v, const CUtensorMap* map, void* base, int64_t ld, bool tma, int row0, int rows, int col, int cols) {
+    const uint32_t block = staging + (uint32_t)(turn * PAIR_BOX);
+    turn ^= 1;
+    if (tma) {
+      if (lane == 0) bulk_wait_read1();  // the copy before the last one used this block
+    }
+    __syncwarp();
+    const uint32_t line = block + (uint32_t)(lane * 64), swz = (uint32_t)((lane >> 1) & 3);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float* w = v + 8 * q;
-      reinterpret_cast<uint4*>(d)[q] = make_uint4(pack16x2_from_float(w[0], w[1], f16), pack16x2_from_float(w[2], w[3], f16),
-                                                  pack16x2_from_float(w[4], w[5], f16), pack16x2_from_float(w[6], w[7], f16));
+      st_shared_u32x4(line + (((uint32_t)q ^ swz) << 4), pack16x2_from_float(w[0], w[1], f16), pack16x2_from_float(w[2], w[3], f16),
+                      pack16x2_from_float(w[4], w[5], f16), pack16x2_from_float(w[6], w[7], f16));
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < count) store16(base, o + j, v[j], f16);
+    if (tma) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (row0 < rows && col < cols) tma_store_2d(map, block, col, row0);
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      const int count = min(32, rows - row0);
+      uint16_t* dst = reinterpret_cast<uint16_t*>(base) + (int64_t)row0 * ld + col + lane;
+      if (col + lane < cols) {
+        for (int r = 0; r < count; ++r, dst += ld) {
+          const uint32_t at = block + (uint32_t)(r * 64) + ((((uint32_t)lane >> 3) ^ (uint32_t)((r >> 1) & 3)) << 4) + (uint32_t)(lane & 7) * 2;
+          uint16_t h;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
+          *dst = h;
+        }
+      }
+      __syncwarp();
+    }
   }
-}
+};
 
 template <int kEpi>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
@@ -762,12 +806,14 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     // ---- epilogue ---------------------------------------------------------------------------------------
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const bool f16 = p.f16 != 0;
+    BlockWriter writer = {ring + PAIR_STAGING + (uint32_t)((warp - 2) * 2 * PAIR_BOX), 0, lane, f16};
     PairTile t;
     for (int i = 0; pair_tile(p, pair, pairs, i, t); ++i) {
       const PairJob& j = p.job[t.job];
-      const int row = t.row_tile * 256 + rank * 128 + quarter * 32 + lane;
-      const bool row_ok = row < j.rows;
-      const bool vec = j.vec != 0;
+      const int row0 = t.row_tile * 256 + rank * 128 + quarter * 32;  // this warp's 32 rows
+      const int row = row0 + lane;
+      const int rows = j.rows, cols = j.cols;
+      const bool tma = j.tma_store != 0;
       if (!__all_sync(0xffffffffu, mbar_wait<true>(acc_full_bar(i & 1), (uint32_t)(i >> 1) & 1u, wc, ST_PAIR_ACC_FULL))) break;
       tc_fence_after();
       const uint32_t acc = tmem + (uint32_t)(i & 1) * 256u + ((uint32_t)(quarter * 32) << 16);
@@ -780,7 +826,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         tmem_ld_32x32(acc + in_tile, v);
         if constexpr (kEpi == DENSE_GLU) tmem_ld_32x32(acc + 128 + in_tile, u);
         const int col = t.col_tile * (kEpi == DENSE_GLU ? 128 : 256) + in_tile;
-        const int count = row_ok ? min(32, j.cols - col) : 0;  // columns of this chunk that exist
         tmem_ld_wait();
         reg_fence32(v);
         if constexpr (kEpi == DENSE_GLU) reg_fence32(u);
@@ -790,27 +835,26 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_to_cta(acc_empty_bar(i & 1), 0));
         }
-        if (count <= 0) continue;
-        const int64_t o = (int64_t)row * j.ld_out + col;
+        if (row0 >= rows || col >= cols) continue;  // (the whole warp)
         if constexpr (kEpi == DENSE_GLU) {
           if (p.pre[0]) {
-            store16x32(p.pre[0], (int64_t)row * p.ld_pre[0] + col, v, count, f16, vec);
-            store16x32(p.pre[1], (int64_t)row * p.ld_pre[1] + col, u, count, f16, vec);
+            writer.write(v, &maps.pre[0], p.pre[0], p.ld_pre[0], tma, row0, rows, col, cols);
+            writer.write(u, &maps.pre[1], p.pre[1], p.ld_pre[1], tma, row0, rows, col, cols);
           }
 #pragma unroll
           for (int q = 0; q < 32; ++q) v[q] = glu_f(v[q], u[q], p.act);
-          store16x32(j.out[0], o, v, count, f16, vec);
         } else if constexpr (kEpi == DENSE_LINEAR) {
+          const int count = row < rows ? min(32, cols - col) : 0;  // of this lane's columns, those that exist
           if (p.bias) {
 #pragma unroll
             for (int q = 0; q < 32; ++q)
               if (q < count) v[q] += p.bias_f32 ? __ldg(reinterpret_cast<const float*>(p.bias) + col + q) : load16(p.bias, col + q, f16);
           }
-          if (p.pre[0]) store16x32(p.pre[0], (int64_t)row * p.ld_pre[0] + col, v, count, f16, vec);
+          if (p.pre[0]) writer.write(v, &maps.pre[0], p.pre[0], p.ld_pre[0], tma, row0, rows, col, cols);
           act_x32(v, p.act);
           if (p.residual) {
             const int64_t ro = (int64_t)row * p.ld_res + col;
-            if (vec && count >= 32) {
+            if (p.vec_res && count >= 32) {
               const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.residual) + ro);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
@@ -829,12 +873,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
                 if (q < count) v[q] += load16(p.residual, ro + q, f16);
             }
           }
-          store16x32(j.out[0], o, v, count, f16, vec);
-        } else {
-          store16x32(j.out[t.which], o, v, count, f16, vec);
         }
+        writer.write(v, &maps.out[t.job][t.which], j.out[t.which], j.ld_out, tma, row0, rows, col, cols);
       }
     }
+    if (lane == 0) bulk_wait_all();  // the copies out of this CTA's shared memory
     __syncwarp();
   }
   tc_fence_before();
@@ -986,6 +1029,8 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
 static int dense_encode(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int f16) {
   uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
   uint64_t strides[1] = {(uint64_t)ld * 2};
@@ -1103,7 +1148,13 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   return dense_launch_tile<false, DENSE_STORE, false>(maps, p, grid, stream);
 }
 
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// a matrix that the pair kernel writes in blocks of 32 x 32
+static int dense_encode_block(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int f16) {
+  uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows};
+  uint64_t strides[1] = {(uint64_t)ld * 2};
+  uint32_t box[2] = {32, 32};
+  return encode_map(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
 
 template <int kEpi>
 static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pairs, cudaStream_t stream) {
@@ -1121,7 +1172,7 @@ static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pair
 }
 
 // One launch of the pair kernel over one or two products of the same epilogue; operand A's rows are the result's rows.
-// `p` arrives with its epilogue fields and each job's outputs, pitch and `vec` set.
+// `p` arrives with its epilogue fields and each job's outputs and pitch set.
 static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceInfo* di, cudaStream_t stream) {
   PairMaps maps;
   memset(&maps, 0, sizeof(maps));
@@ -1148,16 +1199,30 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
       int rc = dense_encode(&maps.job[i].a[q], g[i].a[q].base, g[i].a[q].outer, g[i].a[q].inner, g[i].a[q].ld, g[i].a_mn ? 64 : 128, p.f16);
       if (rc) return rc;
     }
+    const int no = j.stacked ? 2 : 1;
+    j.tma_store = j.ld_out % 8 == 0 && aligned16(j.out[0]) && aligned16(j.out[1]);
+    for (int q = 0; q < 2; ++q) j.tma_store = j.tma_store && (!p.pre[q] || (aligned16(p.pre[q]) && p.ld_pre[q] % 8 == 0));
+    if (j.tma_store) {
+      for (int q = 0; q < no; ++q) {
+        int rc = dense_encode_block(&maps.out[i][q], j.out[q], j.rows, j.cols, j.ld_out, p.f16);
+        if (rc) return rc;
+      }
+      for (int q = 0; q < 2 && p.pre[q]; ++q) {
+        int rc = dense_encode_block(&maps.pre[q], p.pre[q], j.rows, j.cols, p.ld_pre[q], p.f16);
+        if (rc) return rc;
+      }
+    }
     for (int q = 0; q < nb; ++q) {
       int rc = dense_encode(&maps.job[i].b[q], g[i].b[q].base, g[i].b[q].outer, g[i].b[q].inner, g[i].b[q].ld, g[i].b_mn ? 64 : 128, p.f16);
       if (rc) return rc;
     }
   }
-  // time of a tile in stages; below 8 its epilogue takes longer than its products
-  auto cost = [&](int i) { return std::max(8, p.job[i].k_tiles); };
+  // time of a tile in stages; below 5 its epilogue takes longer than its products
+  auto cost = [&](int i) { return std::max(5, p.job[i].k_tiles); };
   if (jobs > 1 && cost(1) > cost(0)) {  // long tiles first, the short ones fill the rest
     std::swap(p.job[0], p.job[1]);
     std::swap(maps.job[0], maps.job[1]);
+    std::swap(maps.out[0], maps.out[1]);
   }
   const int total = p.job[0].tiles + (jobs > 1 ? p.job[1].tiles : 0);
   const int pairs = std::max(1, std::min(di->sm_count / 2, total));
@@ -1251,14 +1316,12 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
     q.pre[1] = a->pre1;
     q.ld_pre[0] = a->ld_pre0;
     q.ld_pre[1] = a->ld_pre1;
-    q.job[0].vec = aligned16(a->y) && a->ld_y % 8 == 0 && aligned16(a->pre0) && aligned16(a->pre1) && (!a->pre0 || a->ld_pre0 % 8 == 0) &&
-                   (!a->pre1 || a->ld_pre1 % 8 == 0);
     if (!gated) {
       q.bias = a->bias;
       q.bias_f32 = a->bias_dtype == B200MOE_DTYPE_F32;
       q.residual = a->residual;
       q.ld_res = a->ld_residual;
-      if (a->residual && (!aligned16(a->residual) || a->ld_residual % 8 != 0)) q.job[0].vec = 0;
+      q.vec_res = aligned16(a->residual) && a->ld_residual % 8 == 0;
     }
     return dense_pair_gemm(&g, 1, q, di, stream);
   }
@@ -1326,8 +1389,7 @@ static int dense_grad_products(const b200moe_dense_args* a, int count, const voi
         x.cols = a->k;
         x.red = a->n;
         q.job[jobs].out[0] = a->dx;
-        q.job[jobs].ld_out = a->k;
-        q.job[jobs++].vec = aligned16(a->dx);
+        q.job[jobs++].ld_out = a->k;
       }
       if (a->dw0) {
         DenseGemm& w = g[jobs];
@@ -1340,8 +1402,7 @@ static int dense_grad_products(const b200moe_dense_args* a, int count, const voi
         w.red = a->m;
         q.job[jobs].out[0] = a->dw0;
         q.job[jobs].out[1] = a->dw1;
-        q.job[jobs].ld_out = a->k;
-        q.job[jobs++].vec = aligned16(a->dw0) && aligned16(a->dw1);
+        q.job[jobs++].ld_out = a->k;
       }
       return dense_pair_gemm(g, jobs, q, di, stream);
     }
