@@ -11,6 +11,7 @@
 #include <atomic>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "b200moe.h"
 #include "common.cuh"
@@ -37,6 +38,8 @@ struct DenseParams {
   int split;                 // CTAs of a cluster that share a tile's reduction
   int stages, stage_bytes;
   int reduce_offset;         // where the partial sums meet, from the start of the ring
+  int reduce_in_ring;        // they meet in the ring itself
+  int smem_bytes;
   int a_mn, b_mn;            // operand is MN-major
   int stacked;               // row tiles beyond row_tiles belong to the second A operand and the second output
   uint32_t idesc;
@@ -172,6 +175,21 @@ __device__ __forceinline__ float act_grad_f(float z, int act) {
   }
 }
 
+// the activation on kN values: one uniform branch, so that v[] stays in registers
+template <int kN>
+__device__ __forceinline__ void act_values(float* v, int act) {
+  if (act == B200MOE_ACT_RELU) {
+#pragma unroll
+    for (int q = 0; q < kN; ++q) v[q] = act_f(v[q], B200MOE_ACT_RELU);
+  } else if (act == B200MOE_ACT_SILU) {
+#pragma unroll
+    for (int q = 0; q < kN; ++q) v[q] = act_f(v[q], B200MOE_ACT_SILU);
+  } else if (act == B200MOE_ACT_GELU) {
+#pragma unroll
+    for (int q = 0; q < kN; ++q) v[q] = act_f(v[q], B200MOE_ACT_GELU);
+  }
+}
+
 // ---------------------------------------------------------------------------------------
 // One tile per CTA.  The tile's reduction may be shared by the CTAs of a cluster: each walks its part of the
 // k-tiles, sends its partial sums to the owners of the columns through distributed shared memory, and every CTA
@@ -191,12 +209,13 @@ __device__ __forceinline__ float act_grad_f(float z, int act) {
 // warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (TMEM lane quarter x every other 16 columns)
 // ---------------------------------------------------------------------------------------
 constexpr int DENSE_THREADS = 320;
-constexpr int DENSE_SMEM = 112 * 1024;  // per CTA, two CTAs to an SM
+constexpr int DENSE_SMEM = 112 * 1024;       // per CTA, two CTAs to an SM
+constexpr int DENSE_SMEM_ALONE = 225 * 1024;  // where every CTA has an SM of its own
 constexpr int kSegTiles = 8;
-constexpr int kSegCols = 64;
+constexpr int kSegCols = 128;
 
 template <bool kTrans, int kEpi, bool kSeg>
-__global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
+__global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t s_bars[2 * 16 + 4];
@@ -255,40 +274,57 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
 
   if (warp == 0) {
     // ---- producer -----------------------------------------------------------------------
+    // (stage, parity and addresses run along: a division by the number of stages in this loop and the issuer's made a stage
+    // cost 700 cycles whatever it held)
+    const uint32_t stage_bytes = (uint32_t)p.stage_bytes, ring_end = ring + (uint32_t)stages * stage_bytes;
+    const bool a_mn = !kGlu && p.a_mn != 0, b_mn = p.b_mn != 0, b_two = C > 64;
+    int kt = kt0;
+    const CUtensorMap *ma = &maps.a[kGlu ? 0 : which], *mb = &maps.b[0];
+    int chain_left = p.chain_tiles - kt;
+    if (chain_left <= 0) {
+      kt -= p.chain_tiles;
+      ma = &maps.a[1];
+      mb = &maps.b[1];
+    }
+    int kc = kt * DENSE_BK;
+    uint32_t dst = ring, fb = full_bar(0), eb = empty_bar(0), parity = 1;
     int issued = 0;
     for (; issued < nk; ++issued) {
-      const int s = issued % stages;
-      const uint32_t phase = (uint32_t)(issued / stages) & 1u;
-      if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(s), phase ^ 1u, wc, ST_DENSE_EMPTY))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(eb, parity, wc, ST_DENSE_EMPTY))) break;
       if (elect_one()) {
-        const uint32_t fb = full_bar(s), dst = ring + (uint32_t)s * p.stage_bytes;
-        int kt = kt0 + issued, chain = 0;
-        if (kt >= p.chain_tiles) {
-          kt -= p.chain_tiles;
-          chain = 1;
-        }
-        const int kc = kt * DENSE_BK;
-        mbar_arrive_expect_tx(fb, (uint32_t)p.stage_bytes);
+        mbar_arrive_expect_tx(fb, stage_bytes);
         if constexpr (kGlu) {
-          tma_load_2d(dst, &maps.a[0], fb, kc, row0);
-          tma_load_2d(dst + 64 * 128, &maps.a[1], fb, kc, row0);
+          tma_load_2d(dst, ma, fb, kc, row0);
+          tma_load_2d(dst + 64 * 128, ma + 1, fb, kc, row0);
+        } else if (a_mn) {
+          tma_load_2d(dst, ma, fb, row0, kc);
+          tma_load_2d(dst + DENSE_SLAB, ma, fb, row0 + 64, kc);
         } else {
-          const CUtensorMap* m = &maps.a[chain | which];
-          if (p.a_mn) {
-            tma_load_2d(dst, m, fb, row0, kc);
-            tma_load_2d(dst + DENSE_SLAB, m, fb, row0 + 64, kc);
-          } else {
-            tma_load_2d(dst, m, fb, kc, row0);
-          }
+          tma_load_2d(dst, ma, fb, kc, row0);
         }
-        const CUtensorMap* m = &maps.b[chain];
-        if (p.b_mn) {
-          for (int q = 0; q < C / 64; ++q) tma_load_2d(dst + DENSE_A_BYTES + q * DENSE_SLAB, m, fb, col0 + 64 * q, kc);
+        if (b_mn) {
+          tma_load_2d(dst + DENSE_A_BYTES, mb, fb, col0, kc);
+          if (b_two) tma_load_2d(dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
         } else {
-          tma_load_2d(dst + DENSE_A_BYTES, m, fb, kc, col0);
+          tma_load_2d(dst + DENSE_A_BYTES, mb, fb, kc, col0);
         }
       }
       __syncwarp();
+      kc += DENSE_BK;
+      if (--chain_left == 0) {
+        kc = 0;
+        ma = &maps.a[1];
+        mb = &maps.b[1];
+      }
+      dst += stage_bytes;
+      fb += 8;
+      eb += 8;
+      if (dst == ring_end) {
+        dst = ring;
+        fb = full_bar(0);
+        eb = empty_bar(0);
+        parity ^= 1u;
+      }
     }
     if (issued < nk) {
       // a wait gave up: the copies already issued still write this CTA's shared memory, so they are waited for
@@ -305,29 +341,40 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     const uint32_t a_lo0 = ((ring >> 4) & 0x3FFFu) | (p.a_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
     const uint32_t b_lo0 = (((ring + DENSE_A_BYTES) >> 4) & 0x3FFFu) | (p.b_mn ? (uint32_t)(DENSE_SLAB >> 4) << 16 : 1u << 16);
     const uint32_t a_step = p.a_mn ? (16u * 128u) >> 4 : 2u, b_step = p.b_mn ? (16u * 128u) >> 4 : 2u;
+    const uint32_t stage_step = (uint32_t)p.stage_bytes >> 4, idesc = p.idesc;
     auto desc = [](uint32_t lo) { return ((uint64_t)HI << 32) | lo; };
     bool ok = true;
-    int seg = 0;
+    int seg = 0, in_seg = 0, stage = 0;
+    uint32_t parity = 0, a_lo = a_lo0, b_lo = b_lo0;
     for (int i = 0; i < nk && ok; ++i) {
-      const int s = i % stages;
-      const int in_seg = kSeg ? i % kSegTiles : i;
       const uint32_t acc = tmem + (kSeg ? (uint32_t)((seg & 1) * C) : 0u);
       if (kSeg && in_seg == 0 && seg >= 2) {
         // the epilogue has taken the segment that used this accumulator
         if (!__all_sync(0xffffffffu, mbar_wait(acc_empty_bar(seg & 1), (uint32_t)((seg >> 1) - 1) & 1u, wc, ST_DENSE_ACC))) { ok = false; break; }
         tc_fence_after();
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), (uint32_t)(i / stages) & 1u, wc, ST_DENSE_FULL))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), parity, wc, ST_DENSE_FULL))) { ok = false; break; }
       const bool seg_end = i + 1 == nk || (kSeg && in_seg == kSegTiles - 1);
       if (elect_one()) {
-        const uint32_t off = ((uint32_t)s * p.stage_bytes) >> 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma_f16_ss<false>(acc, desc(a_lo0 + off + j * a_step), desc(b_lo0 + off + j * b_step), p.idesc, (in_seg | j) != 0);
-        tc_commit(empty_bar(s));
+        for (int j = 0; j < 4; ++j) mma_f16_ss<false>(acc, desc(a_lo + j * a_step), desc(b_lo + j * b_step), idesc, (in_seg | j) != 0);
+        tc_commit(empty_bar(stage));
         if (seg_end) tc_commit(acc_full_bar(kSeg ? seg & 1 : 0));
       }
       __syncwarp();
-      if (seg_end) ++seg;
+      ++in_seg;
+      if (seg_end) {
+        ++seg;
+        if (kSeg) in_seg = 0;
+      }
+      a_lo += stage_step;
+      b_lo += stage_step;
+      if (++stage == stages) {
+        stage = 0;
+        parity ^= 1u;
+        a_lo = a_lo0;
+        b_lo = b_lo0;
+      }
     }
     __syncwarp();
   }
@@ -389,52 +436,101 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
       }
     }
   };
-  // kTrans, one element: feature `row`, token col0 + c
+  // kTrans: kN values of feature `row` for the tokens col0 + c0 + j step, of which the first `count` exist; v = the accumulator
+  // (GLU: the gate's), u = the up projection's.  Every choice is a branch around a whole loop.
+  auto finish = [&](auto size, int row, int c0, int step, int count, float bias, float* v, const float* u) {
+    constexpr int kN = decltype(size)::value;
+    const int64_t t0 = col0 + c0;
+    auto put = [&](void* base, int64_t ld, const float* w) {
+      uint16_t* d = reinterpret_cast<uint16_t*>(base) + t0 * ld + row;
+      const int64_t hop = ld * step;
+      if (f16) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j, d += hop)
+          if (j < count) *d = __half_as_ushort(__float2half_rn(w[j]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j, d += hop)
+          if (j < count) *d = __bfloat16_as_ushort(__float2bfloat16_rn(w[j]));
+      }
+    };
+    if constexpr (kGlu) {
+      if (p.pre[0]) {
+        put(p.pre[0], p.ld_pre[0], v);
+        put(p.pre[1], p.ld_pre[1], u);
+      }
+#pragma unroll
+      for (int j = 0; j < kN; ++j) v[j] = glu_f(v[j], u[j], p.act);
+    } else {
+      float res[kN];
+      const bool has_res = p.residual != nullptr;
+      if (has_res) {
+        const uint16_t* r = reinterpret_cast<const uint16_t*>(p.residual) + t0 * p.ld_res + row;
+        const int64_t hop = p.ld_res * step;
+#pragma unroll
+        for (int j = 0; j < kN; ++j, r += hop) res[j] = j < count ? (f16 ? __half2float(__ushort_as_half(*r)) : __bfloat162float(__ushort_as_bfloat16(*r))) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < kN; ++j) v[j] += bias;
+      if (p.pre[0]) put(p.pre[0], p.ld_pre[0], v);
+      act_values<kN>(v, p.act);
+      if (has_res) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) v[j] += res[j];
+      }
+    }
+    if (p.out_f32) {
+      float* d = reinterpret_cast<float*>(p.out[0]) + t0 * p.ld_out + row;
+      const int64_t hop = p.ld_out * step;
+#pragma unroll
+      for (int j = 0; j < kN; ++j, d += hop)
+        if (j < count) *d = v[j];
+    } else {
+      put(p.out[0], p.ld_out, v);
+    }
+  };
   auto bias_at = [&](int row) -> float {
     if (kEpi != DENSE_LINEAR || !p.bias || row >= p.rows) return 0.0f;
     return p.bias_f32 ? reinterpret_cast<const float*>(p.bias)[row] : load16(p.bias, row, f16);
-  };
-  auto residual_at = [&](int row, int c) -> float {
-    return kEpi == DENSE_LINEAR && p.residual ? load16(p.residual, (int64_t)(col0 + c) * p.ld_res + row, f16) : 0.0f;
-  };
-  auto emit = [&](int row, int c, float v0, float v1, float res) {
-    const int64_t t = col0 + c;
-    float y;
-    if constexpr (kGlu) {
-      if (p.pre[0]) {
-        store16(p.pre[0], t * p.ld_pre[0] + row, v0, f16);
-        store16(p.pre[1], t * p.ld_pre[1] + row, v1, f16);
-      }
-      y = glu_f(v0, v1, p.act);
-    } else {
-      if (p.pre[0]) store16(p.pre[0], t * p.ld_pre[0] + row, v0, f16);
-      y = act_f(v0, p.act) + res;
-    }
-    if (p.out_f32) reinterpret_cast<float*>(p.out[0])[t * p.ld_out + row] = y;
-    else store16(p.out[0], t * p.ld_out + row, y, f16);
   };
 
   const int split = p.split;
   if (kGlu || split > 1) {
     // partial sums meet in shared memory: [rank][column of the owner's slice][row].  With one CTA that is the ring, which the
-    // products have left; with several a region of its own, since another CTA's products may still read its ring.
+    // products have left; with several a region of its own, since another CTA's products may still read its ring, or,
+    // where that would leave too few stages, the ring once all of the cluster's products are done.
     const int slice = (valid + split - 1) / split;  // columns that one CTA of the cluster finishes
     const uint32_t region = ring + p.reduce_offset;
     if (split > 1) {
       __syncwarp();
       cluster_wait();  // (of the arrival at the start)
+      if (p.reduce_in_ring) {
+        cluster_arrive();
+        cluster_wait();
+      }
     }
     if (warp >= 2 && ok) {
       each_chunk([&](int c0, const float* v) {
+        const int count = min(16, valid - c0);
+        if (split == 1) {
+          const uint32_t at = region + (uint32_t)((c0 * 128 + r_in_tile) * 4);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int c = c0 + j;
-          if (c < valid) {
-            if (split == 1) {
-              st_shared_f32(region + (uint32_t)((c * 128 + r_in_tile) * 4), v[j]);
-            } else {
-              const int owner = c / slice;
-              st_cluster_f32(map_to_cta(region, (uint32_t)owner) + (uint32_t)(((rank * slice + c - owner * slice) * 128 + r_in_tile) * 4), v[j]);
+          for (int j = 0; j < 16; ++j)
+            if (j < count) st_shared_f32(at + j * 512, v[j]);
+        } else {
+          int owner = c0 / slice, left = slice - (c0 - owner * slice);
+          const uint32_t base = region + (uint32_t)((rank * slice * 128 + r_in_tile) * 4);
+          uint32_t at = map_to_cta(base, (uint32_t)owner) + (uint32_t)((slice - left) * 512);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (j < count) {
+              st_cluster_f32(at, v[j]);
+              at += 512;
+              if (--left == 0) {
+                left = slice;
+                ++owner;
+                at = map_to_cta(base, (uint32_t)min(owner, split - 1));
+              }
             }
           }
         }
@@ -449,21 +545,35 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     }
     if (warp >= 2) {
       constexpr int kGroups = 256 / kTileRows;  // columns in flight
+      constexpr int kN = 8;
       const int t = (int)threadIdx.x - 64;
       const int r = t % kTileRows, row = row0 + r;
       const int c_begin = rank * slice, c_end = min(valid, c_begin + slice);
       if (row < p.rows) {
         const float* part = reinterpret_cast<const float*>(smem + p.reduce_offset) + r;
         const float bias = bias_at(row);
-        for (int c = c_begin + t / kTileRows; c < c_end; c += kGroups) {
-          const float res = residual_at(row, c);
-          float v0 = 0.0f, v1 = 0.0f;
+        for (int c = c_begin + t / kTileRows; c < c_end; c += kGroups * kN) {
+          const int count = (c_end - c + kGroups - 1) / kGroups;
+          float v[kN], u[kN];
+#pragma unroll
+          for (int j = 0; j < kN; ++j) v[j] = u[j] = 0.0f;
           for (int q = 0; q < split; ++q) {
-            v0 += part[(q * slice + c - c_begin) * 128];
-            if (kGlu) v1 += part[(q * slice + c - c_begin) * 128 + 64];
+            const float* src = part + (q * slice + c - c_begin) * 128;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              if (j < count) {
+                v[j] += src[j * kGroups * 128];
+                if (kGlu) u[j] += src[j * kGroups * 128 + 64];
+              }
+            }
           }
-          if constexpr (kTrans) emit(row, c, v0 + bias, v1, res);
-          else store16(p.out[which], (int64_t)row * p.ld_out + col0 + c, v0, f16);
+          if constexpr (kTrans) {
+            finish(std::integral_constant<int, kN>(), row, c, kGroups, count, bias, v, u);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+              if (j < count) store16(p.out[which], (int64_t)row * p.ld_out + col0 + c + j * kGroups, v[j], f16);
+          }
         }
       }
     }
@@ -474,12 +584,10 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
     each_chunk([&](int c0, const float* v) {
       if (!row_ok) return;
       if constexpr (kTrans) {
-        float res[16];
+        float w[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) res[j] = c0 + j < valid ? residual_at(row, c0 + j) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c0 + j < valid) emit(row, c0 + j, v[j] + bias, 0.0f, res[j]);
+        for (int j = 0; j < 16; ++j) w[j] = v[j];
+        finish(std::integral_constant<int, 16>(), row, c0, 1, min(16, valid - c0), bias, w, w);
       } else {
         const int64_t o = (int64_t)row * p.ld_out + col0 + c0;
         if (p.vec_store && c0 + 16 <= valid) {
@@ -508,11 +616,12 @@ __global__ void __launch_bounds__(DENSE_THREADS, 2) dense_tile_kernel(const __gr
 // ---------------------------------------------------------------------------------------
 // Large products: a persistent kernel of CTA pairs, one pair per two SMs.  A tile is 256 x 256 (cta_group::2: each CTA
 // holds 128 rows of A, 128 columns of B and the accumulator of its 128 rows), its two accumulators of 256 columns fill
-// TMEM, so the epilogue of one tile runs beside the products of the next.  Rows are tokens (or, for a weight's gradient,
+// TMEM, so the epilogue of one tile runs beside the products of the next.  Where tiles of that size would leave pairs
+// without work they have 128 columns (half the flops on three quarters of the bytes).  Rows are tokens (or, for a weight's gradient,
 // the weight's rows), so a thread of the epilogue holds 32 neighbouring columns of one output row.
 //
-// DENSE_GLU: the pair's first CTA loads 128 rows of the gate weights as its half of B, the second the same rows of the up
-// weights: accumulator columns [0, 128) are the gate, [128, 256) the up projection of the same 128 features.
+// DENSE_GLU: the pair's first CTA loads 128 (64) rows of the gate weights as its half of B, the second the same rows of the
+// up weights: the first half of the accumulator's columns are the gate, the second half the up projection of the same features.
 //
 // A launch walks one or two jobs (the two gradient products of a backward pass share a launch: the tiles of the second fill
 // the last wave of the first).  Tiles are dealt out in rounds; where the last round of job 0 leaves pairs idle, they
@@ -535,6 +644,7 @@ struct PairJob {
   int k_tiles, chain_tiles;
   int a_mn, b_mn, stacked;
   int tiles;
+  int tile_cols;              // accumulator columns of a tile: 256 or 128
   int raster;                 // row tiles of a raster group: the group's rows of A stay in L2 while its columns pass
   uint32_t idesc;
   int tma_store;              // the outputs (and pre-activations) have tensor maps: 16-byte aligned base and pitch
@@ -597,20 +707,6 @@ __device__ __forceinline__ bool pair_tile(const PairParams& p, int pair, int pai
   t.which = t.row_tile >= j.row_tiles ? 1 : 0;
   t.row_tile -= t.which * j.row_tiles;
   return true;
-}
-
-// the activation on 32 values: one uniform branch, so that v[] stays in registers
-__device__ __forceinline__ void act_x32(float* v, int act) {
-  if (act == B200MOE_ACT_RELU) {
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_RELU);
-  } else if (act == B200MOE_ACT_SILU) {
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_SILU);
-  } else if (act == B200MOE_ACT_GELU) {
-#pragma unroll
-    for (int q = 0; q < 32; ++q) v[q] = act_f(v[q], B200MOE_ACT_GELU);
-  }
 }
 
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int c0, int c1) {
@@ -727,8 +823,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       const PairJob& j = p.job[t.job];
       const DenseMaps& m = maps.job[t.job];
       const int a0 = t.row_tile * 256 + rank * 128;
-      const int b0 = kEpi == DENSE_GLU ? t.col_tile * 128 : t.col_tile * 256 + rank * 128;
+      const int half_cols = j.tile_cols / 2;  // this CTA's columns of B
+      const int b0 = kEpi == DENSE_GLU ? t.col_tile * half_cols : t.col_tile * j.tile_cols + rank * half_cols;
       const bool a_mn = j.a_mn != 0, b_mn = j.b_mn != 0;
+      const uint32_t bytes = 2u * (uint32_t)(DENSE_A_BYTES + half_cols * 128);
       for (int kt = 0; kt < j.k_tiles; ++kt) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, wc, ST_PAIR_EMPTY))) { ok = false; break; }
         if (elect_one()) {
@@ -738,7 +836,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           const uint32_t da = ring + stage * PAIR_STAGE_BYTES, db = da + DENSE_A_BYTES;
           const CUtensorMap* ma = &m.a[chain | t.which];
           const CUtensorMap* mb = &m.b[kEpi == DENSE_GLU ? rank : chain];
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * PAIR_STAGE_BYTES);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), bytes);
           if (a_mn) {
             tma_load_2d_pair(da, ma, fb, a0, kc);
             tma_load_2d_pair(da + DENSE_SLAB, ma, fb, a0 + 64, kc);
@@ -747,7 +845,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           }
           if (b_mn) {
             tma_load_2d_pair(db, mb, fb, b0, kc);
-            tma_load_2d_pair(db + DENSE_SLAB, mb, fb, b0 + 64, kc);
+            if (half_cols > 64) tma_load_2d_pair(db + DENSE_SLAB, mb, fb, b0 + 64, kc);
           } else {
             tma_load_2d_pair(db, mb, fb, kc, b0);
           }
@@ -817,19 +915,20 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       if (!__all_sync(0xffffffffu, mbar_wait<true>(acc_full_bar(i & 1), (uint32_t)(i >> 1) & 1u, wc, ST_PAIR_ACC_FULL))) break;
       tc_fence_after();
       const uint32_t acc = tmem + (uint32_t)(i & 1) * 256u + ((uint32_t)(quarter * 32) << 16);
-      constexpr int kChunks = kEpi == DENSE_GLU ? 2 : 4;
+      const int out_cols = kEpi == DENSE_GLU ? j.tile_cols / 2 : j.tile_cols;  // output columns of the tile
+      const int chunks = out_cols / 64;                                          // of 32 columns, in this warp's half
 #pragma unroll 1
-      for (int c = 0; c < kChunks; ++c) {
+      for (int c = 0; c < chunks; ++c) {
         __syncwarp();
         float v[32], u[kEpi == DENSE_GLU ? 32 : 1];
-        const int in_tile = half * (kChunks * 32) + c * 32;
+        const int in_tile = (half * chunks + c) * 32;
         tmem_ld_32x32(acc + in_tile, v);
-        if constexpr (kEpi == DENSE_GLU) tmem_ld_32x32(acc + 128 + in_tile, u);
-        const int col = t.col_tile * (kEpi == DENSE_GLU ? 128 : 256) + in_tile;
+        if constexpr (kEpi == DENSE_GLU) tmem_ld_32x32(acc + out_cols + in_tile, u);
+        const int col = t.col_tile * out_cols + in_tile;
         tmem_ld_wait();
         reg_fence32(v);
         if constexpr (kEpi == DENSE_GLU) reg_fence32(u);
-        if (c == kChunks - 1) {
+        if (c == chunks - 1) {
           // the accumulator is in registers: the issuer may overwrite it
           tc_fence_before();
           __syncwarp();
@@ -851,7 +950,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
               if (q < count) v[q] += p.bias_f32 ? __ldg(reinterpret_cast<const float*>(p.bias) + col + q) : load16(p.bias, col + q, f16);
           }
           if (p.pre[0]) writer.write(v, &maps.pre[0], p.pre[0], p.ld_pre[0], tma, row0, rows, col, cols);
-          act_x32(v, p.act);
+          act_values<32>(v, p.act);
           if (p.residual) {
             const int64_t ro = (int64_t)row * p.ld_res + col;
             if (p.vec_res && count >= 32) {
@@ -1087,12 +1186,39 @@ static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsign
   int dev = 0;
   B200_CUDA_CHECK(cudaGetDevice(&dev));
   if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
-    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM));
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM_ALONE));
     ready.fetch_or(1ull << (dev & 63));
   }
-  LaunchConfig c(grid, DENSE_THREADS, DENSE_SMEM, p.split, stream);
+  LaunchConfig c(grid, DENSE_THREADS, (size_t)p.smem_bytes, p.split, stream);
   B200_CUDA_CHECK(cudaLaunchKernelEx(&c.cfg, kern, maps, p));
   return B200MOE_OK;
+}
+
+// Columns of the tile kernel's tiles (as many as there are, up to 128; an MN-major B comes in slabs of 64) and the CTAs that
+// share a tile's reduction, by estimated time in nanoseconds: the stages that the busiest SM loads, at about 80 bytes / ns
+// (between 52 from HBM and 100 from L2, measured), plus what joining the partial sums costs.  5 us start and end a launch.
+struct TileShape {
+  int cols, split;
+  int64_t tiles;
+  double time;
+};
+static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
+  const int64_t tile_rows = g.dual ? 64 : 128;
+  const int64_t rows = (g.rows + tile_rows - 1) / tile_rows * (g.stacked ? 2 : 1);
+  const int64_t stages = (g.red + DENSE_BK - 1) / DENSE_BK * (g.chained ? 2 : 1);
+  TileShape best = {0, 0, 0, 0.0};
+  for (int c = 128; c >= (g.b_mn ? 64 : 16); c /= 2) {
+    if (c > 16 && c / 2 >= g.cols && c / 2 >= (g.b_mn ? 64 : 16)) continue;  // half as many hold them all
+    const int64_t tiles = rows * ((g.cols + c - 1) / c);
+    for (int split = 1; split <= DENSE_MAX_SPLIT && split * 4 <= std::max<int64_t>(4, stages); split *= 2) {
+      const int64_t per_sm = (tiles * split + di->sm_count - 1) / di->sm_count;
+      const double load = (double)per_sm * (double)((stages + split - 1) / split) * (DENSE_A_BYTES + c * 128) / 80.0;
+      const double finish = (double)((per_sm + 1) / 2) * (1000.0 + 16.0 * c) + (split > 1 ? 500.0 + 8.0 * c : 0.0);
+      const double time = 5000.0 + load + finish;
+      if (best.cols == 0 || time < best.time) best = {c, split, tiles, time};
+    }
+  }
+  return best;
 }
 
 // Shared part of every product: tiles, tensor maps, launch.  `p` arrives with its epilogue fields set.
@@ -1106,27 +1232,21 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   p.row_tiles = (int)((g.rows + tile_rows - 1) / tile_rows);
   p.chain_tiles = (int)((g.red + DENSE_BK - 1) / DENSE_BK);
   p.k_tiles = p.chain_tiles * (g.chained ? 2 : 1);
-  // Columns of a tile: as many as there are, up to 128 (float32 sums in registers: 64); halved while that leaves SMs
-  // without a tile (down to 16, MN-major operands come in slabs of 64).
-  const int least = g.b_mn ? 64 : 16, most = g.segmented ? kSegCols : 128;
-  int C = least;
-  while (C < most && C < g.cols) C *= 2;
-  auto tiles_of = [&](int c) { return (int64_t)p.row_tiles * (g.stacked ? 2 : 1) * ((g.cols + c - 1) / c); };
-  while (C > least && tiles_of(C) < di->sm_count) C /= 2;
-  const int64_t tiles = tiles_of(C);
+  TileShape shape = tile_shape(g, di);
+  const int C = shape.cols;
   p.tile_cols = C;
+  p.split = shape.split;
   p.col_tiles = (int)((g.cols + C - 1) / C);
-  // CTAs that share a tile's reduction: as many as find room on the GPU at once, each with at least 4 stages of work
-  p.split = 1;
-  if (C <= 64) {
-    while (p.split < DENSE_MAX_SPLIT && tiles * p.split * 2 <= 2 * di->sm_count && p.k_tiles >= p.split * 2 * 4) p.split *= 2;
-  }
+  const int64_t tiles = shape.tiles;
   p.stage_bytes = DENSE_A_BYTES + C * 128;
   const int reduce_bytes = p.split > 1 ? (C + p.split - 1) * 512 : 0;
-  p.stages = std::min(16, (DENSE_SMEM - 1024 - reduce_bytes) / p.stage_bytes);
-  p.reduce_offset = p.split > 1 ? p.stages * p.stage_bytes : 0;
+  // (the loads of a CTA come after about 1.4 us at 80 GB/s and SM: 110 KB in flight, so a CTA alone on its SM takes it all)
+  p.smem_bytes = tiles * p.split <= di->sm_count ? DENSE_SMEM_ALONE : DENSE_SMEM;
+  p.reduce_in_ring = p.split > 1 && C == 128 && p.smem_bytes == DENSE_SMEM;
+  p.stages = std::min(16, (p.smem_bytes - 1024 - (p.reduce_in_ring ? 0 : reduce_bytes)) / p.stage_bytes);
+  p.reduce_offset = p.split > 1 && !p.reduce_in_ring ? p.stages * p.stage_bytes : 0;
   const int cols = C * (g.segmented ? 2 : 1);
-  p.tmem_cols = cols <= 32 ? 32 : (cols <= 64 ? 64 : 128);
+  p.tmem_cols = cols <= 32 ? 32 : (cols <= 64 ? 64 : (cols <= 128 ? 128 : 256));
   p.idesc = dense_idesc(128, C, p.f16 != 0, g.a_mn, g.b_mn);
   if (tiles * p.split > 0x7fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
 
@@ -1171,35 +1291,67 @@ static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pair
   return B200MOE_OK;
 }
 
+// Estimated time of a launch of the pair kernel in nanoseconds, with tiles of `tile_cols` columns.  A stage of a 256 x 256
+// tile takes 290 ns (512 cycles of the tensor cores), one of a 256 x 128 tile 200 ns (its operands come at about 110 GB/s and
+// SM); a tile's epilogue takes about as long as 5 stages and hides behind the next tile's; start and end cost 7 us.
+static int64_t pair_tiles(const DenseGemm& g, int tile_cols) {
+  const int cols = g.dual ? tile_cols / 2 : tile_cols;
+  return ((g.rows + 255) / 256) * (g.stacked ? 2 : 1) * ((g.cols + cols - 1) / cols);
+}
+static int64_t pair_stages(const DenseGemm& g) { return (g.red + DENSE_BK - 1) / DENSE_BK * (g.chained ? 2 : 1); }
+static double pair_time(const DenseGemm* g, int jobs, int tile_cols, int pairs) {
+  const double stage = tile_cols == 256 ? 290.0 : 200.0;
+  double longest = 0.0, all = 0.0;
+  int64_t tiles = 0;
+  for (int i = 0; i < jobs; ++i) {
+    const double t = stage * (double)std::max<int64_t>(5, pair_stages(g[i]));
+    longest = std::max(longest, t);
+    all += t * (double)pair_tiles(g[i], tile_cols);
+    tiles += pair_tiles(g[i], tile_cols);
+  }
+  const double shared = jobs == 1 ? longest * (double)((tiles + pairs - 1) / pairs) : std::max(longest, all / pairs * 1.05);
+  return 7000.0 + shared;
+}
+static int pair_cols(const DenseGemm* g, int jobs, const DeviceInfo* di, double* time = nullptr) {
+  const double wide = pair_time(g, jobs, 256, di->sm_count / 2), narrow = pair_time(g, jobs, 128, di->sm_count / 2);
+  if (time) *time = std::min(wide, narrow);
+  return narrow < wide ? 128 : 256;
+}
+
 // One launch of the pair kernel over one or two products of the same epilogue; operand A's rows are the result's rows.
 // `p` arrives with its epilogue fields and each job's outputs and pitch set.
 static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceInfo* di, cudaStream_t stream) {
   PairMaps maps;
   memset(&maps, 0, sizeof(maps));
   p.jobs = jobs;
+  const int tile_cols = pair_cols(g, jobs, di);
   for (int i = 0; i < jobs; ++i) {
     PairJob& j = p.job[i];
     j.rows = (int)g[i].rows;
     j.cols = (int)g[i].cols;
+    j.tile_cols = tile_cols;
     j.row_tiles = (int)((g[i].rows + 255) / 256);
-    const int tile_cols = g[i].dual ? 128 : 256;
-    j.col_tiles = (int)((g[i].cols + tile_cols - 1) / tile_cols);
+    const int out_cols = g[i].dual ? tile_cols / 2 : tile_cols;
+    j.col_tiles = (int)((g[i].cols + out_cols - 1) / out_cols);
     j.chain_tiles = (int)((g[i].red + DENSE_BK - 1) / DENSE_BK);
-    j.k_tiles = j.chain_tiles * (g[i].chained ? 2 : 1);
+    j.k_tiles = (int)pair_stages(g[i]);
     j.a_mn = g[i].a_mn;
     j.b_mn = g[i].b_mn;
     j.stacked = g[i].stacked;
-    const int64_t tiles = (int64_t)j.row_tiles * (j.stacked ? 2 : 1) * j.col_tiles;
+    const int64_t tiles = pair_tiles(g[i], tile_cols);
     if (tiles > 0x3fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
     j.tiles = (int)tiles;
     j.raster = 16;
-    j.idesc = dense_idesc(256, 256, p.f16 != 0, g[i].a_mn, g[i].b_mn);
-    const int na = (g[i].chained || g[i].stacked) ? 2 : 1, nb = (g[i].chained || g[i].dual) ? 2 : 1;
+    j.idesc = dense_idesc(256, tile_cols, p.f16 != 0, g[i].a_mn, g[i].b_mn);
+    const int na = (g[i].chained || g[i].stacked) ? 2 : 1, nb = (g[i].chained || g[i].dual) ? 2 : 1, no = j.stacked ? 2 : 1;
     for (int q = 0; q < na; ++q) {
       int rc = dense_encode(&maps.job[i].a[q], g[i].a[q].base, g[i].a[q].outer, g[i].a[q].inner, g[i].a[q].ld, g[i].a_mn ? 64 : 128, p.f16);
       if (rc) return rc;
     }
-    const int no = j.stacked ? 2 : 1;
+    for (int q = 0; q < nb; ++q) {
+      int rc = dense_encode(&maps.job[i].b[q], g[i].b[q].base, g[i].b[q].outer, g[i].b[q].inner, g[i].b[q].ld, g[i].b_mn ? 64 : tile_cols / 2, p.f16);
+      if (rc) return rc;
+    }
     j.tma_store = j.ld_out % 8 == 0 && aligned16(j.out[0]) && aligned16(j.out[1]);
     for (int q = 0; q < 2; ++q) j.tma_store = j.tma_store && (!p.pre[q] || (aligned16(p.pre[q]) && p.ld_pre[q] % 8 == 0));
     if (j.tma_store) {
@@ -1212,10 +1364,6 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
         if (rc) return rc;
       }
     }
-    for (int q = 0; q < nb; ++q) {
-      int rc = dense_encode(&maps.job[i].b[q], g[i].b[q].base, g[i].b[q].outer, g[i].b[q].inner, g[i].b[q].ld, g[i].b_mn ? 64 : 128, p.f16);
-      if (rc) return rc;
-    }
   }
   // time of a tile in stages; below 5 its epilogue takes longer than its products
   auto cost = [&](int i) { return std::max(5, p.job[i].k_tiles); };
@@ -1224,8 +1372,8 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
     std::swap(maps.job[0], maps.job[1]);
     std::swap(maps.out[0], maps.out[1]);
   }
-  const int total = p.job[0].tiles + (jobs > 1 ? p.job[1].tiles : 0);
-  const int pairs = std::max(1, std::min(di->sm_count / 2, total));
+  const int64_t total = (int64_t)p.job[0].tiles + (jobs > 1 ? p.job[1].tiles : 0);
+  const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(di->sm_count / 2, total));
   p.full_rounds = p.job[0].tiles / pairs;
   p.rest = p.job[0].tiles % pairs;
   p.early = p.early_tiles = 0;
@@ -1244,12 +1392,6 @@ static void pair_params(PairParams& p, const b200moe_dense_args* a) {
   p.f16 = a->dtype == B200MOE_DTYPE_F16;
   p.act = a->act;
   p.wait_limit_ns = a->wait_limit_ms > 0 ? (uint64_t)a->wait_limit_ms * 1000000ull : kWaitLimitNs;
-}
-
-// A product of more rows than the tile kernel holds in one tile, and whose 256 x 256 tiles occupy at least half of the SM
-// pairs, goes to the pair kernel.
-static bool pair_pays(int64_t rows, int64_t cols, int64_t tile_cols, const DeviceInfo* di) {
-  return rows > 128 && ((rows + 255) / 256) * ((cols + tile_cols - 1) / tile_cols) * 4 >= di->sm_count;
 }
 
 // a TMA operand: 16-byte aligned base and pitch
@@ -1298,33 +1440,6 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
   if (gated ? a->y_dtype != a->dtype : (a->y_dtype != a->dtype && a->y_dtype != B200MOE_DTYPE_F32))
     return fail(B200MOE_E_UNSUPPORTED, "%s: output dtype %d", op, a->y_dtype);
   if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != B200MOE_DTYPE_F32) return fail(B200MOE_E_UNSUPPORTED, "%s: bias dtype %d", op, a->bias_dtype);
-  if (a->y_dtype != B200MOE_DTYPE_F32 && pair_pays(a->m, a->n, gated ? 128 : 256, di)) {
-    PairParams q;
-    pair_params(q, a);
-    DenseGemm g;
-    g.a[0] = {a->x, a->m, a->k, a->ld_x};
-    g.b[0] = {a->w0, a->n, a->k, a->ld_w0};
-    g.b[1] = {a->w1, a->n, a->k, a->ld_w1};
-    g.dual = gated;
-    g.epi = gated ? DENSE_GLU : DENSE_LINEAR;
-    g.rows = a->m;
-    g.cols = a->n;
-    g.red = a->k;
-    q.job[0].out[0] = a->y;
-    q.job[0].ld_out = a->ld_y;
-    q.pre[0] = a->pre0;
-    q.pre[1] = a->pre1;
-    q.ld_pre[0] = a->ld_pre0;
-    q.ld_pre[1] = a->ld_pre1;
-    if (!gated) {
-      q.bias = a->bias;
-      q.bias_f32 = a->bias_dtype == B200MOE_DTYPE_F32;
-      q.residual = a->residual;
-      q.ld_res = a->ld_residual;
-      q.vec_res = aligned16(a->residual) && a->ld_residual % 8 == 0;
-    }
-    return dense_pair_gemm(&g, 1, q, di, stream);
-  }
   DenseParams p;
   dense_params(p, a);
   p.out[0] = a->y;
@@ -1353,6 +1468,37 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
     p.out_f32 = a->y_dtype == B200MOE_DTYPE_F32;
     g.segmented = p.out_f32 != 0;
   }
+  if (a->y_dtype != B200MOE_DTYPE_F32) {
+    DenseGemm w;
+    w.a[0] = {a->x, a->m, a->k, a->ld_x};
+    w.b[0] = {a->w0, a->n, a->k, a->ld_w0};
+    w.b[1] = {a->w1, a->n, a->k, a->ld_w1};
+    w.dual = gated;
+    w.epi = gated ? DENSE_GLU : DENSE_LINEAR;
+    w.rows = a->m;
+    w.cols = a->n;
+    w.red = a->k;
+    double time = 0.0;
+    pair_cols(&w, 1, di, &time);
+    if (time < tile_shape(g, di).time) {
+      PairParams q;
+      pair_params(q, a);
+      q.job[0].out[0] = a->y;
+      q.job[0].ld_out = a->ld_y;
+      q.pre[0] = a->pre0;
+      q.pre[1] = a->pre1;
+      q.ld_pre[0] = a->ld_pre0;
+      q.ld_pre[1] = a->ld_pre1;
+      if (!gated) {
+        q.bias = a->bias;
+        q.bias_f32 = a->bias_dtype == B200MOE_DTYPE_F32;
+        q.residual = a->residual;
+        q.ld_res = a->ld_residual;
+        q.vec_res = aligned16(a->residual) && a->ld_residual % 8 == 0;
+      }
+      return dense_pair_gemm(&w, 1, q, di, stream);
+    }
+  }
   return dense_gemm(g, p, di, stream);
 }
 
@@ -1366,89 +1512,58 @@ static int grad_row_blocks(int64_t m, int64_t n, int64_t* rows_per_block) {
 
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// dx = sum of dz_i w_i and dw_i = dz_i^T x
+// dx = sum of dz_i w_i and dw_i = dz_i^T x: one launch of the pair kernel, or a launch of the tile kernel each where those are
+// estimated to take less time
 static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, DeviceInfo* di, cudaStream_t stream) {
-  {
-    // both products in one launch of the pair kernel where their tiles fill it
-    const int64_t dx_tiles = a->dx ? ((a->m + 255) / 256) * ((a->k + 255) / 256) : 0;
-    const int64_t dw_tiles = a->dw0 ? count * ((a->n + 255) / 256) * ((a->k + 255) / 256) : 0;
-    if ((dx_tiles + dw_tiles) * 4 >= di->sm_count && a->m >= 128) {
-      PairParams q;
-      pair_params(q, a);
-      DenseGemm g[2];
-      int jobs = 0;
-      if (a->dx) {
-        DenseGemm& x = g[jobs];
-        for (int i = 0; i < count; ++i) {
-          x.a[i] = {dz[i], a->m, a->n, ld_dz};
-          x.b[i] = {i ? a->w1 : a->w0, a->n, a->k, i ? a->ld_w1 : a->ld_w0};
-        }
-        x.chained = count == 2;
-        x.b_mn = true;
-        x.rows = a->m;
-        x.cols = a->k;
-        x.red = a->n;
-        q.job[jobs].out[0] = a->dx;
-        q.job[jobs++].ld_out = a->k;
-      }
-      if (a->dw0) {
-        DenseGemm& w = g[jobs];
-        for (int i = 0; i < count; ++i) w.a[i] = {dz[i], a->m, a->n, ld_dz};
-        w.b[0] = {a->x, a->m, a->k, a->ld_x};
-        w.stacked = count == 2;
-        w.a_mn = w.b_mn = true;
-        w.rows = a->n;
-        w.cols = a->k;
-        w.red = a->m;
-        q.job[jobs].out[0] = a->dw0;
-        q.job[jobs].out[1] = a->dw1;
-        q.job[jobs++].ld_out = a->k;
-      }
-      return dense_pair_gemm(g, jobs, q, di, stream);
-    }
-  }
-  DenseParams p;
+  PairParams q;
+  pair_params(q, a);
+  DenseGemm pair[2], tile[2];
+  int jobs = 0;
   if (a->dx) {
-    dense_params(p, a);
-    p.act = B200MOE_ACT_NONE;
-    p.out[0] = a->dx;
-    p.ld_out = a->k;
-    DenseGemm g;
-    // rows = the k features of x: w [n, k] is MN-major; columns = tokens
-    g.a[0] = {a->w0, a->n, a->k, a->ld_w0};
-    g.b[0] = {dz[0], a->m, a->n, ld_dz};
-    if (count == 2) {
-      g.a[1] = {a->w1, a->n, a->k, a->ld_w1};
-      g.b[1] = {dz[1], a->m, a->n, ld_dz};
-      g.chained = true;
+    // rows = tokens; for the tile kernel rows = the k features of x, columns = tokens.  w [n, k] is MN-major.
+    DenseGemm &x = pair[jobs], &t = tile[jobs];
+    for (int i = 0; i < count; ++i) {
+      x.a[i] = t.b[i] = {dz[i], a->m, a->n, ld_dz};
+      x.b[i] = t.a[i] = {i ? a->w1 : a->w0, a->n, a->k, i ? a->ld_w1 : a->ld_w0};
     }
-    g.a_mn = true;
-    g.rows = a->k;
-    g.cols = a->m;
-    g.red = a->n;
-    g.trans = true;
-    g.epi = DENSE_LINEAR;
-    int rc = dense_gemm(g, p, di, stream);
-    if (rc) return rc;
+    x.chained = t.chained = count == 2;
+    x.b_mn = t.a_mn = true;
+    x.rows = t.cols = a->m;
+    x.cols = t.rows = a->k;
+    x.red = t.red = a->n;
+    t.trans = true;
+    t.epi = DENSE_LINEAR;
+    q.job[jobs].out[0] = a->dx;
+    q.job[jobs++].ld_out = a->k;
   }
   if (a->dw0) {
+    DenseGemm& w = pair[jobs];
+    for (int i = 0; i < count; ++i) w.a[i] = {dz[i], a->m, a->n, ld_dz};
+    w.b[0] = {a->x, a->m, a->k, a->ld_x};
+    w.stacked = count == 2;
+    w.a_mn = w.b_mn = true;
+    w.rows = a->n;
+    w.cols = a->k;
+    w.red = a->m;
+    tile[jobs] = w;
+    q.job[jobs].out[0] = a->dw0;
+    q.job[jobs].out[1] = a->dw1;
+    q.job[jobs++].ld_out = a->k;
+  }
+  if (jobs == 0) return B200MOE_OK;
+  double pair_ns = 0.0, tile_ns = 0.0;
+  pair_cols(pair, jobs, di, &pair_ns);
+  for (int i = 0; i < jobs; ++i) tile_ns += tile_shape(tile[i], di).time;
+  if (pair_ns < tile_ns) return dense_pair_gemm(pair, jobs, q, di, stream);
+  for (int i = 0; i < jobs; ++i) {
+    DenseParams p;
     dense_params(p, a);
-    p.out[0] = a->dw0;
-    p.out[1] = a->dw1;
+    p.act = B200MOE_ACT_NONE;
+    p.out[0] = q.job[i].out[0];
+    p.out[1] = q.job[i].out[1];
     p.ld_out = a->k;
-    p.vec_store = aligned16(a->dw0) && aligned16(a->dw1);
-    DenseGemm g;
-    g.a[0] = {dz[0], a->m, a->n, ld_dz};
-    g.b[0] = {a->x, a->m, a->k, a->ld_x};
-    if (count == 2) {
-      g.a[1] = {dz[1], a->m, a->n, ld_dz};
-      g.stacked = true;
-    }
-    g.a_mn = g.b_mn = true;
-    g.rows = a->n;
-    g.cols = a->k;
-    g.red = a->m;
-    int rc = dense_gemm(g, p, di, stream);
+    p.vec_store = aligned16(p.out[0]) && aligned16(p.out[1]);
+    const int rc = dense_gemm(tile[i], p, di, stream);
     if (rc) return rc;
   }
   return B200MOE_OK;
