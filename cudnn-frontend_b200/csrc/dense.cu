@@ -69,22 +69,50 @@ static uint32_t dense_idesc(int m, int n, bool f16, bool a_mn, bool b_mn) {
          ((uint32_t)(m >> 4) << 24);
 }
 
+// Issue by one lane of a converged warp, as predicated instructions instead of a branch around them: the operands then stay in
+// uniform registers, where a branch moves every descriptor over for every instruction (four products and a commit took
+// 250 cycles that way and 175 like this).
+#define B200_IF_ASM(INSTR) "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t@q " INSTR "\n\t}"
 template <bool kPair>
-__device__ __forceinline__ void mma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16_if(uint32_t go, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   if constexpr (kPair) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
         : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
         : "memory");
   }
 }
+__device__ __forceinline__ void commit_if(uint32_t go, uint32_t bar) {
+  asm volatile(B200_IF_ASM("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];")::"r"(go), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_pair_if(uint32_t go, uint32_t bar) {
+  asm volatile(B200_IF_ASM("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;")::"r"(go),
+               "r"(bar), "h"((uint16_t)3)
+               : "memory");
+}
+__device__ __forceinline__ void expect_tx_if(uint32_t go, uint32_t bar, uint32_t bytes) {
+  asm volatile(B200_IF_ASM("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %2;")::"r"(go), "r"(bar), "r"(bytes) : "memory");
+}
+// into the issuing CTA's own shared memory; kPair: credited to a barrier of either CTA of the pair
+template <bool kPair>
+__device__ __forceinline__ void load_2d_if(uint32_t go, uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1) {
+  if constexpr (kPair)
+    asm volatile(B200_IF_ASM("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];")::"r"(go),
+                 "r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+  else
+    asm volatile(B200_IF_ASM("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];")::"r"(go),
+                 "r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
+#undef B200_IF_ASM
 
 // 32 lanes x 16 consecutive columns -> 16 registers per thread
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float* v) {
@@ -288,28 +316,26 @@ __global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel
     }
     int kc = kt * DENSE_BK;
     uint32_t dst = ring, fb = full_bar(0), eb = empty_bar(0), parity = 1;
+    const uint32_t go = elect_one();  // (the same lane of a full warp every time)
     int issued = 0;
     for (; issued < nk; ++issued) {
       if (!__all_sync(0xffffffffu, mbar_wait(eb, parity, wc, ST_DENSE_EMPTY))) break;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(fb, stage_bytes);
-        if constexpr (kGlu) {
-          tma_load_2d(dst, ma, fb, kc, row0);
-          tma_load_2d(dst + 64 * 128, ma + 1, fb, kc, row0);
-        } else if (a_mn) {
-          tma_load_2d(dst, ma, fb, row0, kc);
-          tma_load_2d(dst + DENSE_SLAB, ma, fb, row0 + 64, kc);
-        } else {
-          tma_load_2d(dst, ma, fb, kc, row0);
-        }
-        if (b_mn) {
-          tma_load_2d(dst + DENSE_A_BYTES, mb, fb, col0, kc);
-          if (b_two) tma_load_2d(dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
-        } else {
-          tma_load_2d(dst + DENSE_A_BYTES, mb, fb, kc, col0);
-        }
+      expect_tx_if(go, fb, stage_bytes);
+      if constexpr (kGlu) {
+        load_2d_if<false>(go, dst, ma, fb, kc, row0);
+        load_2d_if<false>(go, dst + 64 * 128, ma + 1, fb, kc, row0);
+      } else if (a_mn) {
+        load_2d_if<false>(go, dst, ma, fb, row0, kc);
+        load_2d_if<false>(go, dst + DENSE_SLAB, ma, fb, row0 + 64, kc);
+      } else {
+        load_2d_if<false>(go, dst, ma, fb, kc, row0);
       }
-      __syncwarp();
+      if (b_mn) {
+        load_2d_if<false>(go, dst + DENSE_A_BYTES, mb, fb, col0, kc);
+        if (b_two) load_2d_if<false>(go, dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
+      } else {
+        load_2d_if<false>(go, dst + DENSE_A_BYTES, mb, fb, kc, col0);
+      }
       kc += DENSE_BK;
       if (--chain_left == 0) {
         kc = 0;
@@ -346,6 +372,7 @@ __global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel
     bool ok = true;
     int seg = 0, in_seg = 0, stage = 0;
     uint32_t parity = 0, a_lo = a_lo0, b_lo = b_lo0;
+    const uint32_t go = elect_one();
     for (int i = 0; i < nk && ok; ++i) {
       const uint32_t acc = tmem + (kSeg ? (uint32_t)((seg & 1) * C) : 0u);
       if (kSeg && in_seg == 0 && seg >= 2) {
@@ -355,13 +382,10 @@ __global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel
       }
       if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), parity, wc, ST_DENSE_FULL))) { ok = false; break; }
       const bool seg_end = i + 1 == nk || (kSeg && in_seg == kSegTiles - 1);
-      if (elect_one()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma_f16_ss<false>(acc, desc(a_lo + j * a_step), desc(b_lo + j * b_step), idesc, (in_seg | j) != 0);
-        tc_commit(empty_bar(stage));
-        if (seg_end) tc_commit(acc_full_bar(kSeg ? seg & 1 : 0));
-      }
-      __syncwarp();
+      for (int j = 0; j < 4; ++j) mma_f16_if<false>(go, acc, desc(a_lo + j * a_step), desc(b_lo + j * b_step), idesc, (in_seg | j) != 0);
+      commit_if(go, empty_bar(stage));
+      if (seg_end) commit_if(go, acc_full_bar(kSeg ? seg & 1 : 0));
       ++in_seg;
       if (seg_end) {
         ++seg;
@@ -721,12 +745,60 @@ __device__ __forceinline__ void st_shared_u32x4(uint32_t addr, uint32_t a, uint3
 // One warp's block of 32 rows x 32 columns to 16-bit memory: lane = row, v[] = its columns.  Stored from registers, every
 // instruction would touch 32 lines (7000 cycles for a tile of 128 x 256, measured as 87 us for 896 tiles); so the block goes
 // through shared memory (two blocks in turn, 64-byte swizzle: 16-byte writes without bank conflicts) and leaves as one bulk
-// copy, or, where the output has no tensor map, row by row with neighbouring lanes on neighbouring columns.
+// copy, or, where the output has no tensor map, row by row with neighbouring lanes on neighbouring columns.  A residual comes in
+// the same way.
 struct BlockWriter {
   uint32_t staging;  // this warp's two blocks
   int turn;
   int lane;
   bool f16;
+  // v[] += the block of `base` at (row0, col); values beyond rows and cols are not read
+  __device__ __forceinline__ void add(float* v, const void* base, int64_t ld, bool vec, int row0, int rows, int col, int cols) {
+    const uint32_t block = staging + (uint32_t)(turn * PAIR_BOX);
+    turn ^= 1;
+    if (lane == 0) bulk_wait_read1();  // the copy before the last one used this block
+    __syncwarp();
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(base);
+    if (vec && col + 32 <= cols) {
+      // 8 rows at a time, 4 lanes to a row
+      uint4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = row0 + 8 * q + (lane >> 2);
+        w[q] = make_uint4(0, 0, 0, 0);
+        if (r < rows) w[q] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)r * ld + col) + (lane & 3));
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = 8 * q + (lane >> 2);
+        st_shared_u32x4(block + (uint32_t)(r * 64) + ((uint32_t)((lane & 3) ^ ((r >> 1) & 3)) << 4), w[q].x, w[q].y, w[q].z, w[q].w);
+      }
+    } else {
+      const bool in = col + lane < cols;
+      const int count = min(32, rows - row0);
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r) {
+        uint16_t h = 0;
+        if (in && r < count) h = src[(int64_t)(row0 + r) * ld + col + lane];
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(block + (uint32_t)(r * 64) + ((((uint32_t)lane >> 3) ^ (uint32_t)((r >> 1) & 3)) << 4) + (uint32_t)(lane & 7) * 2), "h"(h) : "memory");
+      }
+    }
+    __syncwarp();
+    const uint32_t line = block + (uint32_t)(lane * 64), swz = (uint32_t)((lane >> 1) & 3);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(line + (((uint32_t)q ^ swz) << 4)) : "memory");
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack16x2(w[e], f16);
+        v[8 * q + 2 * e] += f.x;
+        v[8 * q + 2 * e + 1] += f.y;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) bulk_commit();  // (an empty group: the block after this one was last used two groups ago)
+  }
   __device__ __forceinline__ void write(const float* v, const CUtensorMap* map, void* base, int64_t ld, bool tma, int row0, int rows, int col, int cols) {
     const uint32_t block = staging + (uint32_t)(turn * PAIR_BOX);
     turn ^= 1;
@@ -818,6 +890,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     uint32_t phase = 0;
     int issued = 0;
     bool ok = true;
+    const uint32_t go = elect_one();  // (the same lane of a full warp every time)
+    const uint32_t go_leader = rank == 0 ? go : 0u;
     PairTile t;
     for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
       const PairJob& j = p.job[t.job];
@@ -829,28 +903,25 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       const uint32_t bytes = 2u * (uint32_t)(DENSE_A_BYTES + half_cols * 128);
       for (int kt = 0; kt < j.k_tiles; ++kt) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, wc, ST_PAIR_EMPTY))) { ok = false; break; }
-        if (elect_one()) {
-          const int chain = kt >= j.chain_tiles ? 1 : 0;
-          const int kc = (kt - chain * j.chain_tiles) * DENSE_BK;
-          const uint32_t fb = leader_full0 + 8u * stage;
-          const uint32_t da = ring + stage * PAIR_STAGE_BYTES, db = da + DENSE_A_BYTES;
-          const CUtensorMap* ma = &m.a[chain | t.which];
-          const CUtensorMap* mb = &m.b[kEpi == DENSE_GLU ? rank : chain];
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), bytes);
-          if (a_mn) {
-            tma_load_2d_pair(da, ma, fb, a0, kc);
-            tma_load_2d_pair(da + DENSE_SLAB, ma, fb, a0 + 64, kc);
-          } else {
-            tma_load_2d_pair(da, ma, fb, kc, a0);
-          }
-          if (b_mn) {
-            tma_load_2d_pair(db, mb, fb, b0, kc);
-            if (half_cols > 64) tma_load_2d_pair(db + DENSE_SLAB, mb, fb, b0 + 64, kc);
-          } else {
-            tma_load_2d_pair(db, mb, fb, kc, b0);
-          }
+        const int chain = kt >= j.chain_tiles ? 1 : 0;
+        const int kc = (kt - chain * j.chain_tiles) * DENSE_BK;
+        const uint32_t fb = leader_full0 + 8u * stage;
+        const uint32_t da = ring + stage * PAIR_STAGE_BYTES, db = da + DENSE_A_BYTES;
+        const CUtensorMap* ma = &m.a[chain | t.which];
+        const CUtensorMap* mb = &m.b[kEpi == DENSE_GLU ? rank : chain];
+        expect_tx_if(go_leader, full_bar(stage), bytes);
+        if (a_mn) {
+          load_2d_if<true>(go, da, ma, fb, a0, kc);
+          load_2d_if<true>(go, da + DENSE_SLAB, ma, fb, a0 + 64, kc);
+        } else {
+          load_2d_if<true>(go, da, ma, fb, kc, a0);
         }
-        __syncwarp();
+        if (b_mn) {
+          load_2d_if<true>(go, db, mb, fb, b0, kc);
+          if (half_cols > 64) load_2d_if<true>(go, db + DENSE_SLAB, mb, fb, b0 + 64, kc);
+        } else {
+          load_2d_if<true>(go, db, mb, fb, kc, b0);
+        }
         ++issued;
         if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -870,6 +941,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      const uint32_t go = elect_one();
       PairTile t;
       for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
         const PairJob& j = p.job[t.job];
@@ -887,14 +959,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           bool landed = mbar_try_wait(full_bar(stage), phase);
           if (!landed) landed = mbar_wait(full_bar(stage), phase, wc, ST_PAIR_FULL);
           if (!__all_sync(0xffffffffu, landed)) { ok = false; break; }
-          if (elect_one()) {
-            const uint32_t a_lo = a_lo0 + stage * (PAIR_STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (PAIR_STAGE_BYTES >> 4);
+          const uint32_t a_lo = a_lo0 + stage * (PAIR_STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (PAIR_STAGE_BYTES >> 4);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mma_f16_ss<true>(acc, desc(a_lo + q * a_step), desc(b_lo + q * b_step), idesc, (kt | q) != 0);
-            tc_commit_pair(empty_bar(stage), 3);
-            if (kt + 1 == k_tiles) tc_commit_pair(acc_full_bar(i & 1), 3);
-          }
-          __syncwarp();
+          for (int q = 0; q < 4; ++q) mma_f16_if<true>(go, acc, desc(a_lo + q * a_step), desc(b_lo + q * b_step), idesc, (kt | q) != 0);
+          commit_pair_if(go, empty_bar(stage));
+          if (kt + 1 == k_tiles) commit_pair_if(go, acc_full_bar(i & 1));
           if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
         }
       }
@@ -951,27 +1020,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           }
           if (p.pre[0]) writer.write(v, &maps.pre[0], p.pre[0], p.ld_pre[0], tma, row0, rows, col, cols);
           act_values<32>(v, p.act);
-          if (p.residual) {
-            const int64_t ro = (int64_t)row * p.ld_res + col;
-            if (p.vec_res && count >= 32) {
-              const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.residual) + ro);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint4 w = __ldg(src + q);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 f = unpack16x2(ws[e], f16);
-                  v[8 * q + 2 * e] += f.x;
-                  v[8 * q + 2 * e + 1] += f.y;
-                }
-              }
-            } else {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (q < count) v[q] += load16(p.residual, ro + q, f16);
-            }
-          }
+          if (p.residual) writer.add(v, p.residual, p.ld_res, p.vec_res != 0, row0, rows, col, cols);
         }
         writer.write(v, &maps.out[t.job][t.which], j.out[t.which], j.ld_out, tma, row0, rows, col, cols);
       }
@@ -995,6 +1044,31 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 // ---------------------------------------------------------------------------------------
 constexpr int GRAD_COLS = 256;  // columns of a block: 32 lanes x 8
 
+// 8 neighbouring values; beyond `count` zeros.  `whole`: 16-byte aligned and all there
+__device__ __forceinline__ void load8_16(const uint16_t* src, bool whole, int count, bool f16, float* v) {
+  if (whole) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 p = unpack16x2(w[j], f16);
+      v[2 * j] = p.x, v[2 * j + 1] = p.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? load16(src, j, f16) : 0.0f;
+  }
+}
+__device__ __forceinline__ void load8_f32(const float* src, bool whole, int count, float* v) {
+  if (whole) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? src[j] : 0.0f;
+  }
+}
+
 // dg, du [m, ldo] from dh, gate, up [m, n]
 __global__ void __launch_bounds__(256)
     glu_grad_kernel(const void* __restrict__ dh, const void* __restrict__ gate, const void* __restrict__ up, int64_t m, int n, int64_t ld_dh,
@@ -1004,25 +1078,10 @@ __global__ void __launch_bounds__(256)
   if (c >= n) return;
   for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < m; r += (int64_t)gridDim.y * 8) {
     float d[8], g[8], u[8];
-    if (vec && c + 8 <= n) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dh) + r * ld_dh + c));
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(gate) + r * ld_gate + c));
-      const uint4 e = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(up) + r * ld_up + c));
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w}, ew[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 p = unpack16x2(aw[j], f16), q = unpack16x2(bw[j], f16), s = unpack16x2(ew[j], f16);
-        d[2 * j] = p.x, d[2 * j + 1] = p.y, g[2 * j] = q.x, g[2 * j + 1] = q.y, u[2 * j] = s.x, u[2 * j + 1] = s.y;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = c + j < n;
-        d[j] = in ? load16(dh, r * ld_dh + c + j, f16) : 0.0f;
-        g[j] = in ? load16(gate, r * ld_gate + c + j, f16) : 0.0f;
-        u[j] = in ? load16(up, r * ld_up + c + j, f16) : 0.0f;
-      }
-    }
+    const bool whole = vec && c + 8 <= n;
+    load8_16(reinterpret_cast<const uint16_t*>(dh) + r * ld_dh + c, whole, n - c, f16 != 0, d);
+    load8_16(reinterpret_cast<const uint16_t*>(gate) + r * ld_gate + c, whole, n - c, f16 != 0, g);
+    load8_16(reinterpret_cast<const uint16_t*>(up) + r * ld_up + c, whole, n - c, f16 != 0, u);
     uint32_t gw[4], uw[4];
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
@@ -1040,9 +1099,10 @@ __global__ void __launch_bounds__(256)
 
 // dz [m, ldo] = dy act'(z) (dz == NULL: dy is used as it is), and the column sums of the unrounded dz over the block's
 // rows: sums [gridDim.y][n].  Every sum has a fixed order: a warp's rows, then the warps, then (next kernel) the blocks.
+template <int kAct>
 __global__ void __launch_bounds__(256)
     act_grad_kernel(const void* __restrict__ dy, const void* __restrict__ z, int64_t m, int n, int64_t ld_dy, int64_t ld_z, void* __restrict__ dz,
-                    int64_t ldo, float* __restrict__ sums, int act, int f16, int dy_f32, int vec, int64_t rows_per_block) {
+                    int64_t ldo, float* __restrict__ sums, int f16, int dy_f32, int vec, int64_t rows_per_block) {
   __shared__ float s_part[8][GRAD_COLS];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1052,52 +1112,34 @@ __global__ void __launch_bounds__(256)
   for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
   const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(m, r0 + rows_per_block);
   if (c < n) {
-    for (int64_t r = r0 + warp; r < r1; r += 8) {
-      float d[8];
-      const bool whole = vec && c + 8 <= n;
-      if (dy_f32) {
-        const float* src = reinterpret_cast<const float*>(dy) + r * ld_dy + c;
-        if (whole) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-          d[0] = a.x, d[1] = a.y, d[2] = a.z, d[3] = a.w, d[4] = b.x, d[5] = b.y, d[6] = b.z, d[7] = b.w;
-        } else {
+    const bool whole = vec && c + 8 <= n;
+    // two rows in flight per warp
+    for (int64_t r = r0 + warp; r < r1; r += 16) {
+      float d[2][8], g[2][8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] = c + j < n ? src[j] : 0.0f;
-        }
-      } else if (whole) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(dy) + r * ld_dy + c));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 p = unpack16x2(w[j], f16);
-          d[2 * j] = p.x, d[2 * j + 1] = p.y;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = c + j < n ? load16(dy, r * ld_dy + c + j, f16) : 0.0f;
-      }
-      if (z) {
-        if (whole) {
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(z) + r * ld_z + c));
-          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 p = unpack16x2(w[j], f16);
-            d[2 * j] *= act_grad_f(p.x, act), d[2 * j + 1] *= act_grad_f(p.y, act);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j < n) d[j] *= act_grad_f(load16(z, r * ld_z + c + j, f16), act);
+      for (int q = 0; q < 2; ++q) {
+        const int64_t row = r + 8 * q;
+        if (row < r1) {
+          if (dy_f32) load8_f32(reinterpret_cast<const float*>(dy) + row * ld_dy + c, whole, n - c, d[q]);
+          else load8_16(reinterpret_cast<const uint16_t*>(dy) + row * ld_dy + c, whole, n - c, f16 != 0, d[q]);
+          if (kAct != B200MOE_ACT_NONE) load8_16(reinterpret_cast<const uint16_t*>(z) + row * ld_z + c, whole, n - c, f16 != 0, g[q]);
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += d[j];
-      if (dz) {
-        uint32_t w[4];
+      for (int q = 0; q < 2; ++q) {
+        const int64_t row = r + 8 * q;
+        if (row >= r1) break;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack16x2_from_float(d[2 * j], d[2 * j + 1], f16);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + r * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 8; ++j) {
+          if (kAct != B200MOE_ACT_NONE) d[q][j] = c + j < n ? d[q][j] * act_grad_f(g[q][j], kAct) : 0.0f;
+          acc[j] += d[q][j];
+        }
+        if (dz) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = pack16x2_from_float(d[q][2 * j], d[q][2 * j + 1], f16 != 0);
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
   }
@@ -1154,6 +1196,9 @@ struct DenseGemm {
   bool trans = false;
   int epi = DENSE_STORE;
   bool segmented = false;
+  // what the estimates need to know of the epilogue
+  int act = B200MOE_ACT_NONE;
+  bool has_residual = false, saves = false;
 };
 
 // A launch in clusters that may start while its predecessor drains
@@ -1194,9 +1239,22 @@ static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsign
   return B200MOE_OK;
 }
 
+// ---- estimated times in nanoseconds, fitted to both kernels on products of 512 x 1024 to 14336 x 14336 at 1 to 512 tokens ----
+
+// Time that an epilogue adds, per element and SM
+static double epilogue_ns(const DenseGemm& g) {
+  return 0.05 + (g.epi == DENSE_GLU ? 0.1 : 0.0) + (g.act == B200MOE_ACT_GELU ? 0.25 : (g.act == B200MOE_ACT_NONE ? 0.0 : 0.05)) + (g.has_residual ? 0.1 : 0.0) +
+         (g.saves ? 0.1 : 0.0);
+}
+// A product's operands and result cannot pass faster than HBM's 6500 bytes / ns
+static double memory_ns(const DenseGemm& g) {
+  const double rows = (double)g.rows * (g.dual || g.stacked ? 2 : 1), red = (double)g.red * (g.chained ? 2 : 1);
+  return 2.0 * (rows * red + (double)g.cols * red + rows * (double)g.cols) / 6500.0;
+}
+
 // Columns of the tile kernel's tiles (as many as there are, up to 128; an MN-major B comes in slabs of 64) and the CTAs that
-// share a tile's reduction, by estimated time in nanoseconds: the stages that the busiest SM loads, at about 80 bytes / ns
-// (between 52 from HBM and 100 from L2, measured), plus what joining the partial sums costs.  5 us start and end a launch.
+// share a tile's reduction.  A stage takes a CTA 205 ns (the issuer's loop) or as long as its bytes take at 160 GB/s for the SM
+// and 15.8 TB/s for all of L2; two CTAs run on an SM at once; joining partial sums costs more the more columns and CTAs.
 struct TileShape {
   int cols, split;
   int64_t tiles;
@@ -1206,15 +1264,21 @@ static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
   const int64_t tile_rows = g.dual ? 64 : 128;
   const int64_t rows = (g.rows + tile_rows - 1) / tile_rows * (g.stacked ? 2 : 1);
   const int64_t stages = (g.red + DENSE_BK - 1) / DENSE_BK * (g.chained ? 2 : 1);
+  const int least = g.b_mn ? 64 : 16;
   TileShape best = {0, 0, 0, 0.0};
-  for (int c = 128; c >= (g.b_mn ? 64 : 16); c /= 2) {
-    if (c > 16 && c / 2 >= g.cols && c / 2 >= (g.b_mn ? 64 : 16)) continue;  // half as many hold them all
+  for (int c = 128; c >= least; c /= 2) {
+    if (c > least && c / 2 >= g.cols) continue;  // half as many hold them all
     const int64_t tiles = rows * ((g.cols + c - 1) / c);
+    const double bytes = DENSE_A_BYTES + c * 128;
     for (int split = 1; split <= DENSE_MAX_SPLIT && split * 4 <= std::max<int64_t>(4, stages); split *= 2) {
-      const int64_t per_sm = (tiles * split + di->sm_count - 1) / di->sm_count;
-      const double load = (double)per_sm * (double)((stages + split - 1) / split) * (DENSE_A_BYTES + c * 128) / 80.0;
-      const double finish = (double)((per_sm + 1) / 2) * (1000.0 + 16.0 * c) + (split > 1 ? 500.0 + 8.0 * c : 0.0);
-      const double time = 5000.0 + load + finish;
+      const int64_t ctas = tiles * split;
+      const int64_t per_sm = (ctas + di->sm_count - 1) / di->sm_count;
+      const double together = per_sm > 1 ? 2.0 : 1.0, rounds = per_sm > 1 ? (double)((per_sm + 1) / 2) : 1.0;
+      const double stage = std::max({205.0, together * bytes / 160.0, together * bytes * (double)std::min<int64_t>(ctas, di->sm_count) / 15800.0});
+      const double load = std::max(rounds * (double)((stages + split - 1) / split) * stage, memory_ns(g));
+      const double join = split > 1 || g.dual ? 1000.0 + 350.0 * split + 25.0 * c : 2000.0 + 8.0 * c;
+      const double finish = join + epilogue_ns(g) * 128.0 * c / split * together;
+      const double time = 3000.0 + load + finish * (rounds > 1.0 ? 1.4 * rounds : 1.0);
       if (best.cols == 0 || time < best.time) best = {c, split, tiles, time};
     }
   }
@@ -1291,26 +1355,29 @@ static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pair
   return B200MOE_OK;
 }
 
-// Estimated time of a launch of the pair kernel in nanoseconds, with tiles of `tile_cols` columns.  A stage of a 256 x 256
-// tile takes 290 ns (512 cycles of the tensor cores), one of a 256 x 128 tile 200 ns (its operands come at about 110 GB/s and
-// SM); a tile's epilogue takes about as long as 5 stages and hides behind the next tile's; start and end cost 7 us.
+// The pair kernel's launch with tiles of `tile_cols` columns.  A stage of a 256 x 256 tile takes 285 ns (512 cycles of the tensor
+// cores), one of a 256 x 128 tile 210 ns (the issuer's loop); a tile's epilogue takes as long as 5 stages and hides behind
+// the next tile's, the last one's does not; start and end cost 6 us.
 static int64_t pair_tiles(const DenseGemm& g, int tile_cols) {
   const int cols = g.dual ? tile_cols / 2 : tile_cols;
   return ((g.rows + 255) / 256) * (g.stacked ? 2 : 1) * ((g.cols + cols - 1) / cols);
 }
 static int64_t pair_stages(const DenseGemm& g) { return (g.red + DENSE_BK - 1) / DENSE_BK * (g.chained ? 2 : 1); }
 static double pair_time(const DenseGemm* g, int jobs, int tile_cols, int pairs) {
-  const double stage = tile_cols == 256 ? 290.0 : 200.0;
-  double longest = 0.0, all = 0.0;
+  const double stage = tile_cols == 256 ? 285.0 : 210.0;
+  double longest = 0.0, all = 0.0, memory = 0.0, last = 0.0;
   int64_t tiles = 0;
   for (int i = 0; i < jobs; ++i) {
-    const double t = stage * (double)std::max<int64_t>(5, pair_stages(g[i]));
+    const double finish = (epilogue_ns(g[i]) - 0.05) * 128.0 * tile_cols;
+    const double t = std::max(stage * (double)std::max<int64_t>(5, pair_stages(g[i])), finish);
     longest = std::max(longest, t);
+    last = std::max(last, finish);
     all += t * (double)pair_tiles(g[i], tile_cols);
     tiles += pair_tiles(g[i], tile_cols);
+    memory += memory_ns(g[i]);
   }
   const double shared = jobs == 1 ? longest * (double)((tiles + pairs - 1) / pairs) : std::max(longest, all / pairs * 1.05);
-  return 7000.0 + shared;
+  return 6000.0 + std::max(shared, memory) + last;
 }
 static int pair_cols(const DenseGemm* g, int jobs, const DeviceInfo* di, double* time = nullptr) {
   const double wide = pair_time(g, jobs, 256, di->sm_count / 2), narrow = pair_time(g, jobs, 128, di->sm_count / 2);
@@ -1467,7 +1534,10 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
     p.ld_res = a->ld_residual;
     p.out_f32 = a->y_dtype == B200MOE_DTYPE_F32;
     g.segmented = p.out_f32 != 0;
+    g.act = a->act;
+    g.has_residual = a->residual != nullptr;
   }
+  g.saves = a->pre0 != nullptr;
   if (a->y_dtype != B200MOE_DTYPE_F32) {
     DenseGemm w;
     w.a[0] = {a->x, a->m, a->k, a->ld_x};
@@ -1478,6 +1548,9 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
     w.rows = a->m;
     w.cols = a->n;
     w.red = a->k;
+    w.act = g.act;
+    w.has_residual = g.has_residual;
+    w.saves = g.saves;
     double time = 0.0;
     pair_cols(&w, 1, di, &time);
     if (time < tile_shape(g, di).time) {
@@ -1644,8 +1717,12 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
     int64_t rows_per_block;
     const int row_blocks = grad_row_blocks(a->m, a->n, &rows_per_block);
     const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)row_blocks);
-    act_grad_kernel<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo,
-                                              sums, a->act, a->dtype == B200MOE_DTYPE_F16, dy_f32, vec, rows_per_block);
+    const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_kernel<B200MOE_ACT_RELU>
+                      : a->act == B200MOE_ACT_SILU ? act_grad_kernel<B200MOE_ACT_SILU>
+                      : a->act == B200MOE_ACT_GELU ? act_grad_kernel<B200MOE_ACT_GELU>
+                                                   : act_grad_kernel<B200MOE_ACT_NONE>;
+    kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo, sums,
+                                   a->dtype == B200MOE_DTYPE_F16, dy_f32, vec, rows_per_block);
     B200_CUDA_CHECK(cudaGetLastError());
     if (sums) {
       column_sum_kernel<<<(unsigned)((a->n + 255) / 256), 256, 0, stream>>>(sums, row_blocks, (int)a->n, a->dbias);
