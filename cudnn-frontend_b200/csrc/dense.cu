@@ -237,13 +237,16 @@ __device__ __forceinline__ void act_values(float* v, int act) {
 // warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (TMEM lane quarter x every other 16 columns)
 // ---------------------------------------------------------------------------------------
 constexpr int DENSE_THREADS = 320;
+// Two CTAs fit an SM only if registers suffice for 12 + 12 warps: the warps of both start at the same of the SM's four parts, so
+// two of them hold 6 (95 registers a thread left one CTA to an SM).
+constexpr int DENSE_BOUND = 384;
 constexpr int DENSE_SMEM = 112 * 1024;       // per CTA, two CTAs to an SM
 constexpr int DENSE_SMEM_ALONE = 225 * 1024;  // where every CTA has an SM of its own
 constexpr int kSegTiles = 8;
 constexpr int kSegCols = 128;
 
 template <bool kTrans, int kEpi, bool kSeg>
-__global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
+__global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t s_bars[2 * 16 + 4];
@@ -608,10 +611,14 @@ __global__ void __launch_bounds__(DENSE_THREADS, kSeg ? 1 : 2) dense_tile_kernel
     each_chunk([&](int c0, const float* v) {
       if (!row_ok) return;
       if constexpr (kTrans) {
-        float w[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = v[j];
-        finish(std::integral_constant<int, 16>(), row, c0, 1, min(16, valid - c0), bias, w, w);
+        for (int h = 0; h < 16; h += 8) {
+          if (c0 + h >= valid) break;
+          float w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = v[h + j];
+          finish(std::integral_constant<int, 8>(), row, c0 + h, 1, min(8, valid - c0 - h), bias, w, w);
+        }
       } else {
         const int64_t o = (int64_t)row * p.ld_out + col0 + c0;
         if (p.vec_store && c0 + 16 <= valid) {
@@ -1044,65 +1051,92 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 // ---------------------------------------------------------------------------------------
 constexpr int GRAD_COLS = 256;  // columns of a block: 32 lanes x 8
 
-// 8 neighbouring values; beyond `count` zeros.  `whole`: 16-byte aligned and all there
-__device__ __forceinline__ void load8_16(const uint16_t* src, bool whole, int count, bool f16, float* v) {
-  if (whole) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 neighbouring 16-bit or float32 values as they lie in memory, and as float32.  `whole`: 16-byte aligned and all there,
+// otherwise the first `count` exist and zeros follow.  Loading and unpacking are apart so that every load of a step is on its way
+// before the first is used (interleaved with the arithmetic, these kernels ran at 3 TB/s).
+struct Raw8 {
+  uint4 a, b;  // b: the second half of float32 values
+};
+template <bool kF32>
+__device__ __forceinline__ Raw8 raw8(const void* base, int64_t i, bool whole, int count) {
+  Raw8 r;
+  r.a = r.b = make_uint4(0, 0, 0, 0);
+  if constexpr (kF32) {
+    const float* src = reinterpret_cast<const float*>(base) + i;
+    if (whole) {
+      r.a = __ldg(reinterpret_cast<const uint4*>(src));
+      r.b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    } else {
+      uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 p = unpack16x2(w[j], f16);
-      v[2 * j] = p.x, v[2 * j + 1] = p.y;
+      for (int j = 0; j < 8; ++j) w[j] = j < count ? __float_as_uint(src[j]) : 0u;
+      r.a = make_uint4(w[0], w[1], w[2], w[3]);
+      r.b = make_uint4(w[4], w[5], w[6], w[7]);
     }
   } else {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(base) + i;
+    if (whole) {
+      r.a = __ldg(reinterpret_cast<const uint4*>(src));
+    } else {
+      uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? load16(src, j, f16) : 0.0f;
+      for (int j = 0; j < 8; ++j) w[j] = j < count ? src[j] : 0u;
+      r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+  }
+  return r;
+}
+template <bool kF32, bool kF16>
+__device__ __forceinline__ void values8(const Raw8& r, float* v) {
+  if constexpr (kF32) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+  } else {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 p = unpack16x2(w[j], kF16);
+      v[2 * j] = p.x, v[2 * j + 1] = p.y;
+    }
   }
 }
-__device__ __forceinline__ void load8_f32(const float* src, bool whole, int count, float* v) {
-  if (whole) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? src[j] : 0.0f;
-  }
+template <bool kF16>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack16x2_from_float(v[0], v[1], kF16), pack16x2_from_float(v[2], v[3], kF16), pack16x2_from_float(v[4], v[5], kF16),
+                    pack16x2_from_float(v[6], v[7], kF16));
 }
 
-// dg, du [m, ldo] from dh, gate, up [m, n]
+// dg, du [m, ldo] from dh, gate, up [m, n]: 10 bytes per value, bound by HBM (4096 x 14336: 587 MB)
+template <int kAct, bool kF16>
 __global__ void __launch_bounds__(256)
     glu_grad_kernel(const void* __restrict__ dh, const void* __restrict__ gate, const void* __restrict__ up, int64_t m, int n, int64_t ld_dh,
-                    int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int act, int f16, int vec) {
+                    int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int vec) {
   pdl_trigger();
   const int c = (int)blockIdx.x * GRAD_COLS + (threadIdx.x & 31) * 8;
   if (c >= n) return;
+  const bool whole = vec && c + 8 <= n;
   for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < m; r += (int64_t)gridDim.y * 8) {
+    const Raw8 rd = raw8<false>(dh, r * ld_dh + c, whole, n - c), rg = raw8<false>(gate, r * ld_gate + c, whole, n - c),
+               ru = raw8<false>(up, r * ld_up + c, whole, n - c);
     float d[8], g[8], u[8];
-    const bool whole = vec && c + 8 <= n;
-    load8_16(reinterpret_cast<const uint16_t*>(dh) + r * ld_dh + c, whole, n - c, f16 != 0, d);
-    load8_16(reinterpret_cast<const uint16_t*>(gate) + r * ld_gate + c, whole, n - c, f16 != 0, g);
-    load8_16(reinterpret_cast<const uint16_t*>(up) + r * ld_up + c, whole, n - c, f16 != 0, u);
-    uint32_t gw[4], uw[4];
+    values8<false, kF16>(rd, d);
+    values8<false, kF16>(rg, g);
+    values8<false, kF16>(ru, u);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float a0, a1, b0, b1;
-      glu_grad_f(d[j], g[j], u[j], act, a0, b0);
-      glu_grad_f(d[j + 1], g[j + 1], u[j + 1], act, a1, b1);
-      gw[j / 2] = pack16x2_from_float(a0, a1, f16);
-      uw[j / 2] = pack16x2_from_float(b0, b1, f16);
-    }
+    for (int j = 0; j < 8; ++j) glu_grad_f(d[j], g[j], u[j], kAct, g[j], u[j]);
     // (the padding columns of the last 8 are written too: they are part of the padded row)
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = make_uint4(gw[0], gw[1], gw[2], gw[3]);
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = make_uint4(uw[0], uw[1], uw[2], uw[3]);
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = pack8<kF16>(g);
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = pack8<kF16>(u);
   }
 }
 
 // dz [m, ldo] = dy act'(z) (dz == NULL: dy is used as it is), and the column sums of the unrounded dz over the block's
 // rows: sums [gridDim.y][n].  Every sum has a fixed order: a warp's rows, then the warps, then (next kernel) the blocks.
-template <int kAct>
+template <int kAct, bool kF16, bool kDyF32>
 __global__ void __launch_bounds__(256)
     act_grad_kernel(const void* __restrict__ dy, const void* __restrict__ z, int64_t m, int n, int64_t ld_dy, int64_t ld_z, void* __restrict__ dz,
-                    int64_t ldo, float* __restrict__ sums, int f16, int dy_f32, int vec, int64_t rows_per_block) {
+                    int64_t ldo, float* __restrict__ sums, int vec, int64_t rows_per_block) {
   __shared__ float s_part[8][GRAD_COLS];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1113,33 +1147,30 @@ __global__ void __launch_bounds__(256)
   const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(m, r0 + rows_per_block);
   if (c < n) {
     const bool whole = vec && c + 8 <= n;
-    // two rows in flight per warp
-    for (int64_t r = r0 + warp; r < r1; r += 16) {
-      float d[2][8], g[2][8];
+    constexpr int kRows = 2;  // in flight per warp
+    for (int64_t r = r0 + warp; r < r1; r += 8 * kRows) {
+      Raw8 rd[kRows], rz[kRows];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int64_t row = r + 8 * q;
-        if (row < r1) {
-          if (dy_f32) load8_f32(reinterpret_cast<const float*>(dy) + row * ld_dy + c, whole, n - c, d[q]);
-          else load8_16(reinterpret_cast<const uint16_t*>(dy) + row * ld_dy + c, whole, n - c, f16 != 0, d[q]);
-          if (kAct != B200MOE_ACT_NONE) load8_16(reinterpret_cast<const uint16_t*>(z) + row * ld_z + c, whole, n - c, f16 != 0, g[q]);
-        }
+      for (int q = 0; q < kRows; ++q) {
+        const int64_t row = min(r + 8 * q, r1 - 1);
+        rd[q] = raw8<kDyF32>(dy, row * ld_dy + c, whole, n - c);
+        if (kAct != B200MOE_ACT_NONE) rz[q] = raw8<false>(z, row * ld_z + c, whole, n - c);
       }
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < kRows; ++q) {
         const int64_t row = r + 8 * q;
         if (row >= r1) break;
+        float d[8];
+        values8<kDyF32, kF16>(rd[q], d);
+        if (kAct != B200MOE_ACT_NONE) {
+          float g[8];
+          values8<false, kF16>(rz[q], g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (kAct != B200MOE_ACT_NONE) d[q][j] = c + j < n ? d[q][j] * act_grad_f(g[q][j], kAct) : 0.0f;
-          acc[j] += d[q][j];
+          for (int j = 0; j < 8; ++j) d[j] *= act_grad_f(g[j], kAct);
         }
-        if (dz) {
-          uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = pack16x2_from_float(d[q][2 * j], d[q][2 * j + 1], f16 != 0);
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int j = 0; j < 8; ++j) acc[j] += d[j];
+        if (dz) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = pack8<kF16>(d);
       }
     }
   }
@@ -1232,6 +1263,7 @@ static int dense_launch_tile(const DenseMaps& maps, const DenseParams& p, unsign
   B200_CUDA_CHECK(cudaGetDevice(&dev));
   if (!(ready.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
     B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM_ALONE));
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     ready.fetch_or(1ull << (dev & 63));
   }
   LaunchConfig c(grid, DENSE_THREADS, (size_t)p.smem_bytes, p.split, stream);
@@ -1260,6 +1292,9 @@ struct TileShape {
   int64_t tiles;
   double time;
 };
+// SMs that clusters of this size can occupy at once: a cluster lies within one of the chip's groups of SMs, whose sizes are no
+// multiple of 4 or 8 (of 148 SMs: 33 clusters of 4, 15 of 8)
+static int cluster_slots(int split, const DeviceInfo* di) { return split <= 2 ? di->sm_count / 2 * 2 : (split == 4 ? di->sm_count * 33 / 148 * 4 : di->sm_count * 15 / 148 * 8); }
 static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
   const int64_t tile_rows = g.dual ? 64 : 128;
   const int64_t rows = (g.rows + tile_rows - 1) / tile_rows * (g.stacked ? 2 : 1);
@@ -1271,8 +1306,8 @@ static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
     const int64_t tiles = rows * ((g.cols + c - 1) / c);
     const double bytes = DENSE_A_BYTES + c * 128;
     for (int split = 1; split <= DENSE_MAX_SPLIT && split * 4 <= std::max<int64_t>(4, stages); split *= 2) {
-      const int64_t ctas = tiles * split;
-      const int64_t per_sm = (ctas + di->sm_count - 1) / di->sm_count;
+      const int64_t ctas = tiles * split, slots = cluster_slots(split, di);
+      const int64_t per_sm = (ctas + slots - 1) / slots;
       const double together = per_sm > 1 ? 2.0 : 1.0, rounds = per_sm > 1 ? (double)((per_sm + 1) / 2) : 1.0;
       const double stage = std::max({205.0, together * bytes / 160.0, together * bytes * (double)std::min<int64_t>(ctas, di->sm_count) / 15800.0});
       const double load = std::max(rounds * (double)((stages + split - 1) / split) * stage, memory_ns(g));
@@ -1305,7 +1340,7 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   p.stage_bytes = DENSE_A_BYTES + C * 128;
   const int reduce_bytes = p.split > 1 ? (C + p.split - 1) * 512 : 0;
   // (the loads of a CTA come after about 1.4 us at 80 GB/s and SM: 110 KB in flight, so a CTA alone on its SM takes it all)
-  p.smem_bytes = tiles * p.split <= di->sm_count ? DENSE_SMEM_ALONE : DENSE_SMEM;
+  p.smem_bytes = tiles * p.split <= cluster_slots(p.split, di) ? DENSE_SMEM_ALONE : DENSE_SMEM;
   p.reduce_in_ring = p.split > 1 && C == 128 && p.smem_bytes == DENSE_SMEM;
   p.stages = std::min(16, (p.smem_bytes - 1024 - (p.reduce_in_ring ? 0 : reduce_bytes)) / p.stage_bytes);
   p.reduce_offset = p.split > 1 && !p.reduce_in_ring ? p.stages * p.stage_bytes : 0;
@@ -1575,6 +1610,12 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
   return dense_gemm(g, p, di, stream);
 }
 
+template <int kAct>
+static auto act_grad_of(bool f16, bool dy_f32) {
+  return f16 ? (dy_f32 ? act_grad_kernel<kAct, true, true> : act_grad_kernel<kAct, true, false>)
+             : (dy_f32 ? act_grad_kernel<kAct, false, true> : act_grad_kernel<kAct, false, false>);
+}
+
 // blocks along the rows of act_grad_kernel, and the rows of each
 static int grad_row_blocks(int64_t m, int64_t n, int64_t* rows_per_block) {
   const int64_t col_blocks = (n + GRAD_COLS - 1) / GRAD_COLS;
@@ -1685,8 +1726,10 @@ extern "C" int b200moe_gated_ffn_backward(const b200moe_dense_args* a, void* str
   void* du = (uint8_t*)a->workspace + round256(a->m * ldo * 2);
   const int vec = aligned16(a->dy) && aligned16(a->pre0) && aligned16(a->pre1) && a->ld_dy % 8 == 0 && a->ld_pre0 % 8 == 0 && a->ld_pre1 % 8 == 0;
   const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)std::min<int64_t>((a->m + 7) / 8, 32768));
-  glu_grad_kernel<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, dg, du, ldo, a->act,
-                                            a->dtype == B200MOE_DTYPE_F16, vec);
+  const bool f16 = a->dtype == B200MOE_DTYPE_F16, geglu = a->act == B200MOE_ACT_GEGLU;
+  const auto kern = geglu ? (f16 ? glu_grad_kernel<B200MOE_ACT_GEGLU, true> : glu_grad_kernel<B200MOE_ACT_GEGLU, false>)
+                          : (f16 ? glu_grad_kernel<B200MOE_ACT_SWIGLU, true> : glu_grad_kernel<B200MOE_ACT_SWIGLU, false>);
+  kern<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, dg, du, ldo, vec);
   B200_CUDA_CHECK(cudaGetLastError());
   const void* dz[2] = {dg, du};
   return dense_grad_products(a, 2, dz, ldo, di, stream);
@@ -1717,12 +1760,13 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
     int64_t rows_per_block;
     const int row_blocks = grad_row_blocks(a->m, a->n, &rows_per_block);
     const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)row_blocks);
-    const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_kernel<B200MOE_ACT_RELU>
-                      : a->act == B200MOE_ACT_SILU ? act_grad_kernel<B200MOE_ACT_SILU>
-                      : a->act == B200MOE_ACT_GELU ? act_grad_kernel<B200MOE_ACT_GELU>
-                                                   : act_grad_kernel<B200MOE_ACT_NONE>;
-    kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo, sums,
-                                   a->dtype == B200MOE_DTYPE_F16, dy_f32, vec, rows_per_block);
+    const bool f16 = a->dtype == B200MOE_DTYPE_F16;
+    const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_of<B200MOE_ACT_RELU>(f16, dy_f32)
+                      : a->act == B200MOE_ACT_SILU ? act_grad_of<B200MOE_ACT_SILU>(f16, dy_f32)
+                      : a->act == B200MOE_ACT_GELU ? act_grad_of<B200MOE_ACT_GELU>(f16, dy_f32)
+                                                   : act_grad_of<B200MOE_ACT_NONE>(f16, dy_f32);
+    kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo, sums, vec,
+                                   rows_per_block);
     B200_CUDA_CHECK(cudaGetLastError());
     if (sums) {
       column_sum_kernel<<<(unsigned)((a->n + 255) / 256), 256, 0, stream>>>(sums, row_blocks, (int)a->n, a->dbias);
