@@ -78,33 +78,52 @@ __device__ __forceinline__ float choice_weight(float logit, bool chosen, int sig
   return scale * (sigmoid ? sigmoid_exact_f(logit) : expf(logit - row_max) / row_sum);
 }
 
-// One warp per row; lane l holds experts l, l + 32, ...
+// One warp per row; a lane holds kVec neighbouring experts of every 32 kVec.
 //
 // With more than 32 experts the choice goes by candidates: the topk-th largest of the lanes' own maxima is a lower bound of the
 // topk-th largest value, and what reaches it (about topk + 2 of 256) is packed one to a lane and ranked by
 // counting.  Of a biased sigmoid the lanes hold a float32 score that is off by less than 2e-6 (1 + |score|), so the bound
-// is lowered by twice that; where two candidates are nearer than that to one another, the scores of all of them are formed in
-// 64 bits.  Rows with more than 32 candidates, and biased softmax scores (whose sum over the row is needed in 64 bits),
-// take the maxima one after the other.
+// is lowered by twice that; where two neighbours of the ranking are nearer than that to one another, the scores of all candidates
+// are formed in 64 bits.  Rows with more than 32 candidates, and biased softmax scores (whose sum over the row is needed in
+// 64 bits), take the maxima one after the other.
+template <int kPerLane>
+struct RowLayout {
+  static constexpr int kVec = kPerLane >= 4 ? 4 : 1;
+  static __device__ __forceinline__ int expert(int lane, int i) { return (i / kVec) * 32 * kVec + lane * kVec + i % kVec; }
+  static __device__ __forceinline__ int lane(int expert) { return expert / kVec % 32; }
+  static __device__ __forceinline__ int slot(int expert) { return expert / (32 * kVec) * kVec + expert % kVec; }
+};
+
 template <int kPerLane, bool kBias>
 __global__ void __launch_bounds__(256)
     router_topk_kernel(const void* __restrict__ logits, int dtype, int64_t rows, int experts, int64_t ld, const float* __restrict__ bias, int topk,
-                       int sigmoid, int normalize, float scale, float* __restrict__ weights, int32_t* __restrict__ ids) {
+                       int sigmoid, int normalize, float scale, int vec, float* __restrict__ weights, int32_t* __restrict__ ids) {
+  using Row = RowLayout<kPerLane>;
   __shared__ int2 s_choice[8][32];
-  __shared__ uint32_t s_order[8][32];
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
-  int2* choice = s_choice[threadIdx.x >> 5];
-  uint32_t* order = s_order[threadIdx.x >> 5];
+  int2* choice = s_choice[threadIdx.x >> 5];  // key, expert
   float v[kPerLane];
-  if (dtype == B200MOE_DTYPE_F32) {
-    const float* src = reinterpret_cast<const float*>(logits) + row * ld;
+  if (Row::kVec == 4 && vec) {  // (experts a multiple of 4, rows aligned)
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < experts ? __ldg(src + lane + 32 * i) : -INFINITY;
+    for (int i = 0; i < kPerLane; i += 4) {
+      const int e = Row::expert(lane, i);
+      v[i] = v[(i + 1) % kPerLane] = v[(i + 2) % kPerLane] = v[(i + 3) % kPerLane] = -INFINITY;
+      if (e < experts) {
+        if (dtype == B200MOE_DTYPE_F32) {
+          const float4 w = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(logits) + row * ld + e));
+          v[i] = w.x, v[(i + 1) % kPerLane] = w.y, v[(i + 2) % kPerLane] = w.z, v[(i + 3) % kPerLane] = w.w;
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(logits) + row * ld + e));
+          const float2 lo = unpack16x2(w.x, dtype == B200MOE_DTYPE_F16), hi = unpack16x2(w.y, dtype == B200MOE_DTYPE_F16);
+          v[i] = lo.x, v[(i + 1) % kPerLane] = lo.y, v[(i + 2) % kPerLane] = hi.x, v[(i + 3) % kPerLane] = hi.y;
+        }
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) v[i] = lane + 32 * i < experts ? load_any(logits, row * ld + lane + 32 * i, dtype) : -INFINITY;
+    for (int i = 0; i < kPerLane; ++i) v[i] = Row::expert(lane, i) < experts ? load_any(logits, row * ld + Row::expert(lane, i), dtype) : -INFINITY;
   }
   float row_max = -INFINITY, row_sum = 1.0f;
   if (!sigmoid && !normalize) {
@@ -121,10 +140,28 @@ __global__ void __launch_bounds__(256)
   bool done = false;
   if (kPerLane > 1 && (!kBias || sigmoid)) {
     uint32_t key[kPerLane], best = kNever;
+    float offset[kBias ? kPerLane : 1];
+    if constexpr (kBias) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) offset[i] = 0.0f;
+      if (Row::kVec == 4 && vec) {
+#pragma unroll
+        for (int i = 0; i < kPerLane; i += 4) {
+          if (Row::expert(lane, i) < experts) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(bias + Row::expert(lane, i)));
+            offset[i] = w.x, offset[(i + 1) % kPerLane] = w.y, offset[(i + 2) % kPerLane] = w.z, offset[(i + 3) % kPerLane] = w.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+          if (Row::expert(lane, i) < experts) offset[i] = __ldg(bias + Row::expert(lane, i));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       float value = v[i];
-      if (kBias) value = v[i] == -INFINITY ? v[i] : rcp_approx(1.0f + ex2_approx(v[i] * -1.4426950408889634f)) + __ldg(bias + lane + 32 * i);
+      if constexpr (kBias) value = v[i] == -INFINITY ? v[i] : rcp_approx(1.0f + ex2_approx(v[i] * -1.4426950408889634f)) + offset[i];
       key[i] = order_key(value);
       best = max(best, key[i]);
     }
@@ -141,49 +178,46 @@ __global__ void __launch_bounds__(256)
     }
     bound = max(bound, kNever + 1u);
     int count = 0;
+    const unsigned before = (1u << lane) - 1;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const bool in = key[i] >= bound;
       const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (in) {
-        const int at = count + __popc(who & ((1u << lane) - 1));
-        if (at < 32) {
-          choice[at] = make_int2(lane + 32 * i, __float_as_int(v[i]));
-          order[at] = key[i];
-        }
-      }
+      const int at = count + __popc(who & before);
+      if (in && at < 32) choice[at] = make_int2((int)key[i], Row::expert(lane, i));
       count += __popc(who);
     }
     __syncwarp();
     if (fits && count <= 32) {
       const int2 mine = choice[lane];  // (lanes beyond the count hold what is not used)
-      const uint32_t k = order[lane];
       int place = 0;
-      bool near = false;
-      const float score = key_value(k), margin = 4e-6f * (1.0f + fabsf(score));
       for (int q = 0; q < count; ++q) {
-        const uint32_t other = order[q];
-        const int id = choice[q].x;
-        place += other > k || (other == k && id < mine.x);
-        // (a NaN or an infinity is near nothing and needs no digits)
-        if (kBias) near |= id != mine.x && fabsf(key_value(other) - score) <= margin;
-      }
-      if (kBias && __any_sync(0xffffffffu, near && lane < count)) {
-        uint64_t wide = 0;
-        if (lane < count) wide = order_key64(1.0 / (1.0 + exp(-(double)__int_as_float(mine.y))) + (double)bias[mine.x]);
-        place = 0;
-        for (int q = 0; q < count; ++q) {
-          const uint64_t other = __shfl_sync(0xffffffffu, wide, q);
-          const int id = choice[q].x;
-          place += other > wide || (other == wide && id < mine.x);
-        }
+        const int2 other = choice[q];
+        place += (uint32_t)other.x > (uint32_t)mine.x || (other.x == mine.x && other.y < mine.y);
       }
       __syncwarp();
       if (lane < count) choice[place] = mine;  // the places are a permutation of the candidates
       __syncwarp();
+      if constexpr (kBias) {
+        // (a NaN or an infinity is near nothing and needs no digits)
+        const float score = key_value((uint32_t)choice[lane].x), next = key_value((uint32_t)choice[min(lane + 1, 31)].x);
+        if (__any_sync(0xffffffffu, lane + 1 < count && score - next <= 4e-6f * (1.0f + fabsf(score)))) {
+          uint64_t wide = 0;
+          if (lane < count) wide = order_key64(1.0 / (1.0 + exp(-(double)load_any(logits, row * ld + mine.y, dtype))) + (double)bias[mine.y]);
+          place = 0;
+          for (int q = 0; q < count; ++q) {
+            const uint64_t other = __shfl_sync(0xffffffffu, wide, q);
+            const int id = __shfl_sync(0xffffffffu, mine.y, q);
+            place += other > wide || (other == wide && id < mine.y);
+          }
+          __syncwarp();
+          if (lane < count) choice[place] = mine;
+          __syncwarp();
+        }
+      }
       if (lane < min(count, topk)) {
-        my_id = choice[lane].x;
-        my_logit = __int_as_float(choice[lane].y);
+        my_id = choice[lane].y;
+        my_logit = kBias ? load_any(logits, row * ld + my_id, dtype) : key_value((uint32_t)choice[lane].x);
       }
       done = true;
     }
@@ -208,7 +242,7 @@ __global__ void __launch_bounds__(256)
       if (!sigmoid) sum = warp_sum(sum);
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) {
-        const int e = lane + 32 * i;
+        const int e = Row::expert(lane, i);
         key[i] = v[i] == -INFINITY ? kNever64 : order_key64((sigmoid ? wide[i] : wide[i] / sum) + (double)(e < experts ? bias[e] : 0.0f));
       }
     } else {
@@ -232,13 +266,13 @@ __global__ void __launch_bounds__(256)
         top = __reduce_max_sync(0xffffffffu, best);
       }
       if (top <= never) break;  // nothing left that may be chosen
-      const int id = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * at : 0x7fffffff);
-      const float l = __shfl_sync(0xffffffffu, logit, id & 31);
+      const int id = __reduce_min_sync(0xffffffffu, best == top ? Row::expert(lane, at) : 0x7fffffff);
+      const float l = __shfl_sync(0xffffffffu, logit, Row::lane(id));
       if (lane == j) my_id = id, my_logit = l;
-      if (lane == (id & 31)) {
+      if (lane == Row::lane(id)) {
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i)
-          if (i == (id >> 5)) key[i] = never;
+          if (i == Row::slot(id)) key[i] = never;
       }
     }
   }
@@ -336,8 +370,9 @@ template <int kPerLane>
 static void router_launch(const void* logits, int dtype, int64_t rows, int experts, int64_t ld, const float* bias, int topk, int sigmoid, int normalize,
                           float scale, float* weights, int32_t* ids, cudaStream_t stream) {
   const unsigned grid = (unsigned)((rows + 7) / 8);
-  if (bias) router_topk_kernel<kPerLane, true><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, weights, ids);
-  else router_topk_kernel<kPerLane, false><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, weights, ids);
+  const int vec = experts % 4 == 0 && ld % 4 == 0 && (uintptr_t)logits % 16 == 0 && (uintptr_t)bias % 16 == 0;
+  if (bias) router_topk_kernel<kPerLane, true><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, vec, weights, ids);
+  else router_topk_kernel<kPerLane, false><<<grid, 256, 0, stream>>>(logits, dtype, rows, experts, ld, bias, topk, sigmoid, normalize, scale, vec, weights, ids);
 }
 
 }  // namespace b200moe
