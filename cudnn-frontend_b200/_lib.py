@@ -76,7 +76,7 @@ class GemmArgs(Structure):
 class DenseArgs(Structure):
     _fields_ = [(name, c_void_p) for name in ("x", "w0", "w1", "bias", "residual", "dy", "y", "pre0", "pre1", "dx", "dw0", "dw1", "dbias", "workspace")] + [
         (name, c_int64) for name in ("workspace_bytes", "m", "n", "k", "ld_x", "ld_w0", "ld_w1", "ld_residual", "ld_dy", "ld_y", "ld_pre0", "ld_pre1")
-    ] + [(name, c_int32) for name in ("dtype", "y_dtype", "bias_dtype", "act", "wait_limit_ms")]  # fmt: skip
+    ] + [(name, c_int32) for name in ("dtype", "y_dtype", "bias_dtype", "act", "wait_limit_ms", "flags")]  # fmt: skip
 
 
 _SIGNATURES = {

@@ -54,6 +54,7 @@ struct DenseParams {
   const void* bias;
   const void* residual;
   int64_t ld_out, ld_res, ld_pre[2];
+  int test_skip_b_loads;     // test hook: no load of operand B is issued, so every wait runs out
   uint64_t wait_limit_ns;
 };
 
@@ -320,6 +321,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
     int kc = kt * DENSE_BK;
     uint32_t dst = ring, fb = full_bar(0), eb = empty_bar(0), parity = 1;
     const uint32_t go = elect_one();  // (the same lane of a full warp every time)
+    const uint32_t go_b = p.test_skip_b_loads ? 0u : go;
     int issued = 0;
     for (; issued < nk; ++issued) {
       if (!__all_sync(0xffffffffu, mbar_wait(eb, parity, wc, ST_DENSE_EMPTY))) break;
@@ -334,10 +336,10 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         load_2d_if<false>(go, dst, ma, fb, kc, row0);
       }
       if (b_mn) {
-        load_2d_if<false>(go, dst + DENSE_A_BYTES, mb, fb, col0, kc);
-        if (b_two) load_2d_if<false>(go, dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
+        load_2d_if<false>(go_b, dst + DENSE_A_BYTES, mb, fb, col0, kc);
+        if (b_two) load_2d_if<false>(go_b, dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
       } else {
-        load_2d_if<false>(go, dst + DENSE_A_BYTES, mb, fb, kc, col0);
+        load_2d_if<false>(go_b, dst + DENSE_A_BYTES, mb, fb, kc, col0);
       }
       kc += DENSE_BK;
       if (--chain_left == 0) {
@@ -695,6 +697,7 @@ struct PairParams {
   const void* residual;
   int64_t ld_res;
   int vec_res;                // residual rows may be read 16 bytes at a time
+  int test_skip_b_loads;      // test hook, as in DenseParams
   uint64_t wait_limit_ns;
 };
 
@@ -898,7 +901,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     int issued = 0;
     bool ok = true;
     const uint32_t go = elect_one();  // (the same lane of a full warp every time)
-    const uint32_t go_leader = rank == 0 ? go : 0u;
+    const uint32_t go_leader = rank == 0 ? go : 0u, go_b = p.test_skip_b_loads ? 0u : go;
     PairTile t;
     for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
       const PairJob& j = p.job[t.job];
@@ -924,10 +927,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           load_2d_if<true>(go, da, ma, fb, kc, a0);
         }
         if (b_mn) {
-          load_2d_if<true>(go, db, mb, fb, b0, kc);
-          if (half_cols > 64) load_2d_if<true>(go, db + DENSE_SLAB, mb, fb, b0 + 64, kc);
+          load_2d_if<true>(go_b, db, mb, fb, b0, kc);
+          if (half_cols > 64) load_2d_if<true>(go_b, db + DENSE_SLAB, mb, fb, b0 + 64, kc);
         } else {
-          load_2d_if<true>(go, db, mb, fb, kc, b0);
+          load_2d_if<true>(go_b, db, mb, fb, kc, b0);
         }
         ++issued;
         if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
@@ -1491,6 +1494,7 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
 
 static void pair_params(PairParams& p, const b200moe_dense_args* a) {
   memset(&p, 0, sizeof(p));
+  p.test_skip_b_loads = (a->flags & B200MOE_FLAG_TEST_SKIP_B_LOADS) != 0;
   p.f16 = a->dtype == B200MOE_DTYPE_F16;
   p.act = a->act;
   p.wait_limit_ns = a->wait_limit_ms > 0 ? (uint64_t)a->wait_limit_ms * 1000000ull : kWaitLimitNs;
@@ -1526,6 +1530,7 @@ static int dense_check_common(const char* op, const b200moe_dense_args* a, bool 
 
 static void dense_params(DenseParams& p, const b200moe_dense_args* a) {
   memset(&p, 0, sizeof(p));
+  p.test_skip_b_loads = (a->flags & B200MOE_FLAG_TEST_SKIP_B_LOADS) != 0;
   p.f16 = a->dtype == B200MOE_DTYPE_F16;
   p.act = a->act;
   p.wait_limit_ns = a->wait_limit_ms > 0 ? (uint64_t)a->wait_limit_ms * 1000000ull : kWaitLimitNs;

@@ -94,8 +94,9 @@ struct RowLayout {
   static __device__ __forceinline__ int slot(int expert) { return expert / (32 * kVec) * kVec + expert % kVec; }
 };
 
+// (six blocks to an SM instead of four: 23.7 -> 22.0 us for 32768 x 256 with a bias; the warps wait for one another's loads and votes)
 template <int kPerLane, bool kBias>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, kPerLane <= 8 ? 6 : (kPerLane == 16 ? 4 : 2))
     router_topk_kernel(const void* __restrict__ logits, int dtype, int64_t rows, int experts, int64_t ld, const float* __restrict__ bias, int topk,
                        int sigmoid, int normalize, float scale, int vec, float* __restrict__ weights, int32_t* __restrict__ ids) {
   using Row = RowLayout<kPerLane>;

@@ -419,6 +419,7 @@ typedef struct b200moe_dense_args {
   int32_t bias_dtype;
   int32_t act;
   int32_t wait_limit_ms; /* as in b200moe_gemm_args */
+  int32_t flags;         /* 0, or B200MOE_FLAG_TEST_SKIP_B_LOADS */
 } b200moe_dense_args;
 int b200moe_gated_ffn(const b200moe_dense_args* args, void* stream);
 int b200moe_gated_ffn_backward(const b200moe_dense_args* args, void* stream);

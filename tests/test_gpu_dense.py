@@ -393,3 +393,30 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,n,kernel", [(3, 256, "tile"), (40, 300, "tile"), (2048, 2048, "pair")])
+def test_bounded_waits_report_and_recover(m, n, kernel):
+    """A launch whose operand B never arrives ends after its wait limit, says which wait gave up, and leaves the device
+    usable: the next launch is right."""
+    import ctypes
+
+    import cudnn_frontend_b200 as cf
+    from cudnn_frontend_b200 import _lib, ops
+
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    k = 2048
+    x, w = rows(gen, m, k, BF16), rows(gen, n, k, BF16, scale=k**-0.5)
+    want = cf.linear(x, w)
+    y = torch.zeros_like(want)
+    args = dict(x=x.data_ptr(), w0=w.data_ptr(), y=y.data_ptr(), m=m, n=n, k=k, ld_x=k, ld_w0=k, ld_y=n, act=_lib.ACT_NONE, wait_limit_ms=20)
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) == 0
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _lib.load().b200moe_linear(ctypes.byref(_lib.DenseArgs(flags=_lib.FLAG_TEST_SKIP_B_LOADS, **args)), stream) == 0
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) in ({"tile": (401, 402, 403), "pair": (411, 412, 413, 414)}[kernel])
+    assert _lib.load().b200moe_linear(ctypes.byref(_lib.DenseArgs(**args)), stream) == 0
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) == 0
+    assert torch.equal(y, want)

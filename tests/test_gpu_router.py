@@ -41,7 +41,7 @@ def plain(logits, topk, score, normalize, bias, scale, dw=None):
     return out
 
 
-CASES = [(1, 1, 1), (3, 4, 2), (64, 8, 2), (5, 33, 7), (130, 64, 6), (257, 60, 4), (100, 256, 8), (9, 300, 16), (33, 512, 32), (17, 1024, 1), (2000, 128, 8)]
+CASES = [(1, 1, 1), (3, 4, 2), (64, 8, 2), (5, 33, 7), (130, 64, 6), (257, 60, 4), (100, 256, 8), (9, 300, 16), (33, 512, 32), (17, 1024, 1), (2000, 128, 8), (8195, 60, 8), (9000, 256, 3), (8193, 8, 2)]
 
 
 @pytest.mark.parametrize("t,e,k", CASES)
