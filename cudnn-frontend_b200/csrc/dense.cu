@@ -660,9 +660,11 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
 // the last wave of the first).  Tiles are dealt out in rounds; where the last round of job 0 leaves pairs idle, they
 // begin job 1 `early` rounds sooner.
 //
-// warps: 0 producer, 1 MMA issuer (first CTA) and TMEM owner, 2-9 epilogue (TMEM lane quarter x column half)
+// warps: 0 producer of A, 10 producer of B (with MN-major operands a stage takes four copies per CTA, more than one warp issues
+// in the time of its products), 1 MMA issuer (first CTA) and TMEM owner, 2-9 epilogue (TMEM lane quarter x column half)
 // ---------------------------------------------------------------------------------------
-constexpr int PAIR_THREADS = 320;
+constexpr int PAIR_THREADS = 352;
+constexpr int PAIR_WARP_B = 10;
 constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE_BYTES = 2 * DENSE_A_BYTES;
 constexpr int PAIR_EPI_WARPS = 8;
@@ -893,46 +895,47 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   pdl_wait();
   pdl_trigger();
 
-  if (warp == 0) {
-    // ---- producer: this CTA's halves of A and B; every copy is credited to the first CTA's barrier --------------
+  if (warp == 0 || warp == PAIR_WARP_B) {
+    // ---- producers: this CTA's halves of A and B; every copy is credited to the first CTA's barrier --------------
+    const bool side_b = warp != 0;
     const uint32_t leader_full0 = map_to_cta(full_bar(0), 0);
+    const uint32_t dst0 = ring + (side_b ? DENSE_A_BYTES : 0);
     int stage = 0;
     uint32_t phase = 0;
     int issued = 0;
     bool ok = true;
-    const uint32_t go = elect_one();  // (the same lane of a full warp every time)
-    const uint32_t go_leader = rank == 0 ? go : 0u, go_b = p.test_skip_b_loads ? 0u : go;
+    const uint32_t elected = elect_one();  // (the same lane of a full warp every time)
+    const uint32_t go = side_b && p.test_skip_b_loads ? 0u : elected;
+    const uint32_t go_announce = !side_b && rank == 0 ? elected : 0u;
     PairTile t;
     for (int i = 0; ok && pair_tile(p, pair, pairs, i, t); ++i) {
       const PairJob& j = p.job[t.job];
       const DenseMaps& m = maps.job[t.job];
-      const int a0 = t.row_tile * 256 + rank * 128;
       const int half_cols = j.tile_cols / 2;  // this CTA's columns of B
-      const int b0 = kEpi == DENSE_GLU ? t.col_tile * half_cols : t.col_tile * j.tile_cols + rank * half_cols;
-      const bool a_mn = j.a_mn != 0, b_mn = j.b_mn != 0;
+      const int first = !side_b                ? t.row_tile * 256 + rank * 128
+                        : kEpi == DENSE_GLU ? t.col_tile * half_cols
+                                            : t.col_tile * j.tile_cols + rank * half_cols;
+      const bool mn = (side_b ? j.b_mn : j.a_mn) != 0, two = !side_b || half_cols > 64;
       const uint32_t bytes = 2u * (uint32_t)(DENSE_A_BYTES + half_cols * 128);
-      for (int kt = 0; kt < j.k_tiles; ++kt) {
+      const CUtensorMap* map = side_b ? &m.b[kEpi == DENSE_GLU ? rank : 0] : &m.a[t.which];
+      const int k_tiles = j.k_tiles;
+      int chain_left = j.chain_tiles, kc = 0;
+      for (int kt = 0; kt < k_tiles; ++kt) {
         if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, wc, ST_PAIR_EMPTY))) { ok = false; break; }
-        const int chain = kt >= j.chain_tiles ? 1 : 0;
-        const int kc = (kt - chain * j.chain_tiles) * DENSE_BK;
-        const uint32_t fb = leader_full0 + 8u * stage;
-        const uint32_t da = ring + stage * PAIR_STAGE_BYTES, db = da + DENSE_A_BYTES;
-        const CUtensorMap* ma = &m.a[chain | t.which];
-        const CUtensorMap* mb = &m.b[kEpi == DENSE_GLU ? rank : chain];
-        expect_tx_if(go_leader, full_bar(stage), bytes);
-        if (a_mn) {
-          load_2d_if<true>(go, da, ma, fb, a0, kc);
-          load_2d_if<true>(go, da + DENSE_SLAB, ma, fb, a0 + 64, kc);
+        const uint32_t fb = leader_full0 + 8u * stage, dst = dst0 + stage * PAIR_STAGE_BYTES;
+        expect_tx_if(go_announce, full_bar(stage), bytes);
+        if (mn) {
+          load_2d_if<true>(go, dst, map, fb, first, kc);
+          if (two) load_2d_if<true>(go, dst + DENSE_SLAB, map, fb, first + 64, kc);
         } else {
-          load_2d_if<true>(go, da, ma, fb, kc, a0);
-        }
-        if (b_mn) {
-          load_2d_if<true>(go_b, db, mb, fb, b0, kc);
-          if (half_cols > 64) load_2d_if<true>(go_b, db + DENSE_SLAB, mb, fb, b0 + 64, kc);
-        } else {
-          load_2d_if<true>(go_b, db, mb, fb, kc, b0);
+          load_2d_if<true>(go, dst, map, fb, kc, first);
         }
         ++issued;
+        kc += DENSE_BK;
+        if (--chain_left == 0) {
+          kc = 0;
+          map = side_b ? &m.b[1] : &m.a[1];
+        }
         if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
       }
     }
@@ -1446,7 +1449,8 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
     const int64_t tiles = pair_tiles(g[i], tile_cols);
     if (tiles > 0x3fffffff) return fail(B200MOE_E_SHAPE, "the product has too many tiles");
     j.tiles = (int)tiles;
-    j.raster = 16;
+    // (8 and 16 row tiles to a group are alike within 2 %; 8 for the plain products, 16 for the gated block measured best)
+    j.raster = g[i].dual ? 16 : 8;
     j.idesc = dense_idesc(256, tile_cols, p.f16 != 0, g[i].a_mn, g[i].b_mn);
     const int na = (g[i].chained || g[i].stacked) ? 2 : 1, nb = (g[i].chained || g[i].dual) ? 2 : 1, no = j.stacked ? 2 : 1;
     for (int q = 0; q < na; ++q) {
