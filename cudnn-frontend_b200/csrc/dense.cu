@@ -235,9 +235,11 @@ __device__ __forceinline__ void act_values(float* v, int act) {
 // 7e-6 of the result (measured), 4e-7 over the 512 elements of a segment.  Used for float32 outputs; a 16-bit
 // output's rounding (2^-9) hides it.
 //
-// warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-9 epilogue (TMEM lane quarter x every other 16 columns)
+// warps: 0 producer of A, 10 producer of B, 1 MMA issuer and TMEM owner, 2-9 epilogue (TMEM lane quarter x every other 16
+// columns)
 // ---------------------------------------------------------------------------------------
-constexpr int DENSE_THREADS = 320;
+constexpr int DENSE_THREADS = 352;
+constexpr int DENSE_WARP_B = 10;
 // Two CTAs fit an SM only if registers suffice for 12 + 12 warps: the warps of both start at the same of the SM's four parts, so
 // two of them hold 6 (95 registers a thread left one CTA to an SM).
 constexpr int DENSE_BOUND = 384;
@@ -304,54 +306,50 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
   pdl_wait();
   pdl_trigger();
 
-  if (warp == 0) {
-    // ---- producer -----------------------------------------------------------------------
+  if (warp == 0 || (!kGlu && warp == DENSE_WARP_B)) {
+    // ---- producers ----------------------------------------------------------------------
     // (stage, parity and addresses run along: a division by the number of stages in this loop and the issuer's made a stage
-    // cost 700 cycles whatever it held)
-    const uint32_t stage_bytes = (uint32_t)p.stage_bytes, ring_end = ring + (uint32_t)stages * stage_bytes;
-    const bool a_mn = !kGlu && p.a_mn != 0, b_mn = p.b_mn != 0, b_two = C > 64;
-    int kt = kt0;
-    const CUtensorMap *ma = &maps.a[kGlu ? 0 : which], *mb = &maps.b[0];
-    int chain_left = p.chain_tiles - kt;
+    // cost 700 cycles whatever it held; one warp for both operands took 420.  The gated block's one warp issues both all the
+    // same: 17.5 us against 18.8 for 128 tokens of 7168 -> 2 x 2048.)
+    const bool side_b = warp != 0;
+    const uint32_t stage_bytes = (uint32_t)p.stage_bytes, dst0 = ring + (side_b ? DENSE_A_BYTES : 0), dst_end = dst0 + (uint32_t)stages * stage_bytes;
+    const bool mn = side_b ? p.b_mn != 0 : (!kGlu && p.a_mn != 0), two = !side_b || C > 64;
+    const int first = side_b ? col0 : row0;
+    const CUtensorMap* map = side_b ? &maps.b[0] : &maps.a[kGlu ? 0 : which];
+    const CUtensorMap* map1 = side_b ? &maps.b[1] : &maps.a[1];  // of the second chain, or the up weights
+    int kt = kt0, chain_left = p.chain_tiles - kt;
     if (chain_left <= 0) {
       kt -= p.chain_tiles;
-      ma = &maps.a[1];
-      mb = &maps.b[1];
+      map = map1;
     }
     int kc = kt * DENSE_BK;
-    uint32_t dst = ring, fb = full_bar(0), eb = empty_bar(0), parity = 1;
-    const uint32_t go = elect_one();  // (the same lane of a full warp every time)
-    const uint32_t go_b = p.test_skip_b_loads ? 0u : go;
+    uint32_t dst = dst0, fb = full_bar(0), eb = empty_bar(0), parity = 1;
+    const uint32_t elected = elect_one();  // (the same lane of a full warp every time)
+    const uint32_t go = side_b && p.test_skip_b_loads ? 0u : elected, go_announce = side_b ? 0u : elected;
     int issued = 0;
     for (; issued < nk; ++issued) {
       if (!__all_sync(0xffffffffu, mbar_wait(eb, parity, wc, ST_DENSE_EMPTY))) break;
-      expect_tx_if(go, fb, stage_bytes);
-      if constexpr (kGlu) {
-        load_2d_if<false>(go, dst, ma, fb, kc, row0);
-        load_2d_if<false>(go, dst + 64 * 128, ma + 1, fb, kc, row0);
-      } else if (a_mn) {
-        load_2d_if<false>(go, dst, ma, fb, row0, kc);
-        load_2d_if<false>(go, dst + DENSE_SLAB, ma, fb, row0 + 64, kc);
+      expect_tx_if(go_announce, fb, stage_bytes);
+      if (mn) {
+        load_2d_if<false>(go, dst, map, fb, first, kc);
+        if (two) load_2d_if<false>(go, dst + DENSE_SLAB, map, fb, first + 64, kc);
       } else {
-        load_2d_if<false>(go, dst, ma, fb, kc, row0);
-      }
-      if (b_mn) {
-        load_2d_if<false>(go_b, dst + DENSE_A_BYTES, mb, fb, col0, kc);
-        if (b_two) load_2d_if<false>(go_b, dst + DENSE_A_BYTES + DENSE_SLAB, mb, fb, col0 + 64, kc);
-      } else {
-        load_2d_if<false>(go_b, dst + DENSE_A_BYTES, mb, fb, kc, col0);
+        load_2d_if<false>(go, dst, map, fb, kc, first);
+        if constexpr (kGlu) {
+          load_2d_if<false>(go, dst + 64 * 128, map1, fb, kc, first);
+          load_2d_if<false>(p.test_skip_b_loads ? 0u : go, dst + DENSE_A_BYTES, &maps.b[0], fb, kc, col0);
+        }
       }
       kc += DENSE_BK;
       if (--chain_left == 0) {
         kc = 0;
-        ma = &maps.a[1];
-        mb = &maps.b[1];
+        map = map1;
       }
       dst += stage_bytes;
       fb += 8;
       eb += 8;
-      if (dst == ring_end) {
-        dst = ring;
+      if (dst == dst_end) {
+        dst = dst0;
         fb = full_bar(0);
         eb = empty_bar(0);
         parity ^= 1u;
@@ -410,12 +408,13 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
 
   // ---- epilogue -------------------------------------------------------------------------
   const bool f16 = p.f16 != 0;
+  const bool finisher = warp >= 2 && warp < 10;
   const int quarter = warp & 3, half = (warp - 2) >> 2;  // this warp: TMEM lanes 32 quarter .. + 31, chunks half, half + 2, ...
   const int r_in_tile = quarter * 32 + lane;
   const int valid = min(C, p.cols - col0);
   float sums[kSeg ? kSegCols / 2 : 1];
   bool ok = true;
-  if (warp >= 2) {
+  if (finisher) {
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     if constexpr (kSeg) {
 #pragma unroll
@@ -538,7 +537,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         cluster_wait();
       }
     }
-    if (warp >= 2 && ok) {
+    if (finisher && ok) {
       each_chunk([&](int c0, const float* v) {
         const int count = min(16, valid - c0);
         if (split == 1) {
@@ -572,7 +571,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
     } else {
       __syncthreads();
     }
-    if (warp >= 2) {
+    if (finisher) {
       constexpr int kGroups = 256 / kTileRows;  // columns in flight
       constexpr int kN = 8;
       const int t = (int)threadIdx.x - 64;
@@ -606,7 +605,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         }
       }
     }
-  } else if (warp >= 2 && ok) {
+  } else if (finisher && ok) {
     const int row = row0 + r_in_tile;
     const bool row_ok = row < p.rows;
     const float bias = bias_at(row);
@@ -1291,7 +1290,7 @@ static double memory_ns(const DenseGemm& g) {
 }
 
 // Columns of the tile kernel's tiles (as many as there are, up to 128; an MN-major B comes in slabs of 64) and the CTAs that
-// share a tile's reduction.  A stage takes a CTA 205 ns (the issuer's loop) or as long as its bytes take at 160 GB/s for the SM
+// share a tile's reduction.  A stage takes a CTA 190 ns (the issuer's loop) or as long as its bytes take at 160 GB/s for the SM
 // and 15.8 TB/s for all of L2; two CTAs run on an SM at once; joining partial sums costs more the more columns and CTAs.
 struct TileShape {
   int cols, split;
@@ -1315,7 +1314,7 @@ static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
       const int64_t ctas = tiles * split, slots = cluster_slots(split, di);
       const int64_t per_sm = (ctas + slots - 1) / slots;
       const double together = per_sm > 1 ? 2.0 : 1.0, rounds = per_sm > 1 ? (double)((per_sm + 1) / 2) : 1.0;
-      const double stage = std::max({205.0, together * bytes / 160.0, together * bytes * (double)std::min<int64_t>(ctas, di->sm_count) / 15800.0});
+      const double stage = std::max({190.0, together * bytes / 160.0, together * bytes * (double)std::min<int64_t>(ctas, di->sm_count) / 15800.0});
       const double load = std::max(rounds * (double)((stages + split - 1) / split) * stage, memory_ns(g));
       const double join = split > 1 || g.dual ? 1000.0 + 350.0 * split + 25.0 * c : 2000.0 + 8.0 * c;
       const double finish = join + epilogue_ns(g) * 128.0 * c / split * together;
@@ -1397,7 +1396,7 @@ static int dense_launch_pair(const PairMaps& maps, const PairParams& p, int pair
 }
 
 // The pair kernel's launch with tiles of `tile_cols` columns.  A stage of a 256 x 256 tile takes 285 ns (512 cycles of the tensor
-// cores), one of a 256 x 128 tile 210 ns (the issuer's loop); a tile's epilogue takes as long as 5 stages and hides behind
+// cores), one of a 256 x 128 tile 180 ns (the issuer's loop); a tile's epilogue takes as long as 5 stages and hides behind
 // the next tile's, the last one's does not; start and end cost 6 us.
 static int64_t pair_tiles(const DenseGemm& g, int tile_cols) {
   const int cols = g.dual ? tile_cols / 2 : tile_cols;
@@ -1405,7 +1404,7 @@ static int64_t pair_tiles(const DenseGemm& g, int tile_cols) {
 }
 static int64_t pair_stages(const DenseGemm& g) { return (g.red + DENSE_BK - 1) / DENSE_BK * (g.chained ? 2 : 1); }
 static double pair_time(const DenseGemm* g, int jobs, int tile_cols, int pairs) {
-  const double stage = tile_cols == 256 ? 285.0 : 210.0;
+  const double stage = tile_cols == 256 ? 285.0 : 180.0;
   double longest = 0.0, all = 0.0, memory = 0.0, last = 0.0;
   int64_t tiles = 0;
   for (int i = 0; i < jobs; ++i) {
