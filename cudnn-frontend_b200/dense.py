@@ -8,19 +8,21 @@ residual in its epilogue.  Both have their backward pass.  The reference has no 
 All functions take bf16 or fp16 tensors ``[rows, cols]`` with contiguous rows (any pitch that is a multiple
 of 8 elements, 16-byte aligned, for what a tensor map reads: ``x`` and the weights), sum in float32 and round
 once.  They allocate their outputs and launch on ``stream`` (default: the current stream of the tensors' device); when
-another stream is passed, outputs and workspace belong to that stream.  They are not recorded by autograd:
-the backward functions are called explicitly, as with the grouped GEMMs.
+another stream is passed, outputs and workspace belong to that stream, and inputs must stay alive until it has passed the
+call.  They are not recorded by autograd: the backward functions are called explicitly, as with the grouped GEMMs.
+While ``torch.compile`` traces, the forward functions go through custom ops (``torch.ops.b200moe.gated_ffn`` and ``linear``),
+so the graph sees one opaque op per launch.
 """
 
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .ops import call_on
+from .ops import _ptr, call_on
 
 _TYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _GLU = {"swiglu": _lib.ACT_SWIGLU, "geglu": _lib.ACT_GEGLU}
@@ -61,6 +63,11 @@ def _weight(name: str, w: torch.Tensor, k: int, x: torch.Tensor) -> int:
     return _pitch(name, w, shape, x.dtype, x.device)
 
 
+def _eager_stream_only(stream) -> None:
+    if stream is not None:
+        raise NotImplementedError("stream is an eager-only launch option")
+
+
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_func: str = "swiglu", return_preact: bool = False, stream=None):
     """``act(x w_gate^T) * (x w_up^T)``: ``x [tokens, k]``, weights ``[n, k]`` -> ``h [tokens, n]``, and with
     ``return_preact`` also ``gate`` and ``up`` (what :func:`gated_ffn_backward` reads).
@@ -68,6 +75,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_fun
     ``act_func`` as in the grouped FC1: ``"swiglu"`` = ``gate * sigmoid(gate) * up``, ``"geglu"`` = the reference's
     GeGLU, ``gate <= 7``, ``-7 <= up <= 7``, ``(up + 1) * gate * sigmoid(1.702 * gate)`` (gate and up are returned
     without the limits)."""
+    if torch.compiler.is_compiling():
+        _eager_stream_only(stream)
+        out = torch.ops.b200moe.gated_ffn(x, w_gate, w_up, act_func, return_preact)
+        return tuple(out) if return_preact else out[0]
     m, k = _check_x(x)
     if act_func not in _GLU:
         raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
@@ -92,9 +103,10 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_fun
 
 
 def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
-                       act_func: str = "swiglu", stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+                       act_func: str = "swiglu", input_grad: bool = True, weight_grad: bool = True, stream=None):  # fmt: skip
     """Backward pass of :func:`gated_ffn` from ``dh [tokens, n]`` and the saved ``gate`` and ``up``: returns
-    ``(dx, dw_gate, dw_up)``.  A value that GeGLU limits has no gradient."""
+    ``(dx, dw_gate, dw_up)``, with ``None`` for what ``input_grad`` or ``weight_grad`` leaves out.  A value that GeGLU limits has
+    no gradient."""
     m, k = _check_x(x)
     if act_func not in _GLU:
         raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
@@ -107,13 +119,14 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
 
     def launch(s):
         lib = _lib.load()
-        dx, dw_gate, dw_up = x.new_empty((m, k)), x.new_empty((n, k)), x.new_empty((n, k))
+        dx = x.new_empty((m, k)) if input_grad else None
+        dw_gate, dw_up = (x.new_empty((n, k)), x.new_empty((n, k))) if weight_grad else (None, None)
         need = lib.b200moe_dense_workspace_bytes(m, n, 1)
         work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
         args = _lib.DenseArgs(
-            x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), dy=dh.data_ptr(), pre0=gate.data_ptr(), pre1=up.data_ptr(), dx=dx.data_ptr(),
-            dw0=dw_gate.data_ptr(), dw1=dw_up.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g,
+            x=x.data_ptr(), w0=w_gate.data_ptr(), w1=w_up.data_ptr(), dy=dh.data_ptr(), pre0=gate.data_ptr(), pre1=up.data_ptr(),
+            dx=_ptr(dx), dw0=_ptr(dw_gate), dw1=_ptr(dw_up), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x, ld_w0=ld_g,
             ld_w1=ld_u, ld_dy=lds[0], ld_pre0=lds[1], ld_pre1=lds[2], dtype=t, y_dtype=t, act=_GLU[act_func])  # fmt: skip
         _lib.check(lib.b200moe_gated_ffn_backward(ctypes.byref(args), s))
         return dx, dw_gate, dw_up
@@ -128,6 +141,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     ``out_dtype`` (x's type, or float32, which is then exact to float32 rounding).  ``act_func``: ``None``, ``"relu"``,
     ``"silu"`` or ``"gelu"`` (the error-function form).  With ``return_preact`` the result is ``(y, x weight^T + bias)``,
     the second in x's type, for :func:`linear_backward`."""
+    if torch.compiler.is_compiling():
+        _eager_stream_only(stream)
+        out = torch.ops.b200moe.linear(x, weight, bias, act_func, residual, out_dtype, return_preact)
+        return tuple(out) if return_preact else out[0]
     m, k = _check_x(x)
     if act_func not in _ACT:
         raise ValueError(f"act_func must be None, 'relu', 'silu' or 'gelu', got {act_func!r}")
@@ -164,10 +181,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 
 def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, preact: Optional[torch.Tensor] = None, act_func: Optional[str] = None,
-                    bias_grad: bool = False, stream=None) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:  # fmt: skip
+                    bias_grad: bool = False, input_grad: bool = True, weight_grad: bool = True, stream=None):  # fmt: skip
     """Backward pass of :func:`linear` from ``dy [tokens, n]`` (x's type or float32): returns ``(dx, dweight, dbias)``,
-    ``dbias`` float32 or ``None``.  ``preact`` is the saved pre-activation (needed with an activation).  The residual's
-    gradient is ``dy`` itself."""
+    ``dbias`` float32, with ``None`` for what is not asked for.  ``preact`` is the saved pre-activation (needed with an
+    activation).  The residual's gradient is ``dy`` itself (of a residual row that every token shares: its column sums)."""
     m, k = _check_x(x)
     if act_func not in _ACT:
         raise ValueError(f"act_func must be None, 'relu', 'silu' or 'gelu', got {act_func!r}")
@@ -185,16 +202,43 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
 
     def launch(s):
         lib = _lib.load()
-        dx, dw = x.new_empty((m, k)), x.new_empty((n, k))
+        dx, dw = x.new_empty((m, k)) if input_grad else None, x.new_empty((n, k)) if weight_grad else None
         db = x.new_empty((n,), dtype=torch.float32) if bias_grad else None
         need = lib.b200moe_dense_workspace_bytes(m, n, 0)
         work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
         args = _lib.DenseArgs(
-            x=x.data_ptr(), w0=weight.data_ptr(), dy=dy.data_ptr(), pre0=None if act_func is None else preact.data_ptr(), dx=dx.data_ptr(),
-            dw0=dw.data_ptr(), dbias=None if db is None else db.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x,
+            x=x.data_ptr(), w0=weight.data_ptr(), dy=dy.data_ptr(), pre0=None if act_func is None else preact.data_ptr(),
+            dx=_ptr(dx), dw0=_ptr(dw), dbias=_ptr(db), workspace=work.data_ptr(), workspace_bytes=need, m=m, n=n, k=k, ld_x=ld_x,
             ld_w0=ld_w, ld_dy=ld_dy, ld_pre0=ld_z, dtype=t, y_dtype=_lib.DTYPE_F32 if dy.dtype == torch.float32 else t, act=_ACT[act_func])  # fmt: skip
         _lib.check(lib.b200moe_linear_backward(ctypes.byref(args), s))
         return dx, dw, db
 
     return call_on(x.device, stream, launch)
+
+
+# ---------------------------------------------------------------------------------------------
+# torch custom ops
+# ---------------------------------------------------------------------------------------------
+@torch.library.custom_op("b200moe::gated_ffn", mutates_args=(), device_types="cuda")
+def _gated_ffn_op(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act_func: str, return_preact: bool) -> List[torch.Tensor]:
+    out = gated_ffn(x, w_gate, w_up, act_func, return_preact)
+    return list(out) if return_preact else [out]
+
+
+@_gated_ffn_op.register_fake
+def _(x, w_gate, w_up, act_func, return_preact):
+    return [x.new_empty((x.shape[0], w_gate.shape[0])) for _ in range(3 if return_preact else 1)]
+
+
+@torch.library.custom_op("b200moe::linear", mutates_args=(), device_types="cuda")
+def _linear_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], act_func: Optional[str], residual: Optional[torch.Tensor],
+               out_dtype: Optional[torch.dtype], return_preact: bool) -> List[torch.Tensor]:  # fmt: skip
+    out = linear(x, weight, bias, act_func, residual, out_dtype, return_preact)
+    return list(out) if return_preact else [out]
+
+
+@_linear_op.register_fake
+def _(x, weight, bias, act_func, residual, out_dtype, return_preact):
+    shape = (x.shape[0], weight.shape[0])
+    return [x.new_empty(shape, dtype=out_dtype or x.dtype)] + ([x.new_empty(shape)] if return_preact else [])

@@ -42,7 +42,12 @@ def router_topk(logits: torch.Tensor, topk: int, score_func: str = "softmax", no
     (decided in 64 bits), in falling order and ties to the lowest index.  A logit of -inf is never chosen; a slot left
     without an expert gets id -1, which :func:`route` skips, and weight 0.  NaN sorts above everything.  The weights are
     ``scale * score`` with ``score_func`` softmax over the row or sigmoid, with ``normalize`` divided by the sum of the
-    chosen scores; the bias decides the choice only.  ``E <= 1024``, ``topk <= 32``."""
+    chosen scores; the bias decides the choice only.  ``E <= 1024``, ``topk <= 32``.  While ``torch.compile`` traces, the call
+    goes through the custom op ``torch.ops.b200moe.router_topk``."""
+    if torch.compiler.is_compiling():
+        if stream is not None:
+            raise NotImplementedError("stream is an eager-only launch option")
+        return torch.ops.b200moe.router_topk(logits, topk, score_func, normalize, bias, scale)
     ld = _check_logits(logits, score_func)
     t, e = logits.shape
     if topk < 0:
@@ -282,3 +287,13 @@ def interleave_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor) -> torch.Tensor
     g = w_gate.reshape(*lead, i // 32, 1, 32, k)
     u = w_up.reshape(*lead, i // 32, 1, 32, k)
     return torch.cat([g, u], dim=-3).reshape(*lead, 2 * i, k)
+
+
+@torch.library.custom_op("b200moe::router_topk", mutates_args=(), device_types="cuda")
+def _router_topk_op(logits: torch.Tensor, topk: int, score_func: str, normalize: bool, bias: Optional[torch.Tensor], scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    return router_topk(logits, topk, score_func, normalize, bias, scale)
+
+
+@_router_topk_op.register_fake
+def _(logits, topk, score_func, normalize, bias, scale):
+    return logits.new_empty((logits.shape[0], topk), dtype=torch.float32), logits.new_empty((logits.shape[0], topk), dtype=torch.int32)

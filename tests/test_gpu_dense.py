@@ -210,6 +210,49 @@ def test_broadcast_residual_and_single_row_views():
     assert torch.equal(cf.linear(one, w), cf.linear(one.contiguous(), w))
 
 
+def test_gradients_that_are_not_asked_for():
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    for m, k, n in ((40, 64, 96), (1500, 512, 2048)):
+        x, w, u, dy = rows(gen, m, k, BF16), rows(gen, n, k, BF16), rows(gen, n, k, BF16), rows(gen, m, n, BF16)
+        full = cf.linear_backward(dy, x, w, bias_grad=True)
+        dx, none, _ = cf.linear_backward(dy, x, w, weight_grad=False)
+        none2, dw, none3 = cf.linear_backward(dy, x, w, input_grad=False)
+        assert none is none2 is none3 is None
+        assert rel_fro(dx, full[0].double()) <= eps(BF16) and rel_fro(dw, full[1].double()) <= eps(BF16)
+        only = cf.linear_backward(dy, x, w, bias_grad=True, input_grad=False, weight_grad=False)
+        assert only[0] is only[1] is None and torch.equal(only[2], full[2])
+        full = cf.gated_ffn_backward(dy, x, w, u, dy, dy)
+        dx, *none = cf.gated_ffn_backward(dy, x, w, u, dy, dy, weight_grad=False)
+        none4, *dws = cf.gated_ffn_backward(dy, x, w, u, dy, dy, input_grad=False)
+        assert none == [None, None] and none4 is None
+        for a, b in zip((dx, *dws), full):
+            assert rel_fro(a, b.double()) <= eps(BF16)
+
+
+def test_traced_calls_go_through_the_custom_ops():
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    x, wg, wu, wd, wr = rows(gen, 30, 64, BF16), rows(gen, 96, 64, BF16), rows(gen, 96, 64, BF16), rows(gen, 64, 96, BF16), rows(gen, 8, 64, BF16)
+
+    def layer(x):
+        w, ids = cf.router_topk(cf.linear(x, wr, out_dtype=torch.float32), 2)
+        h, gate, up = cf.gated_ffn(x, wg, wu, return_preact=True)
+        return (*cf.linear(h, wd, act_func="silu", residual=x, return_preact=True), gate, up, w, ids)
+
+    seen = []
+
+    def backend(graph, _):
+        seen.extend(str(n.target) for n in graph.graph.nodes if n.op == "call_function")
+        return graph.forward
+
+    got = torch.compile(layer, backend=backend, fullgraph=True)(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, layer(x)))
+    assert sum("b200moe" in t for t in seen) == 4
+
+
 def test_no_tokens():
     import cudnn_frontend_b200 as cf
 
