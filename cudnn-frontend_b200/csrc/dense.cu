@@ -1673,15 +1673,16 @@ static auto act_grad_of(bool f16, bool dy_f32) {
 // blocks along the rows of act_grad_kernel, and the rows of each
 static int grad_row_blocks(int64_t m, int64_t n, int64_t* rows_per_block) {
   const int64_t col_blocks = (n + GRAD_COLS - 1) / GRAD_COLS;
-  int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((m + 31) / 32, 148 * 8 / std::max<int64_t>(1, col_blocks)));
+  // (up to 128 rows one block: its sums are the result, and no second kernel is needed)
+  int64_t blocks = m <= 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>((m + 31) / 32, 148 * 8 / std::max<int64_t>(1, col_blocks)));
   *rows_per_block = (m + blocks - 1) / std::max<int64_t>(1, blocks);
   return (int)((m + *rows_per_block - 1) / *rows_per_block);
 }
 
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// dx = sum of dz_i w_i and dw_i = dz_i^T x: one launch of the pair kernel, or a launch of the tile kernel each where those are
-// estimated to take less time
+// dx = sum of dz_i w_i and dw_i = dz_i^T x: one launch of the pair kernel, or a launch each of the kernel that suits it where
+// those are estimated to take less time (a weight gradient of few tiles over many tokens shares its reduction in the tile kernel)
 static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, DeviceInfo* di, cudaStream_t stream) {
   PairParams q;
   pair_params(q, a);
@@ -1719,11 +1720,22 @@ static int dense_grad_products(const b200moe_dense_args* a, int count, const voi
     q.job[jobs++].ld_out = a->k;
   }
   if (jobs == 0) return B200MOE_OK;
-  double pair_ns = 0.0, tile_ns = 0.0;
-  pair_cols(pair, jobs, di, &pair_ns);
-  for (int i = 0; i < jobs; ++i) tile_ns += tile_shape(tile[i], di).time;
-  if (pair_ns < tile_ns) return dense_pair_gemm(pair, jobs, q, di, stream);
+  double joint = 0.0, apart = 0.0, pair_ns[2] = {0.0, 0.0}, tile_ns[2] = {0.0, 0.0};
+  pair_cols(pair, jobs, di, &joint);
   for (int i = 0; i < jobs; ++i) {
+    pair_cols(&pair[i], 1, di, &pair_ns[i]);
+    tile_ns[i] = tile_shape(tile[i], di).time;
+    apart += std::min(pair_ns[i], tile_ns[i]) - (i > 0 ? 2000.0 : 0.0);  // (the second launch starts while the first drains)
+  }
+  if (joint <= apart) return dense_pair_gemm(pair, jobs, q, di, stream);
+  for (int i = 0; i < jobs; ++i) {
+    if (pair_ns[i] <= tile_ns[i]) {
+      PairParams one = q;
+      one.job[0] = q.job[i];
+      const int rc = dense_pair_gemm(&pair[i], 1, one, di, stream);
+      if (rc) return rc;
+      continue;
+    }
     DenseParams p;
     dense_params(p, a);
     p.act = B200MOE_ACT_NONE;
@@ -1808,11 +1820,11 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
   const bool as_is = !has_act && !dy_f32 && aligned16(a->dy) && a->ld_dy % 8 == 0;
   const void* dz = as_is ? a->dy : a->workspace;
   if (!as_is || a->dbias) {
-    float* sums = a->dbias ? (float*)((uint8_t*)a->workspace + round256(a->m * ldo * 2)) : nullptr;
-    const int64_t dy_unit = dy_f32 ? 4 : 8;
-    const int vec = aligned16(a->dy) && a->ld_dy % dy_unit == 0 && (!has_act || (aligned16(a->pre0) && a->ld_pre0 % 8 == 0));
     int64_t rows_per_block;
     const int row_blocks = grad_row_blocks(a->m, a->n, &rows_per_block);
+    float* sums = !a->dbias ? nullptr : (row_blocks == 1 ? a->dbias : (float*)((uint8_t*)a->workspace + round256(a->m * ldo * 2)));
+    const int64_t dy_unit = dy_f32 ? 4 : 8;
+    const int vec = aligned16(a->dy) && a->ld_dy % dy_unit == 0 && (!has_act || (aligned16(a->pre0) && a->ld_pre0 % 8 == 0));
     const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)row_blocks);
     const bool f16 = a->dtype == B200MOE_DTYPE_F16;
     const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_of<B200MOE_ACT_RELU>(f16, dy_f32)
@@ -1822,7 +1834,7 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
     kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo, sums, vec,
                                    rows_per_block);
     B200_CUDA_CHECK(cudaGetLastError());
-    if (sums) {
+    if (sums && row_blocks > 1) {
       column_sum_kernel<<<(unsigned)((a->n + 255) / 256), 256, 0, stream>>>(sums, row_blocks, (int)a->n, a->dbias);
       B200_CUDA_CHECK(cudaGetLastError());
     }

@@ -42,6 +42,8 @@ def _check_x(x: torch.Tensor) -> Tuple[int, int]:
 
 def _pitch(name: str, t: torch.Tensor, shape, dtype, device) -> int:
     """Row pitch of a ``shape`` tensor with contiguous rows."""
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():  # (the usual case, in few steps)
+        return shape[1] if shape[0] > 1 else (shape[1] + 7) // 8 * 8
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != dtype:
@@ -54,6 +56,11 @@ def _pitch(name: str, t: torch.Tensor, shape, dtype, device) -> int:
         raise ValueError(f"{name} must have contiguous rows")
     # the pitch of a single row is free: the next multiple of 8
     return pitch if rows > 1 else (cols + 7) // 8 * 8
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of t's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _weight(name: str, w: torch.Tensor, k: int, x: torch.Tensor) -> int:
@@ -119,8 +126,8 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
 
     def launch(s):
         lib = _lib.load()
-        dx = x.new_empty((m, k)) if input_grad else None
-        dw_gate, dw_up = (x.new_empty((n, k)), x.new_empty((n, k))) if weight_grad else (None, None)
+        dx = _like(x) if input_grad else None
+        dw_gate, dw_up = (_like(w_gate), _like(w_up)) if weight_grad else (None, None)
         need = lib.b200moe_dense_workspace_bytes(m, n, 1)
         work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
@@ -172,7 +179,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
             args.residual = residual.data_ptr()
         z = None
         if return_preact:
-            z = x.new_empty((m, n))
+            z = torch.empty_like(y) if out_dtype is x.dtype else x.new_empty((m, n))
             args.pre0 = z.data_ptr()
         _lib.check(_lib.load().b200moe_linear(ctypes.byref(args), s))
         return (y, z) if return_preact else y
@@ -202,7 +209,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
 
     def launch(s):
         lib = _lib.load()
-        dx, dw = x.new_empty((m, k)) if input_grad else None, x.new_empty((n, k)) if weight_grad else None
+        dx, dw = _like(x) if input_grad else None, _like(weight) if weight_grad else None
         db = x.new_empty((n,), dtype=torch.float32) if bias_grad else None
         need = lib.b200moe_dense_workspace_bytes(m, n, 0)
         work = x.new_empty((need,), dtype=torch.uint8)

@@ -58,7 +58,7 @@ def call_on(device: torch.device, stream, fn):
     """``fn(raw stream handle)`` with ``device`` and ``stream`` current (``None`` = the device's current stream; a torch
     stream or a raw CUstream handle otherwise).  What ``fn`` allocates belongs to that stream, so neither outputs nor a
     workspace that is dropped on return can be handed to another stream's work while the kernels still run."""
-    if stream is None and device.index == torch.cuda.current_device():
+    if stream is None and device.index == torch._C._cuda_getDevice():
         return fn(torch._C._cuda_getCurrentRawStream(device.index))  # (the public way builds a Stream object: 3 us)
     with torch.cuda.device(device):
         if stream is None:
