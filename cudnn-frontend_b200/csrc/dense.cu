@@ -132,8 +132,8 @@ __device__ __forceinline__ void reg_fence16(float* v) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
                  "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t cluster_addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // Programmatic dependent launch: a kernel launched with the attribute may start while its predecessor on the stream
@@ -554,10 +554,11 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
 
   const int split = p.split;
   if (kGlu || split > 1) {
-    // partial sums meet in shared memory: [rank][column of the owner's slice][row].  With one CTA that is the ring, which the
-    // products have left; with several a region of its own, since another CTA's products may still read its ring, or,
-    // where that would leave too few stages, the ring once all of the cluster's products are done.
-    const int slice = (valid + split - 1) / split;  // columns that one CTA of the cluster finishes
+    // partial sums meet in shared memory, four columns of a row side by side: [rank][4 columns of the owner's slice][row][4].
+    // With one CTA that is the ring, which the products have left; with several a region of its own, since another CTA's
+    // products may still read its ring, or, where that would leave too few stages, the ring once all of the cluster's
+    // products are done.
+    const int slice4 = ((valid + split - 1) / split + 3) / 4;  // groups of 4 columns that one CTA of the cluster finishes
     const uint32_t region = ring + p.reduce_offset;
     if (split > 1) {
       __syncwarp();
@@ -569,26 +570,17 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
     }
     if (finisher && ok) {
       each_chunk([&](int c0, const float* v) {
-        const int count = min(16, valid - c0);
-        if (split == 1) {
-          const uint32_t at = region + (uint32_t)((c0 * 128 + r_in_tile) * 4);
+        const uint32_t base = region + (uint32_t)((rank * slice4 * 128 + r_in_tile) * 16);
+        int owner = (c0 / 4) / slice4, at = c0 / 4 - owner * slice4;
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (j < count) st_shared_f32(at + j * 512, v[j]);
-        } else {
-          int owner = c0 / slice, left = slice - (c0 - owner * slice);
-          const uint32_t base = region + (uint32_t)((rank * slice * 128 + r_in_tile) * 4);
-          uint32_t at = map_to_cta(base, (uint32_t)owner) + (uint32_t)((slice - left) * 512);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j < count) {
-              st_cluster_f32(at, v[j]);
-              at += 512;
-              if (--left == 0) {
-                left = slice;
-                ++owner;
-                at = map_to_cta(base, (uint32_t)min(owner, split - 1));
-              }
+        for (int j = 0; j < 16; j += 4) {
+          if (c0 + j < valid) {
+            const float4 w = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            if (split == 1) st_shared_f32x4(base + (uint32_t)((c0 + j) * 512), w);
+            else st_cluster_f32x4(map_to_cta(base, (uint32_t)owner) + (uint32_t)(at * 2048), w);
+            if (++at == slice4) {
+              at = 0;
+              ++owner;
             }
           }
         }
@@ -602,37 +594,32 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
       __syncthreads();
     }
     if (finisher) {
-      constexpr int kGroups = 256 / kTileRows;  // columns in flight
-      constexpr int kN = 8;
+      constexpr int kGroups = 256 / kTileRows;  // groups of columns in flight
       const int t = (int)threadIdx.x - 64;
       const int r = t % kTileRows, row = row0 + r;
-      const int c_begin = rank * slice, c_end = min(valid, c_begin + slice);
       if (row < p.rows) {
-        const float* part = reinterpret_cast<const float*>(smem + p.reduce_offset) + r;
+        const float4* part = reinterpret_cast<const float4*>(smem + p.reduce_offset) + r;
         const float bias = bias_at(row);
-        for (int c = c_begin + t / kTileRows; c < c_end; c += kGroups * kN) {
-          const int count = (c_end - c + kGroups - 1) / kGroups;
-          float v[kN], u[kN];
-          uint16_t raw[kN];
-          if constexpr (kTrans) fetch(std::integral_constant<int, kN>(), row, c, kGroups, count, raw);
-#pragma unroll
-          for (int j = 0; j < kN; ++j) v[j] = u[j] = 0.0f;
+        for (int g = t / kTileRows; g < slice4; g += kGroups) {
+          const int c = (rank * slice4 + g) * 4, count = min(4, valid - c);
+          if (count <= 0) break;
+          uint16_t raw[4];
+          if constexpr (kTrans) fetch(std::integral_constant<int, 4>(), row, c, 1, count, raw);
+          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           for (int q = 0; q < split; ++q) {
-            const float* src = part + (q * slice + c - c_begin) * 128;
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              if (j < count) {
-                v[j] += src[j * kGroups * 128];
-                if (kGlu) u[j] += src[j * kGroups * 128 + 64];
-              }
+            const float4 w = part[(q * slice4 + g) * 128];
+            v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+            if constexpr (kGlu) {
+              const float4 x = part[(q * slice4 + g) * 128 + 64];
+              u[0] += x.x, u[1] += x.y, u[2] += x.z, u[3] += x.w;
             }
           }
           if constexpr (kTrans) {
-            finish(std::integral_constant<int, kN>(), row, c, kGroups, count, bias, v, u, raw);
+            finish(std::integral_constant<int, 4>(), row, c, 1, count, bias, v, u, raw);
           } else {
 #pragma unroll
-            for (int j = 0; j < kN; ++j)
-              if (j < count) store16(p.out[which], (int64_t)row * p.ld_out + col0 + c + j * kGroups, v[j], f16);
+            for (int j = 0; j < 4; ++j)
+              if (j < count) store16(p.out[which], (int64_t)row * p.ld_out + col0 + c + j, v[j], f16);
           }
         }
       }
@@ -1384,7 +1371,8 @@ static int dense_gemm(const DenseGemm& g, DenseParams& p, DeviceInfo* di, cudaSt
   p.col_tiles = (int)((g.cols + C - 1) / C);
   const int64_t tiles = shape.tiles;
   p.stage_bytes = DENSE_A_BYTES + C * 128;
-  const int reduce_bytes = p.split > 1 ? (C + p.split - 1) * 512 : 0;
+  // (a slice of columns per CTA, rounded up to 4)
+  const int reduce_bytes = p.split > 1 ? p.split * (((C + p.split - 1) / p.split + 3) / 4 * 4) * 512 : 0;
   // (the loads of a CTA come after about 1.4 us at 80 GB/s and SM: 110 KB in flight, so a CTA alone on its SM takes it all)
   p.smem_bytes = tiles * p.split <= cluster_slots(p.split, di) ? DENSE_SMEM_ALONE : DENSE_SMEM;
   p.reduce_in_ring = p.split > 1 && C == 128 && p.smem_bytes == DENSE_SMEM;

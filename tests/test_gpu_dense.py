@@ -463,3 +463,26 @@ def test_bounded_waits_report_and_recover(m, n, kernel):
     torch.cuda.synchronize()
     assert ops.device_status(clear=True) == 0
     assert torch.equal(y, want)
+
+
+def test_offsets_beyond_32_bits():
+    """Inputs and outputs of more than 2^32 bytes and 2^31 elements: their last rows against the same rows alone."""
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    m, k, n = 540_000, 4096, 16  # x: 2.2e9 elements
+    x = torch.empty((m, k), dtype=BF16, device="cuda").normal_(generator=gen)
+    w = rows(gen, n, k, BF16, scale=k**-0.5)
+    for kw in ({}, {"out_dtype": torch.float32}):
+        assert rel_fro(cf.linear(x, w, **kw)[-300:], x[-300:].double() @ w.double().t()) <= eps(BF16)
+    dy = rows(gen, m, n, BF16)
+    dx, dw, _ = cf.linear_backward(dy, x, w)
+    assert rel_fro(dx[-300:], dy[-300:].double() @ w.double()) <= eps(BF16)
+    want = sum(dy[i : i + 60_000].float().t() @ x[i : i + 60_000].float() for i in range(0, m, 60_000))
+    assert rel_fro(dw, want.double()) <= eps(BF16)
+    del x, dx
+    m, k, n = 60_000, 64, 40_000  # results: 2.4e9 elements
+    x, w = rows(gen, m, k, BF16), rows(gen, n, k, BF16, scale=k**-0.5)
+    g = x[-300:].double() @ w.double().t()
+    assert rel_fro(cf.linear(x, w)[-300:], g) <= eps(BF16)
+    assert rel_fro(cf.gated_ffn(x, w, w)[-300:], g * torch.sigmoid(g) * g) <= eps(BF16)
