@@ -60,6 +60,8 @@ def call_on(device: torch.device, stream, fn):
     workspace that is dropped on return can be handed to another stream's work while the kernels still run."""
     if stream is None and device.index == torch._C._cuda_getDevice():
         return fn(torch._C._cuda_getCurrentRawStream(device.index))  # (the public way builds a Stream object: 3 us)
+    if isinstance(stream, torch.cuda.Stream) and stream.device != device:
+        raise ValueError(f"stream belongs to {stream.device}, the tensors live on {device}")
     with torch.cuda.device(device):
         if stream is None:
             return fn(torch._C._cuda_getCurrentRawStream(device.index))
