@@ -16,6 +16,7 @@ DTYPE_BF16, DTYPE_E4M3, DTYPE_F16, DTYPE_F32, DTYPE_E5M2, DTYPE_E2M1 = 0, 1, 2, 
 ACT_SWIGLU, ACT_GEGLU, ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4, 5
 ABI_VERSION = 7  # b200moe_abi_version() of the header these declarations mirror
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+DENSE_WORKSPACE_F16 = 2
 FLAG_DISCRETE_COL_SFD = 1
 FLAG_TILE_SINGLE = 2
 FLAG_TILE_PAIR = 4

@@ -54,6 +54,7 @@ struct DenseParams {
   const void* bias;
   const void* residual;
   int64_t ld_out, ld_res, ld_pre[2];
+  const uint32_t* amax;      // the operands of a gradient were scaled by grad_scale of this: the result is scaled back
   int test_skip_b_loads;     // test hook: no load of operand B is issued, so every wait runs out
   uint64_t wait_limit_ns;
 };
@@ -152,6 +153,18 @@ __device__ __forceinline__ void store16(void* p, int64_t i, float v, bool f16) {
 __device__ __forceinline__ float2 unpack16x2(uint32_t w, bool f16) {
   return f16 ? __half22float2(*reinterpret_cast<__half2*>(&w)) : __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
 }
+
+// ---------------------------------------------------------------------------------------
+// Scale of an fp16 gradient operand (dz, or dg and du together): the power of two that brings its largest finite magnitude `amax`
+// (the bits of a float32, kept on the device) into [2^14, 2^15).  fp16 holds 2^-24 to 65504, a gradient from float32 values or from
+// products with `up` may lie anywhere; so scaled, values down to 2^-29 of the largest keep all their bits and none
+// overflows.  The sums of the products are taken back by the inverse, in float32: both factors are exact.  Finding amax takes a pass of its own
+// over what dz is formed from (backward pass of the gated block, 1531 x 7168, 2048: 157 -> 161 to 166 us).
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ int grad_exponent(uint32_t amax) { return amax ? min(14 - ((int)(amax >> 23) - 127), 126) : 0; }
+__device__ __forceinline__ float pow2_f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ float grad_scale(const uint32_t* amax) { return amax ? pow2_f(grad_exponent(*amax)) : 1.0f; }
+__device__ __forceinline__ float grad_unscale(const uint32_t* amax) { return amax ? pow2_f(-grad_exponent(*amax)) : 1.0f; }
 
 // ---------------------------------------------------------------------------------------
 // Activations.  sigmoid(v) = 1 / (1 + 2^(-v log2 e)) on the approximate exponential and reciprocal (about 2^-22
@@ -493,6 +506,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
   };
   // kTrans: kN values of feature `row` for the tokens col0 + c0 + j step, of which the first `count` exist; v = the accumulator
   // (GLU: the gate's), u = the up projection's.  Every choice is a branch around a whole loop.
+  const float unscale = !kGlu && finisher ? grad_unscale(p.amax) : 1.0f;
   // residual values (raw) of the same elements; their loads are issued by `fetch`, ahead of whatever v waits for
   auto fetch = [&](auto size, int row, int c0, int step, int count, uint16_t* raw) {
     constexpr int kN = decltype(size)::value;
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
       for (int j = 0; j < kN; ++j) v[j] = glu_f(v[j], u[j], p.act);
     } else {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) v[j] += bias;
+      for (int j = 0; j < kN; ++j) v[j] = fmaf(v[j], unscale, bias);
       if (p.pre[0]) put(p.pre[0], p.ld_pre[0], v);
       act_values<kN>(v, p.act);
       if (p.residual) {
@@ -619,7 +633,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (j < count) store16(p.out[which], (int64_t)row * p.ld_out + col0 + c + j, v[j], f16);
+              if (j < count) store16(p.out[which], (int64_t)row * p.ld_out + col0 + c + j, v[j] * unscale, f16);
           }
         }
       }
@@ -652,14 +666,14 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         if (p.vec_store && c0 + 16 <= valid) {
           uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = pack16x2_from_float(v[2 * j], v[2 * j + 1], f16);
+          for (int j = 0; j < 8; ++j) w[j] = pack16x2_from_float(v[2 * j] * unscale, v[2 * j + 1] * unscale, f16);
           uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out[which]) + o);
           d[0] = make_uint4(w[0], w[1], w[2], w[3]);
           d[1] = make_uint4(w[4], w[5], w[6], w[7]);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c0 + j < valid) store16(p.out[which], o + j, v[j], f16);
+            if (c0 + j < valid) store16(p.out[which], o + j, v[j] * unscale, f16);
         }
       }
     });
@@ -725,6 +739,7 @@ struct PairParams {
   const void* residual;
   int64_t ld_res;
   int vec_res;                // residual rows may be read 16 bytes at a time
+  const uint32_t* amax;       // as in DenseParams
   int test_skip_b_loads;      // test hook, as in DenseParams
   uint64_t wait_limit_ns;
 };
@@ -1012,6 +1027,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     // ---- epilogue ---------------------------------------------------------------------------------------
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const bool f16 = p.f16 != 0;
+    const float unscale = kEpi == DENSE_STORE ? grad_unscale(p.amax) : 1.0f;
     BlockWriter writer = {ring + PAIR_STAGING + (uint32_t)((warp - 2) * 2 * PAIR_BOX), 0, lane, f16};
     PairTile t;
     for (int i = 0; pair_tile(p, pair, pairs, i, t); ++i) {
@@ -1060,6 +1076,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           if (p.pre[0]) writer.write(v, &maps.pre[0], p.pre[0], p.ld_pre[0], tma, row0, rows, col, cols);
           act_values<32>(v, p.act);
           if (p.residual) writer.add(v, p.residual, p.ld_res, p.vec_res != 0, row0, rows, col, cols);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) v[q] *= unscale;
         }
         writer.write(v, &maps.out[t.job][t.which], j.out[t.which], j.ld_out, tma, row0, rows, col, cols);
       }
@@ -1139,16 +1158,41 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
                     pack16x2_from_float(v[6], v[7], kF16));
 }
 
-// dg, du [m, ldo] from dh, gate, up [m, n]: 10 bytes per value, bound by HBM (4096 x 14336: 587 MB)
-template <int kAct, bool kF16>
+// The largest finite magnitude of a block's values goes to *amax (zero before): its bits order like the values, and a maximum does not
+// depend on the order.
+__device__ __forceinline__ void find_max8(const float* v, uint32_t& top) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
+    if (b < 0x7f800000u) top = max(top, b);
+  }
+}
+__device__ __forceinline__ void publish_max(uint32_t top, uint32_t* amax) {
+  __shared__ uint32_t s_top[8];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = __reduce_max_sync(0xffffffffu, threadIdx.x < 8 ? s_top[threadIdx.x] : 0u);
+    if (threadIdx.x == 0 && top) atomicMax(amax, top);
+  }
+}
+
+// dg, du [m, ldo] from dh, gate, up [m, n]: 10 bytes per value, bound by HBM (4096 x 14336: 587 MB).
+// They are rounded to the operands' 16 bits, as the tensor cores take both operands in one type; the rounding of each is independent, so
+// the gradient products' error grows from one rounding's to two.  fp16 values are scaled (grad_scale); kFind: nothing is
+// written, only their largest magnitude is found, in a launch of its own before.
+template <int kAct, bool kF16, bool kFind>
 __global__ void __launch_bounds__(256)
     glu_grad_kernel(const void* __restrict__ dh, const void* __restrict__ gate, const void* __restrict__ up, int64_t m, int n, int64_t ld_dh,
-                    int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int vec) {
-  pdl_trigger();
+                    int64_t ld_gate, int64_t ld_up, void* __restrict__ dg, void* __restrict__ du, int64_t ldo, int vec, uint32_t* __restrict__ amax) {
+  if (!kFind) pdl_trigger();
   const int c = (int)blockIdx.x * GRAD_COLS + (threadIdx.x & 31) * 8;
-  if (c >= n) return;
+  if (!kFind && c >= n) return;
   const bool whole = vec && c + 8 <= n;
-  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < m; r += (int64_t)gridDim.y * 8) {
+  const float scale = kF16 && !kFind ? grad_scale(amax) : 1.0f;
+  uint32_t top = 0;
+  for (int64_t r = c < n ? (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5) : m; r < m; r += (int64_t)gridDim.y * 8) {
     const Raw8 rd = raw8<false>(dh, r * ld_dh + c, whole, n - c), rg = raw8<false>(gate, r * ld_gate + c, whole, n - c),
                ru = raw8<false>(up, r * ld_up + c, whole, n - c);
     float d[8], g[8], u[8];
@@ -1157,20 +1201,33 @@ __global__ void __launch_bounds__(256)
     values8<false, kF16>(ru, u);
 #pragma unroll
     for (int j = 0; j < 8; ++j) glu_grad_f(d[j], g[j], u[j], kAct, g[j], u[j]);
+    if constexpr (kFind) {
+      find_max8(g, top);
+      find_max8(u, top);
+      continue;
+    }
+    if constexpr (kF16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] *= scale, u[j] *= scale;
+    }
     // (the padding columns of the last 8 are written too: they are part of the padded row)
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = pack8<kF16>(g);
     *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = pack8<kF16>(u);
   }
+  if constexpr (kFind) publish_max(top, amax);
 }
 
 // dz [m, ldo] = dy act'(z) (dz == NULL: dy is used as it is), and the column sums of the unrounded dz over the block's
 // rows: sums [gridDim.y][n].  Every sum has a fixed order: a warp's rows, then the warps, then (next kernel) the blocks.
-template <int kAct, bool kF16, bool kDyF32>
+// Rounding, scale of fp16 values and kFind as in glu_grad_kernel.
+template <int kAct, bool kF16, bool kDyF32, bool kFind>
 __global__ void __launch_bounds__(256)
     act_grad_kernel(const void* __restrict__ dy, const void* __restrict__ z, int64_t m, int n, int64_t ld_dy, int64_t ld_z, void* __restrict__ dz,
-                    int64_t ldo, float* __restrict__ sums, int vec, int64_t rows_per_block) {
-  __shared__ float s_part[8][GRAD_COLS];
-  pdl_trigger();
+                    int64_t ldo, float* __restrict__ sums, int vec, int64_t rows_per_block, uint32_t* __restrict__ amax) {
+  __shared__ float s_part[kFind ? 1 : 8][GRAD_COLS];
+  if (!kFind) pdl_trigger();
+  const float scale = kF16 && !kFind ? grad_scale(amax) : 1.0f;
+  uint32_t top = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = (int)blockIdx.x * GRAD_COLS + lane * 8;
   float acc[8];
@@ -1200,13 +1257,23 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[j] *= act_grad_f(g[j], kAct);
         }
+        if constexpr (kFind) {
+          find_max8(d, top);
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] += d[j];
+        if constexpr (kF16) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[j] *= scale;
+        }
         if (dz) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = pack8<kF16>(d);
       }
     }
   }
-  if (sums) {
+  if constexpr (kFind) {
+    publish_max(top, amax);
+  } else if (sums) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) s_part[warp][lane * 8 + j] = acc[j];
     __syncthreads();
@@ -1653,16 +1720,20 @@ static int dense_forward(const char* op, const b200moe_dense_args* a, bool gated
 }
 
 template <int kAct>
-static auto act_grad_of(bool f16, bool dy_f32) {
-  return f16 ? (dy_f32 ? act_grad_kernel<kAct, true, true> : act_grad_kernel<kAct, true, false>)
-             : (dy_f32 ? act_grad_kernel<kAct, false, true> : act_grad_kernel<kAct, false, false>);
+static auto act_grad_of(bool f16, bool dy_f32, bool find) {
+  if (find) return dy_f32 ? act_grad_kernel<kAct, true, true, true> : act_grad_kernel<kAct, true, false, true>;
+  return f16 ? (dy_f32 ? act_grad_kernel<kAct, true, true, false> : act_grad_kernel<kAct, true, false, false>)
+             : (dy_f32 ? act_grad_kernel<kAct, false, true, false> : act_grad_kernel<kAct, false, false, false>);
 }
 
+// Blocks of a launch that walks its rows: eight to an SM of a whole chip.  (No device decides it: the workspace's size is asked for before
+// there is one, and the order of the column sums does not depend on the device either.)
+constexpr int GRAD_BLOCKS = 148 * 8;
 // blocks along the rows of act_grad_kernel, and the rows of each
 static int grad_row_blocks(int64_t m, int64_t n, int64_t* rows_per_block) {
   const int64_t col_blocks = (n + GRAD_COLS - 1) / GRAD_COLS;
   // (up to 128 rows one block: its sums are the result, and no second kernel is needed)
-  int64_t blocks = m <= 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>((m + 31) / 32, 148 * 8 / std::max<int64_t>(1, col_blocks)));
+  int64_t blocks = m <= 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>((m + 31) / 32, GRAD_BLOCKS / std::max<int64_t>(1, col_blocks)));
   *rows_per_block = (m + blocks - 1) / std::max<int64_t>(1, blocks);
   return (int)((m + *rows_per_block - 1) / *rows_per_block);
 }
@@ -1671,9 +1742,11 @@ static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // dx = sum of dz_i w_i and dw_i = dz_i^T x: one launch of the pair kernel, or a launch each of the kernel that suits it where
 // those are estimated to take less time (a weight gradient of few tiles over many tokens shares its reduction in the tile kernel)
-static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, DeviceInfo* di, cudaStream_t stream) {
+static int dense_grad_products(const b200moe_dense_args* a, int count, const void* const* dz, int64_t ld_dz, const uint32_t* amax, DeviceInfo* di,
+                               cudaStream_t stream) {
   PairParams q;
   pair_params(q, a);
+  q.amax = amax;
   DenseGemm pair[2], tile[2];
   int jobs = 0;
   if (a->dx) {
@@ -1726,6 +1799,7 @@ static int dense_grad_products(const b200moe_dense_args* a, int count, const voi
     }
     DenseParams p;
     dense_params(p, a);
+    p.amax = amax;
     p.act = B200MOE_ACT_NONE;
     p.out[0] = q.job[i].out[0];
     p.out[1] = q.job[i].out[1];
@@ -1745,12 +1819,17 @@ static int zero_outputs(const b200moe_dense_args* a, bool gated, cudaStream_t st
   return B200MOE_OK;
 }
 
-static int64_t dense_workspace(int64_t m, int64_t n, bool gated) {
+// dz (or dg and du), the partial column sums of the linear form, and in the last 256 bytes the largest magnitude of fp16 values
+constexpr int64_t AMAX_BYTES = 256;
+static int64_t dense_workspace(int64_t m, int64_t n, bool gated, bool f16) {
   const int64_t ldo = (n + 7) / 8 * 8;
   if (m <= 0) return 0;
-  if (gated) return 2 * round256(m * ldo * 2);
+  if (gated) return 2 * round256(m * ldo * 2) + (f16 ? AMAX_BYTES : 0);
   int64_t rows_per_block;
-  return round256(m * ldo * 2) + round256((int64_t)grad_row_blocks(m, n, &rows_per_block) * n * 4);
+  return round256(m * ldo * 2) + round256((int64_t)grad_row_blocks(m, n, &rows_per_block) * n * 4) + AMAX_BYTES;
+}
+static uint32_t* amax_word(const b200moe_dense_args* a, bool gated, bool f16) {
+  return reinterpret_cast<uint32_t*>((uint8_t*)a->workspace + dense_workspace(a->m, a->n, gated, f16) - AMAX_BYTES);
 }
 
 }  // namespace b200moe
@@ -1761,7 +1840,9 @@ extern "C" int b200moe_gated_ffn(const b200moe_dense_args* a, void* stream) { re
 
 extern "C" int b200moe_linear(const b200moe_dense_args* a, void* stream) { return dense_forward("linear", a, false, (cudaStream_t)stream); }
 
-extern "C" int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t gated) { return dense_workspace(m, n, gated != 0); }
+extern "C" int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t form) {
+  return dense_workspace(m, n, (form & 1) != 0, (form & B200MOE_DENSE_WORKSPACE_F16) != 0);
+}
 
 extern "C" int b200moe_gated_ffn_backward(const b200moe_dense_args* a, void* stream_v) {
   const char* op = "gated_ffn_backward";
@@ -1774,19 +1855,29 @@ extern "C" int b200moe_gated_ffn_backward(const b200moe_dense_args* a, void* str
   if (!a->dy || !a->pre0 || !a->pre1) return fail(B200MOE_E_NULL, "%s: dh, gate and up are required", op);
   if (a->ld_dy < a->n || a->ld_pre0 < a->n || a->ld_pre1 < a->n) return fail(B200MOE_E_SHAPE, "%s: a pitch is below n", op);
   const int64_t ldo = (a->n + 7) / 8 * 8;
-  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, true))
-    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, true));
+  const bool f16 = a->dtype == B200MOE_DTYPE_F16, geglu = a->act == B200MOE_ACT_GEGLU;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, true, f16))
+    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, true, f16));
   void* dg = a->workspace;
   void* du = (uint8_t*)a->workspace + round256(a->m * ldo * 2);
   const int vec = aligned16(a->dy) && aligned16(a->pre0) && aligned16(a->pre1) && a->ld_dy % 8 == 0 && a->ld_pre0 % 8 == 0 && a->ld_pre1 % 8 == 0;
-  const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)std::min<int64_t>((a->m + 7) / 8, 32768));
-  const bool f16 = a->dtype == B200MOE_DTYPE_F16, geglu = a->act == B200MOE_ACT_GEGLU;
-  const auto kern = geglu ? (f16 ? glu_grad_kernel<B200MOE_ACT_GEGLU, true> : glu_grad_kernel<B200MOE_ACT_GEGLU, false>)
-                          : (f16 ? glu_grad_kernel<B200MOE_ACT_SWIGLU, true> : glu_grad_kernel<B200MOE_ACT_SWIGLU, false>);
-  kern<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, dg, du, ldo, vec);
+  const unsigned col_blocks = (unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS);
+  const int64_t row_blocks = (a->m + 7) / 8;
+  uint32_t* amax = f16 ? amax_word(a, true, true) : nullptr;
+  if (f16) {
+    const dim3 grid(col_blocks, (unsigned)std::max<int64_t>(1, std::min<int64_t>(row_blocks, GRAD_BLOCKS / col_blocks)));
+    const auto find = geglu ? glu_grad_kernel<B200MOE_ACT_GEGLU, true, true> : glu_grad_kernel<B200MOE_ACT_SWIGLU, true, true>;
+    B200_CUDA_CHECK(cudaMemsetAsync(amax, 0, sizeof(uint32_t), stream));
+    find<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, nullptr, nullptr, ldo, vec, amax);
+    B200_CUDA_CHECK(cudaGetLastError());
+  }
+  const dim3 grid(col_blocks, (unsigned)std::min<int64_t>(row_blocks, 32768));
+  const auto kern = geglu ? (f16 ? glu_grad_kernel<B200MOE_ACT_GEGLU, true, false> : glu_grad_kernel<B200MOE_ACT_GEGLU, false, false>)
+                          : (f16 ? glu_grad_kernel<B200MOE_ACT_SWIGLU, true, false> : glu_grad_kernel<B200MOE_ACT_SWIGLU, false, false>);
+  kern<<<grid, 256, 0, stream>>>(a->dy, a->pre0, a->pre1, a->m, (int)a->n, a->ld_dy, a->ld_pre0, a->ld_pre1, dg, du, ldo, vec, amax);
   B200_CUDA_CHECK(cudaGetLastError());
   const void* dz[2] = {dg, du};
-  return dense_grad_products(a, 2, dz, ldo, di, stream);
+  return dense_grad_products(a, 2, dz, ldo, amax, di, stream);
 }
 
 extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream_v) {
@@ -1800,13 +1891,16 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
   const bool has_act = a->act != B200MOE_ACT_NONE;
   if (!a->dy || (has_act && !a->pre0)) return fail(B200MOE_E_NULL, "%s: dy, and with an activation the pre-activation, are required", op);
   if (a->ld_dy < a->n || (has_act && a->ld_pre0 < a->n)) return fail(B200MOE_E_SHAPE, "%s: a pitch is below n", op);
-  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, false))
-    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, false));
+  const bool f16 = a->dtype == B200MOE_DTYPE_F16;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dense_workspace(a->m, a->n, false, f16))
+    return fail(B200MOE_E_WORKSPACE, "%s: needs %lld bytes of 16-byte aligned workspace", op, (long long)dense_workspace(a->m, a->n, false, f16));
   const bool dy_f32 = a->y_dtype == B200MOE_DTYPE_F32;
   int64_t ldo = (a->n + 7) / 8 * 8;
   // without an activation the gradient products read dy itself, where TMA can
   const bool as_is = !has_act && !dy_f32 && aligned16(a->dy) && a->ld_dy % 8 == 0;
   const void* dz = as_is ? a->dy : a->workspace;
+  // (an fp16 dy that is only moved into padded rows keeps its values)
+  uint32_t* amax = f16 && (has_act || dy_f32) && (a->dx || a->dw0) ? amax_word(a, false, f16) : nullptr;
   if (!as_is || a->dbias) {
     int64_t rows_per_block;
     const int row_blocks = grad_row_blocks(a->m, a->n, &rows_per_block);
@@ -1814,19 +1908,25 @@ extern "C" int b200moe_linear_backward(const b200moe_dense_args* a, void* stream
     const int64_t dy_unit = dy_f32 ? 4 : 8;
     const int vec = aligned16(a->dy) && a->ld_dy % dy_unit == 0 && (!has_act || (aligned16(a->pre0) && a->ld_pre0 % 8 == 0));
     const dim3 grid((unsigned)((a->n + GRAD_COLS - 1) / GRAD_COLS), (unsigned)row_blocks);
-    const bool f16 = a->dtype == B200MOE_DTYPE_F16;
-    const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_of<B200MOE_ACT_RELU>(f16, dy_f32)
-                      : a->act == B200MOE_ACT_SILU ? act_grad_of<B200MOE_ACT_SILU>(f16, dy_f32)
-                      : a->act == B200MOE_ACT_GELU ? act_grad_of<B200MOE_ACT_GELU>(f16, dy_f32)
-                                                   : act_grad_of<B200MOE_ACT_NONE>(f16, dy_f32);
-    kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is ? nullptr : a->workspace, ldo, sums, vec,
-                                   rows_per_block);
-    B200_CUDA_CHECK(cudaGetLastError());
+    auto launch = [&](bool find) {
+      const auto kern = a->act == B200MOE_ACT_RELU   ? act_grad_of<B200MOE_ACT_RELU>(f16, dy_f32, find)
+                        : a->act == B200MOE_ACT_SILU ? act_grad_of<B200MOE_ACT_SILU>(f16, dy_f32, find)
+                        : a->act == B200MOE_ACT_GELU ? act_grad_of<B200MOE_ACT_GELU>(f16, dy_f32, find)
+                                                     : act_grad_of<B200MOE_ACT_NONE>(f16, dy_f32, find);
+      kern<<<grid, 256, 0, stream>>>(a->dy, has_act ? a->pre0 : nullptr, a->m, (int)a->n, a->ld_dy, a->ld_pre0, as_is || find ? nullptr : a->workspace, ldo,
+                                     find ? nullptr : sums, vec, rows_per_block, amax);
+      return cudaGetLastError();
+    };
+    if (amax) {
+      B200_CUDA_CHECK(cudaMemsetAsync(amax, 0, sizeof(uint32_t), stream));
+      B200_CUDA_CHECK(launch(true));
+    }
+    B200_CUDA_CHECK(launch(false));
     if (sums && row_blocks > 1) {
       column_sum_kernel<<<(unsigned)((a->n + 255) / 256), 256, 0, stream>>>(sums, row_blocks, (int)a->n, a->dbias);
       B200_CUDA_CHECK(cudaGetLastError());
     }
   }
   const void* dzs[2] = {dz, nullptr};
-  return dense_grad_products(a, 1, dzs, as_is ? a->ld_dy : ldo, di, stream);
+  return dense_grad_products(a, 1, dzs, as_is ? a->ld_dy : ldo, amax, di, stream);
 }

@@ -113,7 +113,8 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
                        act_func: str = "swiglu", input_grad: bool = True, weight_grad: bool = True, stream=None):  # fmt: skip
     """Backward pass of :func:`gated_ffn` from ``dh [tokens, n]`` and the saved ``gate`` and ``up``: returns
     ``(dx, dw_gate, dw_up)``, with ``None`` for what ``input_grad`` or ``weight_grad`` leaves out.  A value that GeGLU limits has
-    no gradient."""
+    no gradient.  The gradients of gate and up are rounded to x's type before the products; in fp16 they are scaled by a power of two
+    over the call, so they may lie outside its range (what is below 2^-29 of their largest loses bits)."""
     m, k = _check_x(x)
     if act_func not in _GLU:
         raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
@@ -128,7 +129,7 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
         lib = _lib.load()
         dx = _like(x) if input_grad else None
         dw_gate, dw_up = (_like(w_gate), _like(w_up)) if weight_grad else (None, None)
-        need = lib.b200moe_dense_workspace_bytes(m, n, 1)
+        need = lib.b200moe_dense_workspace_bytes(m, n, 1 | (_lib.DENSE_WORKSPACE_F16 if x.dtype == torch.float16 else 0))
         work = x.new_empty((need,), dtype=torch.uint8)
         t = _TYPES[x.dtype]
         args = _lib.DenseArgs(
@@ -191,7 +192,11 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
                     bias_grad: bool = False, input_grad: bool = True, weight_grad: bool = True, stream=None):  # fmt: skip
     """Backward pass of :func:`linear` from ``dy [tokens, n]`` (x's type or float32): returns ``(dx, dweight, dbias)``,
     ``dbias`` float32, with ``None`` for what is not asked for.  ``preact`` is the saved pre-activation (needed with an
-    activation).  The residual's gradient is ``dy`` itself (of a residual row that every token shares: its column sums)."""
+    activation).  The residual's gradient is ``dy`` itself (of a residual row that every token shares: its column sums).
+
+    ``dy act'(preact)`` is rounded to x's type before the products (``dbias`` is summed before that).  In fp16 it is scaled by a
+    power of two over the call, so a float32 ``dy`` may lie outside fp16's range; what is below 2^-29 of its largest value loses
+    bits."""
     m, k = _check_x(x)
     if act_func not in _ACT:
         raise ValueError(f"act_func must be None, 'relu', 'silu' or 'gelu', got {act_func!r}")

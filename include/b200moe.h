@@ -383,10 +383,16 @@ int b200moe_peer_free(void* ptr);
  * the pitch of a row in elements (dx, dw0, dw1 are dense).  x, w0 and w1 must start on 16-byte boundaries with pitches of a multiple
  * of 8, and k must be a multiple of 8; m and n may be anything, m == 0 included (the weights' gradients are then zero).
  * dtype: B200MOE_DTYPE_BF16 or _F16, of every 16-bit tensor.  y_dtype: dtype, or (linear) B200MOE_DTYPE_F32, of y and
- * dy.  bias_dtype: dtype or F32.  The backward passes need b200moe_dense_workspace_bytes(m, n, gated) bytes, 16-byte
- * aligned; what it holds before and after a call means nothing.  Products are summed in float32; results do not depend on
- * timing.
+ * dy.  bias_dtype: dtype or F32.  The backward passes need b200moe_dense_workspace_bytes(m, n, form) bytes, 16-byte
+ * aligned; what it holds before and after a call means nothing.  form: 1 for the gated block, 0 for the linear form, plus
+ * B200MOE_DENSE_WORKSPACE_F16 where dtype is F16 (the gated block then needs 256 bytes more).  Products are summed in float32;
+ * results do not depend on timing.
+ *
+ * dz (dg and du) is rounded to dtype before the products, so dx and the weights' gradients carry two roundings; dbias is
+ * summed before.  In fp16 it is scaled by a power of two that brings its largest finite value into [2^14, 2^15), and the products
+ * are scaled back: it may lie outside fp16's range, and values down to 2^-29 of the largest keep all their bits.
  */
+#define B200MOE_DENSE_WORKSPACE_F16 2
 typedef struct b200moe_dense_args {
   const void* x;
   const void* w0;
@@ -425,7 +431,7 @@ int b200moe_gated_ffn(const b200moe_dense_args* args, void* stream);
 int b200moe_gated_ffn_backward(const b200moe_dense_args* args, void* stream);
 int b200moe_linear(const b200moe_dense_args* args, void* stream);
 int b200moe_linear_backward(const b200moe_dense_args* args, void* stream);
-int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t gated);
+int64_t b200moe_dense_workspace_bytes(int64_t m, int64_t n, int32_t form);
 
 /*
  * The gate in front of the experts (no reference counterpart; the ids go to b200moe_route, the weights to the GEMMs' prob).

@@ -70,6 +70,13 @@ def test_workspace_of_the_backward_passes():
     assert need(1 << 20, 1 << 14, 1) == 2 * (1 << 35)  # beyond 32 bits
 
 
+def test_workspace_holds_the_scale_of_float16_gradients():
+    need = _lib.load().b200moe_dense_workspace_bytes
+    assert need(3, 100, 1 | _lib.DENSE_WORKSPACE_F16) == 2 * 768 + 256
+    assert need(3, 100, _lib.DENSE_WORKSPACE_F16) == need(3, 100, 0) >= 768 + 400 + 256
+    assert need(0, 100, 1 | _lib.DENSE_WORKSPACE_F16) == 0
+
+
 def test_cpu_tensors_and_unknown_names_are_refused():
     x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((24, 64), dtype=torch.bfloat16)
     for call in (

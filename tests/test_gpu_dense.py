@@ -486,3 +486,122 @@ def test_offsets_beyond_32_bits():
     g = x[-300:].double() @ w.double().t()
     assert rel_fro(cf.linear(x, w)[-300:], g) <= eps(BF16)
     assert rel_fro(cf.gated_ffn(x, w, w)[-300:], g * torch.sigmoid(g) * g) <= eps(BF16)
+
+
+def scaled_operand_tol(a):
+    """What rounding dz (dg, du) to fp16 may cost beyond half a step of each value.  The call scales them by a power of two so that
+    the largest lies in [2^14, 2^15); the smallest step of fp16, 2^-24, is then at most 2^-24 2^-14 of the largest, and a rounding
+    half of that."""
+    return 2.0**-39 * a.abs().max()
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 8), (3, 64, 40), (65, 192, 300), (700, 512, 1024), (2049, 264, 1290), (1024, 2048, 256)])
+@pytest.mark.parametrize("act,dy_f32", [(None, True), ("silu", True), ("gelu", False), ("relu", True)])
+@pytest.mark.parametrize("size", [1e-7, 1.0, 1e5])
+def test_float16_gradients_keep_their_range(m, k, n, act, dy_f32, size):
+    """dz far below or above what fp16 holds, with gradients that it does hold: inputs and weights are large where dy is small
+    (float32 values of 1e-7, far below fp16's normal numbers) and small where it is large."""
+    import cudnn_frontend_b200 as cf
+
+    if not dy_f32:
+        size = min(size, 2e4)  # (3 standard deviations below 65504; times |act'| <= 1.13 it may leave the range)
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n)
+    other = min(64.0, 3000.0 / size / (m + n) ** 0.5)  # gradients of a few thousand at most: no sum leaves fp16's range
+    x, w = rows(gen, m, k, FP16, 8, other), rows(gen, n, k, FP16, 0, other)
+    dy = rows(gen, m, n, torch.float32 if dy_f32 else FP16, 8, size)
+    if not dy_f32:
+        dy.clamp_(-65504, 65504)
+    z = rows(gen, m, n, FP16, 0, 2.0) if act else None
+    dx, dw, db = cf.linear_backward(dy, x, w, preact=z, act_func=act, bias_grad=True)
+    dz = dy.double()
+    if act:
+        z64 = z.double().requires_grad_()
+        (dz,) = torch.autograd.grad(act64(z64, act), z64, dz)
+    x, w = x.double(), w.double()
+    e, tiny = eps(FP16) / 2, torch.finfo(FP16).tiny * eps(FP16)
+    near = 2.0**-18 * (dy.double().abs() if act else torch.zeros_like(dz))
+    step = scaled_operand_tol(dz)
+    for name, got, a, near_a, b, red in (("dx", dx, dz, near, w, n), ("dw", dw, dz.t(), near.t(), x, m)):
+        want, s = a @ b, a.abs() @ b.abs()
+        off = s * (e + trunc(red)) + (near_a + step) @ b.abs()
+        within(got, want, e * (want.abs() + off) + off + tiny, name)
+    within(db, dz.sum(0), dz.abs().sum(0) * (m + 8) * 2.0**-24 + near.sum(0) + 1e-30, "dbias")
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 8), (3, 64, 40), (65, 192, 300), (700, 512, 1024), (2049, 264, 1290), (128, 2048, 512)])
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+@pytest.mark.parametrize("dh_size,up_size", [(1e4, 30.0), (1e-4, 1e-3), (1.0, 1.0)])
+def test_float16_gated_gradients_keep_their_range(m, k, n, act, dh_size, up_size):
+    """dg = dh up act'(gate) beyond 65504, or far below fp16's normal numbers, with gradients that fp16 holds."""
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n)
+    other = min(64.0, 1500.0 / (dh_size * max(up_size, 4.0)) / (m + n) ** 0.5)
+    x, wg, wu = rows(gen, m, k, FP16, 8, other), rows(gen, n, k, FP16, 0, other), rows(gen, n, k, FP16, 8, other)
+    dh, gate, up = rows(gen, m, n, FP16, 0, dh_size), rows(gen, m, n, FP16, 8, 4.0), rows(gen, m, n, FP16, 0, up_size)
+    dx, dwg, dwu = cf.gated_ffn_backward(dh, x, wg, wu, gate, up, act_func=act)
+    g, u = gate.double().requires_grad_(), up.double().requires_grad_()
+    dg, du = torch.autograd.grad(glu64(g, u, act), (g, u), dh.double())
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    e, tiny = eps(FP16) / 2, torch.finfo(FP16).tiny * eps(FP16)
+    step = max(scaled_operand_tol(dg), scaled_operand_tol(du))
+    # act'(gate) = s (1 + g (1 - s)) may cancel: an absolute error of 2^-18 of its terms, which stay below 1.2 for the values it has
+    # (|dh| (|up| + 1) for the gate, |dh gate| for up)
+    near_g, near_u = 2.0**-18 * dh.double().abs() * (u.detach().abs() + 1), 2.0**-18 * (dh.double() * g.detach()).abs()
+    for name, got, pairs, red in (
+        ("dx", dx, ((dg, near_g, wg), (du, near_u, wu)), 2 * n), ("dw_gate", dwg, ((dg.t(), near_g.t(), x),), m), ("dw_up", dwu, ((du.t(), near_u.t(), x),), m)):  # fmt: skip
+        want, s = sum(a @ b for a, _, b in pairs), sum(a.abs() @ b.abs() for a, _, b in pairs)
+        off = s * (e + trunc(red)) + sum((near + step) @ b.abs() for _, near, b in pairs)
+        within(got, want, e * (want.abs() + off) + off + tiny, name)
+
+
+def test_float16_gradients_with_infinities_and_zeros():
+    """An infinite or NaN value reaches its own row of dx and its own row of dw only, and does not decide the scale of the others; a
+    gradient of nothing but zeros gives zeros."""
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    for m, k, n in ((20, 64, 40), (1500, 512, 2048)):
+        x, w = rows(gen, m, k, FP16, 0, 64.0), rows(gen, n, k, FP16, 0, 64.0)
+        dy = rows(gen, m, n, torch.float32, 0, 1e-7)
+        clean = cf.linear_backward(dy, x, w)
+        bad = dy.clone()
+        bad[3, 7], bad[4, 8] = float("nan"), float("inf")
+        dx, dw, _ = cf.linear_backward(bad, x, w)
+        rest = [i for i in range(m) if i not in (3, 4)]
+        cols = [i for i in range(n) if i not in (7, 8)]
+        assert rel_fro(dx[rest], clean[0][rest].double()) <= eps(FP16) and torch.isnan(dx[3]).all() and not torch.isfinite(dx[4]).any()
+        assert torch.isnan(dw[7]).all() and not torch.isfinite(dw[8]).any()
+        # (dw's other rows read dz's rows 3 and 4 as well, where their values are finite: 2 of m terms)
+        assert rel_fro(dw[cols], clean[1][cols].double()) <= eps(FP16)
+        zero = cf.linear_backward(torch.zeros_like(dy), x, w, bias_grad=True)
+        assert not any(t.any() for t in zero)
+        h = torch.zeros((m, n), dtype=FP16, device="cuda")
+        assert not any(t.any() for t in cf.gated_ffn_backward(h, x, w, w, h, h))
+
+
+def test_captured_float16_gradients_follow_new_magnitudes():
+    """The scale of an fp16 call is found by every replay anew."""
+    import cudnn_frontend_b200 as cf
+
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    m, k, n = 130, 256, 384
+    x, w, u = rows(gen, m, k, FP16, 0, 30.0), rows(gen, n, k, FP16, 0, 30.0), rows(gen, n, k, FP16, 0, 30.0)
+    z = rows(gen, m, n, FP16, 0, 2.0)
+    dy, dh = torch.zeros((m, n), device="cuda"), torch.zeros((m, n), dtype=FP16, device="cuda")
+
+    def step():
+        return (*cf.linear_backward(dy, x, w, preact=z, act_func="silu", bias_grad=True), *cf.gated_ffn_backward(dh, x, w, u, z, z))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for size in (1e-6, 1.0, 1e-9, 0.0, 1e-3):
+        dy.copy_(size * torch.randn((m, n), device="cuda", generator=gen))
+        dh.copy_(dy)
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(out, want))
+        assert bool(want[1].any()) == (size > 0)
