@@ -157,7 +157,7 @@ __device__ __forceinline__ float2 unpack16x2(uint32_t w, bool f16) {
 // ---------------------------------------------------------------------------------------
 // Scale of an fp16 gradient operand (dz, or dg and du together): the power of two that brings its largest finite magnitude `amax`
 // (the bits of a float32, kept on the device) into [2^14, 2^15).  fp16 holds 2^-24 to 65504, a gradient from float32 values or from
-// products with `up` may lie anywhere; so scaled, values down to 2^-29 of the largest keep all their bits and none
+// products with `up` may lie anywhere; so scaled, values down to 2^-28 of the largest keep all their bits and none
 // overflows.  The sums of the products are taken back by the inverse, in float32: both factors are exact.  Finding amax takes a pass of its own
 // over what dz is formed from (backward pass of the gated block, 1531 x 7168, 2048: 157 -> 161 to 166 us).
 // ---------------------------------------------------------------------------------------
@@ -722,7 +722,7 @@ struct PairJob {
   int tile_cols;              // accumulator columns of a tile: 256 or 128
   int raster;                 // row tiles of a raster group: the group's rows of A stay in L2 while its columns pass
   uint32_t idesc;
-  int tma_store;              // the outputs (and pre-activations) have tensor maps: 16-byte aligned base and pitch
+  int tma_store;              // the outputs (and pre-activations) of every job have tensor maps: 16-byte aligned base and pitch
   void* out[2];
   int64_t ld_out;
 };
@@ -798,8 +798,8 @@ __device__ __forceinline__ void st_shared_u32x4(uint32_t addr, uint32_t a, uint3
 // One warp's block of 32 rows x 32 columns to 16-bit memory: lane = row, v[] = its columns.  Stored from registers, every
 // instruction would touch 32 lines (7000 cycles for a tile of 128 x 256, measured as 87 us for 896 tiles); so the block goes
 // through shared memory (two blocks in turn, 64-byte swizzle: 16-byte writes without bank conflicts) and leaves as one bulk
-// copy, or, where the output has no tensor map, row by row with neighbouring lanes on neighbouring columns.  A residual comes in
-// the same way.
+// copy, or, where an output has no tensor map, row by row with neighbouring lanes on neighbouring columns.  A residual comes in
+// the same way.  A launch keeps to one of the two forms: only the first waits for earlier copies that still read a block.
 struct BlockWriter {
   uint32_t staging;  // this warp's two blocks
   int turn;
@@ -1529,6 +1529,9 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
   memset(&maps, 0, sizeof(maps));
   p.jobs = jobs;
   const int tile_cols = pair_cols(g, jobs, di);
+  bool tma_store = true;
+  for (int i = 0; i < jobs; ++i) tma_store = tma_store && p.job[i].ld_out % 8 == 0 && aligned16(p.job[i].out[0]) && aligned16(p.job[i].out[1]);
+  for (int q = 0; q < 2; ++q) tma_store = tma_store && (!p.pre[q] || (aligned16(p.pre[q]) && p.ld_pre[q] % 8 == 0));
   for (int i = 0; i < jobs; ++i) {
     PairJob& j = p.job[i];
     j.rows = (int)g[i].rows;
@@ -1557,9 +1560,8 @@ static int dense_pair_gemm(const DenseGemm* g, int jobs, PairParams& p, DeviceIn
       int rc = dense_encode(&maps.job[i].b[q], g[i].b[q].base, g[i].b[q].outer, g[i].b[q].inner, g[i].b[q].ld, g[i].b_mn ? 64 : tile_cols / 2, p.f16);
       if (rc) return rc;
     }
-    j.tma_store = j.ld_out % 8 == 0 && aligned16(j.out[0]) && aligned16(j.out[1]);
-    for (int q = 0; q < 2; ++q) j.tma_store = j.tma_store && (!p.pre[q] || (aligned16(p.pre[q]) && p.ld_pre[q] % 8 == 0));
-    if (j.tma_store) {
+    j.tma_store = tma_store;
+    if (tma_store) {
       for (int q = 0; q < no; ++q) {
         int rc = dense_encode_block(&maps.out[i][q], j.out[q], j.rows, j.cols, j.ld_out, p.f16);
         if (rc) return rc;

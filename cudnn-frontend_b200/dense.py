@@ -114,7 +114,7 @@ def gated_ffn_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     """Backward pass of :func:`gated_ffn` from ``dh [tokens, n]`` and the saved ``gate`` and ``up``: returns
     ``(dx, dw_gate, dw_up)``, with ``None`` for what ``input_grad`` or ``weight_grad`` leaves out.  A value that GeGLU limits has
     no gradient.  The gradients of gate and up are rounded to x's type before the products; in fp16 they are scaled by a power of two
-    over the call, so they may lie outside its range (what is below 2^-29 of their largest loses bits)."""
+    over the call, so they may lie outside its range (what is below 2^-28 of their largest loses bits)."""
     m, k = _check_x(x)
     if act_func not in _GLU:
         raise ValueError(f"act_func must be 'swiglu' or 'geglu', got {act_func!r}")
@@ -195,7 +195,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     activation).  The residual's gradient is ``dy`` itself (of a residual row that every token shares: its column sums).
 
     ``dy act'(preact)`` is rounded to x's type before the products (``dbias`` is summed before that).  In fp16 it is scaled by a
-    power of two over the call, so a float32 ``dy`` may lie outside fp16's range; what is below 2^-29 of its largest value loses
+    power of two over the call, so a float32 ``dy`` may lie outside fp16's range; what is below 2^-28 of its largest value loses
     bits."""
     m, k = _check_x(x)
     if act_func not in _ACT:

@@ -390,7 +390,7 @@ int b200moe_peer_free(void* ptr);
  *
  * dz (dg and du) is rounded to dtype before the products, so dx and the weights' gradients carry two roundings; dbias is
  * summed before.  In fp16 it is scaled by a power of two that brings its largest finite value into [2^14, 2^15), and the products
- * are scaled back: it may lie outside fp16's range, and values down to 2^-29 of the largest keep all their bits.
+ * are scaled back: it may lie outside fp16's range, and values down to 2^-28 of the largest keep all their bits.
  */
 #define B200MOE_DENSE_WORKSPACE_F16 2
 typedef struct b200moe_dense_args {

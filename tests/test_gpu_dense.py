@@ -605,3 +605,33 @@ def test_captured_float16_gradients_follow_new_magnitudes():
         want = step()
         assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(out, want))
         assert bool(want[1].any()) == (size > 0)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,k,n", [(40, 64, 96), (2049, 264, 1290), (4096, 512, 2304)])
+def test_gradients_of_unlike_alignment(m, k, n, gated):
+    """dx and the weights' gradients need no alignment: where one of them has none, each equals what aligned memory gets.  (Both
+    products may share a launch, whose blocks leave through shared memory by bulk copies, or row by row.)"""
+    import ctypes
+
+    import cudnn_frontend_b200 as cf
+    from cudnn_frontend_b200 import _lib
+
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    x, w, u = rows(gen, m, k, BF16), rows(gen, n, k, BF16, scale=k**-0.5), rows(gen, n, k, BF16, scale=k**-0.5)
+    dy, gate, up = rows(gen, m, n, BF16, 6), rows(gen, m, n, BF16, 6), rows(gen, m, n, BF16, 6)
+    want = cf.gated_ffn_backward(dy, x, w, u, gate, up) if gated else cf.linear_backward(dy, x, w)[:2]
+    lib, act = _lib.load(), _lib.ACT_SWIGLU if gated else _lib.ACT_NONE
+    work = torch.empty((lib.b200moe_dense_workspace_bytes(m, n, int(gated)),), dtype=torch.uint8, device="cuda")
+    for odd in range(1, 1 << len(want)):  # which outputs start between two 16-byte boundaries
+        outs = [torch.full((t.numel() + 8,), 3.0, dtype=BF16, device="cuda") for t in want]
+        at = [3 * (odd >> i & 1) for i in range(len(want))]
+        args = dict(x=x.data_ptr(), w0=w.data_ptr(), dy=dy.data_ptr(), workspace=work.data_ptr(), workspace_bytes=work.numel(), m=m, n=n, k=k, ld_x=k, ld_w0=k,
+                    ld_dy=n + 6, act=act, **dict(zip(("dx", "dw0", "dw1"), (o.data_ptr() + 2 * a for o, a in zip(outs, at)))))  # fmt: skip
+        if gated:
+            args |= dict(w1=u.data_ptr(), ld_w1=k, pre0=gate.data_ptr(), pre1=up.data_ptr(), ld_pre0=n + 6, ld_pre1=n + 6)
+        fn = lib.b200moe_gated_ffn_backward if gated else lib.b200moe_linear_backward
+        _lib.check(fn(ctypes.byref(_lib.DenseArgs(**args)), torch.cuda.current_stream().cuda_stream))
+        for o, a, t in zip(outs, at, want):
+            assert torch.equal(o[a : a + t.numel()].view(t.shape), t)
+            assert (o[:a] == 3).all() and (o[a + t.numel() :] == 3).all()
