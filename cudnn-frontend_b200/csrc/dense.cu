@@ -22,7 +22,7 @@ constexpr int DENSE_BK = 64;                          // elements of the reducti
 constexpr int DENSE_SLAB = DENSE_BK * 128;            // an MN-major slab: 64 columns x 64 rows of the reduction
 constexpr int DENSE_A_BYTES = 128 * DENSE_BK * 2;     // 128 operand rows
 constexpr int DENSE_MAX_SPLIT = 8;                    // portable cluster size
-constexpr int ST_DENSE_EMPTY = 401, ST_DENSE_FULL = 402, ST_DENSE_ACC = 403, ST_DENSE_DRAIN = 404;
+constexpr int ST_DENSE_EMPTY = 401, ST_DENSE_FULL = 402, ST_DENSE_ACC = 403;
 
 // epilogues
 constexpr int DENSE_GLU = 0;     // gate and up accumulators -> activation product
@@ -142,6 +142,20 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t cluster_addr, float4 v
 // memory is touched before the wait.  The trigger lets the successor start in the same way.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Where a wait gave up, a CTA may not end, nor free its TMEM, while its copies still write its shared memory or its products still
+// read it: after all warps have stopped issuing, they are waited for, whichever warp it was that gave up.  The limit is one for all waits
+// of a CTA from `t0` on; the abort flag, which is set by then, does not end them.
+__device__ __noinline__ void drain_wait(uint32_t bar, uint32_t parity, uint64_t t0, uint64_t limit_ns) {
+#pragma unroll 1
+  while (!mbar_try_wait_hint(bar, parity, kWaitHintNs) && global_timer_ns() - t0 <= limit_ns) {
+  }
+}
+// the copies of the last `issued` stages, the latest round of each stage
+__device__ __forceinline__ void drain_copies(uint32_t full_bar0, int issued, int stages, uint64_t limit_ns) {
+  const uint64_t t0 = global_timer_ns();
+  for (int i = max(0, issued - stages); i < issued; ++i) drain_wait(full_bar0 + 8u * (uint32_t)(i % stages), (uint32_t)(i / stages) & 1u, t0, limit_ns);
+}
 
 __device__ __forceinline__ float load16(const void* p, int64_t i, bool f16) {
   return f16 ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
@@ -292,9 +306,10 @@ template <bool kTrans, int kEpi, bool kSeg>
 __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t s_bars[2 * 16 + 4];
+  __shared__ uint64_t s_bars[2 * 16 + 5];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ int s_issued[2];  // stages whose copies each producer has issued
   constexpr bool kGlu = kEpi == DENSE_GLU;
   constexpr int kTileRows = kGlu ? 64 : 128;
   const uint32_t ring = smem_u32(smem);
@@ -304,6 +319,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
   auto empty_bar = [&](int s) { return bars + 8u * (16 + s); };
   auto acc_full_bar = [&](int b) { return bars + 8u * (32 + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (34 + b); };
+  const uint32_t drain_bar = bars + 8u * 36;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WaitCtx wc = {&s_abort, p.wait_limit_ns};
 
@@ -328,7 +344,8 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
       mbar_init(acc_full_bar(b), 1);
       mbar_init(acc_empty_bar(b), 8);
     }
-    s_abort = 0;
+    mbar_init(drain_bar, 1);
+    s_abort = s_issued[0] = s_issued[1] = 0;
     fence_mbar_init();
     prefetch_tensormap(&maps.a[0]);
     prefetch_tensormap(&maps.b[0]);
@@ -395,11 +412,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         parity ^= 1u;
       }
     }
-    if (issued < nk) {
-      // a wait gave up: the copies already issued still write this CTA's shared memory, so they are waited for
-      // (with a limit) before the CTA may end
-      for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full_bar(i % stages), (uint32_t)(i / stages) & 1u, wc, ST_DENSE_DRAIN);
-    }
+    if (lane == 0) s_issued[side_b] = issued;
     __syncwarp();
   } else if (warp == 1) {
     // ---- MMA issuer ---------------------------------------------------------------------
@@ -680,6 +693,14 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
   }
   tc_fence_before();
   __syncthreads();
+  if (*wc.abort_flag) {
+    if (warp == 0) drain_copies(full_bar(0), max(s_issued[0], s_issued[1]), stages, p.wait_limit_ns);
+    if (warp == 1) {
+      commit_if(elect_one(), drain_bar);  // (of all products that this lane has issued)
+      drain_wait(drain_bar, 0, global_timer_ns(), p.wait_limit_ns);
+    }
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, p.tmem_cols);
@@ -711,7 +732,7 @@ constexpr int PAIR_EPI_WARPS = 8;
 constexpr int PAIR_BOX = 32 * 32 * 2;  // a block of 32 rows x 32 columns of the output
 constexpr int PAIR_STAGING = PAIR_STAGES * PAIR_STAGE_BYTES;  // two blocks per epilogue warp
 constexpr int PAIR_SMEM = PAIR_STAGING + PAIR_EPI_WARPS * 2 * PAIR_BOX + 1024;
-constexpr int ST_PAIR_EMPTY = 411, ST_PAIR_FULL = 412, ST_PAIR_ACC_EMPTY = 413, ST_PAIR_ACC_FULL = 414, ST_PAIR_DRAIN = 415;
+constexpr int ST_PAIR_EMPTY = 411, ST_PAIR_FULL = 412, ST_PAIR_ACC_EMPTY = 413, ST_PAIR_ACC_FULL = 414;
 
 struct PairJob {
   int rows, cols;
@@ -895,15 +916,17 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t s_bars[2 * PAIR_STAGES + 4];
+  __shared__ uint64_t s_bars[2 * PAIR_STAGES + 5];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ int s_issued[4];  // first CTA's: stages whose copies each producer of the pair has issued
   const uint32_t ring = smem_u32(smem);
   const uint32_t bars = smem_u32(s_bars);
   auto full_bar = [&](int s) { return bars + 8u * s; };
   auto empty_bar = [&](int s) { return bars + 8u * (PAIR_STAGES + s); };
   auto acc_full_bar = [&](int b) { return bars + 8u * (2 * PAIR_STAGES + b); };
   auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * PAIR_STAGES + 2 + b); };
+  const uint32_t drain_bar = bars + 8u * (2 * PAIR_STAGES + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WaitCtx wc = {&s_abort, p.wait_limit_ns};
   const int rank = (int)cluster_ctarank();
@@ -918,6 +941,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       mbar_init(acc_full_bar(b), 1);
       mbar_init(acc_empty_bar(b), 2 * PAIR_EPI_WARPS);
     }
+    mbar_init(drain_bar, 1);
     s_abort = 0;
     fence_mbar_init();
     prefetch_tensormap(&maps.job[0].a[0]);
@@ -980,11 +1004,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && rank == 0) {
-      // a wait gave up: the copies of both CTAs are credited here; wait (with a limit) until they have landed.  The second
-      // CTA ends after the cluster barrier below, so its shared memory outlives them too.
-      for (int i = max(0, issued - PAIR_STAGES); i < issued; ++i) mbar_wait(full_bar(i % PAIR_STAGES), (uint32_t)(i / PAIR_STAGES) & 1u, wc, ST_PAIR_DRAIN);
-    }
+    if (lane == 0) st_shared_cluster(map_to_cta(smem_u32(&s_issued[rank * 2 + (side_b ? 1 : 0)]), 0), (uint32_t)issued);
     __syncwarp();
   } else if (warp == 1) {
     // ---- MMA issuer -------------------------------------------------------------------------------------
@@ -1088,8 +1108,21 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *wc.abort_flag) st_shared_cluster(map_to_cta(smem_u32(&s_abort), (uint32_t)(rank ^ 1)), 1u);
+  __syncwarp();
   cluster_arrive();  // the other CTA's arrivals and the issuer's products reach this CTA until both are here
   cluster_wait();
+  if (*wc.abort_flag) {
+    // (in both CTAs or in none: the copies of both are credited to the first, the products' end is told to both)
+    if (warp == 0 && rank == 0) drain_copies(full_bar(0), max(max(s_issued[0], s_issued[1]), max(s_issued[2], s_issued[3])), PAIR_STAGES, p.wait_limit_ns);
+    if (warp == 1) {
+      if (rank == 0) commit_pair_if(elect_one(), drain_bar);
+      drain_wait(drain_bar, 0, global_timer_ns(), p.wait_limit_ns);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem, 512);

@@ -635,3 +635,57 @@ def test_gradients_of_unlike_alignment(m, k, n, gated):
         for o, a, t in zip(outs, at, want):
             assert torch.equal(o[a : a + t.numel()].view(t.shape), t)
             assert (o[:a] == 3).all() and (o[a + t.numel() :] == 3).all()
+
+
+def dense_call(form, m, k, n, gen):
+    """A call of a C entry point on fresh inputs: (function, arguments, outputs, what the outputs have to be)."""
+    import cudnn_frontend_b200 as cf
+    from cudnn_frontend_b200 import _lib
+
+    lib = _lib.load()
+    x, w, u = rows(gen, m, k, BF16), rows(gen, n, k, BF16, scale=k**-0.5), rows(gen, n, k, BF16, scale=k**-0.5)
+    args = dict(x=x.data_ptr(), w0=w.data_ptr(), m=m, n=n, k=k, ld_x=k, ld_w0=k, act=_lib.ACT_NONE)
+    if form == "linear":
+        want = [cf.linear(x, w)]
+    elif form == "float32":
+        want, args = [cf.linear(x, w, out_dtype=torch.float32)], args | dict(y_dtype=_lib.DTYPE_F32)
+    elif form == "gated":
+        want, args = list(cf.gated_ffn(x, w, u, return_preact=True)), args | dict(w1=u.data_ptr(), ld_w1=k, act=_lib.ACT_SWIGLU)
+    else:
+        dy = rows(gen, m, n, BF16, 8)
+        want, work = list(cf.linear_backward(dy, x, w)[:2]), torch.empty((lib.b200moe_dense_workspace_bytes(m, n, 0),), dtype=torch.uint8, device="cuda")
+        args |= dict(dy=dy.data_ptr(), ld_dy=n + 8, workspace=work.data_ptr(), workspace_bytes=work.numel())
+        x = (x, dy, work)
+    outs = [torch.full_like(t, 3.0) for t in want]
+    names = ("dx", "dw0") if form == "backward" else ("y", "pre0", "pre1")
+    args |= dict(zip(names, (o.data_ptr() for o in outs)))
+    if form != "backward":
+        args |= dict(ld_y=n, ld_pre0=n, ld_pre1=n)
+    fn = {"gated": lib.b200moe_gated_ffn, "backward": lib.b200moe_linear_backward}.get(form, lib.b200moe_linear)
+    return fn, args, outs, want, (x, w, u)
+
+
+# one CTA to a tile and several, one stage of the reduction and many more than the ring holds, and the kernel of CTA pairs
+WAITS = [(5, 64, 200), (40, 512, 300), (300, 4096, 520), (3, 8192, 256), (2048, 256, 2048), (2304, 2048, 2048)]
+
+
+@pytest.mark.parametrize("form", ["linear", "float32", "gated", "backward"])
+@pytest.mark.parametrize("m,k,n", WAITS)
+def test_expired_waits_leave_nothing_in_flight(m, k, n, form):
+    """A launch whose operand B never arrives ends after its wait limit, whether its producers had more to issue or not, and what it had
+    in flight is no part of the launch behind it on the same stream."""
+    import ctypes
+
+    from cudnn_frontend_b200 import _lib, ops
+
+    gen = torch.Generator(device="cuda").manual_seed(24)
+    fn, args, outs, want, _ = dense_call(form, m, k, n, gen)
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) == 0
+    stream = torch.cuda.current_stream().cuda_stream
+    assert fn(ctypes.byref(_lib.DenseArgs(flags=_lib.FLAG_TEST_SKIP_B_LOADS, wait_limit_ms=20, **args)), stream) == 0
+    assert fn(ctypes.byref(_lib.DenseArgs(**args)), stream) == 0
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) in (401, 402, 403, 411, 412, 413, 414)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert ops.device_status(clear=True) == 0
