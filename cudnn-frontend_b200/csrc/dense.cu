@@ -613,14 +613,17 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
         }
       });
     }
+    // where a wait gave up, sums are missing: the CTAs of the cluster tell one another and store nothing
     __syncwarp();
     if (split > 1) {
+      if (lane < split && *wc.abort_flag) st_shared_cluster(map_to_cta(smem_u32(&s_abort), (uint32_t)lane), 1u);
+      __syncwarp();
       cluster_arrive();
       cluster_wait();
     } else {
       __syncthreads();
     }
-    if (finisher) {
+    if (finisher && !*wc.abort_flag) {
       constexpr int kGroups = 256 / kTileRows;  // groups of columns in flight
       const int t = (int)threadIdx.x - 64;
       const int r = t % kTileRows, row = row0 + r;

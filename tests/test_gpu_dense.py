@@ -689,3 +689,26 @@ def test_expired_waits_leave_nothing_in_flight(m, k, n, form):
     assert ops.device_status(clear=True) in (401, 402, 403, 411, 412, 413, 414)
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
     assert ops.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("form", ["linear", "float32", "gated", "backward"])
+@pytest.mark.parametrize("m,k,n", WAITS)
+def test_expired_waits_store_nothing(m, k, n, form):
+    """Where sums are missing, outputs stay as they were, also where CTAs exchange partial sums or gate and up meet in shared memory."""
+    import ctypes
+
+    from cudnn_frontend_b200 import _lib, ops
+
+    gen = torch.Generator(device="cuda").manual_seed(25)
+    fn, args, outs, want, _ = dense_call(form, m, k, n, gen)
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) == 0
+    stream = torch.cuda.current_stream().cuda_stream
+    assert fn(ctypes.byref(_lib.DenseArgs(flags=_lib.FLAG_TEST_SKIP_B_LOADS, wait_limit_ms=20, **args)), stream) == 0
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) in (401, 402, 403, 411, 412, 413, 414)
+    assert all((t == 3.0).all() for t in outs)
+    assert fn(ctypes.byref(_lib.DenseArgs(**args)), stream) == 0
+    torch.cuda.synchronize()
+    assert ops.device_status(clear=True) == 0
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
