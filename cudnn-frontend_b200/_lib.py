@@ -168,7 +168,9 @@ def load() -> ctypes.CDLL:
     if lib.b200moe_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{path} has ABI version {lib.b200moe_abi_version()}, this package needs {ABI_VERSION}: rebuild the library")
     for name, (restype, argtypes) in _SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:  # entry points are added within an ABI version
+            raise RuntimeError(f"{path} has no {name}: it is older than this package, rebuild the library")
         fn.restype = restype
         fn.argtypes = argtypes
     _lib = lib

@@ -94,3 +94,18 @@ def test_cpu_tensors_and_unknown_names_are_refused():
 def test_new_names_are_public():
     for name in ("gated_ffn", "gated_ffn_backward", "linear", "linear_backward", "router_topk", "router_topk_backward"):
         assert callable(getattr(cf, name)) and name in dir(cf)
+
+
+def test_an_older_library_of_the_same_version_asks_to_be_rebuilt(monkeypatch):
+    """Entry points were added within an ABI version: a library that lacks one is refused by name, before it is called."""
+
+    class Older:
+        def __init__(self, path):
+            for name in _lib.EXPORTED_SYMBOLS:
+                if "gated_ffn" not in name:
+                    setattr(self, name, lambda *args: _lib.ABI_VERSION)
+
+    monkeypatch.setattr(_lib, "_lib", None)
+    monkeypatch.setattr(_lib.ctypes, "CDLL", Older)
+    with pytest.raises(RuntimeError, match="b200moe_gated_ffn.*rebuild the library"):
+        _lib.load()
