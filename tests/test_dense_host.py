@@ -109,3 +109,14 @@ def test_an_older_library_of_the_same_version_asks_to_be_rebuilt(monkeypatch):
     monkeypatch.setattr(_lib.ctypes, "CDLL", Older)
     with pytest.raises(RuntimeError, match="b200moe_gated_ffn.*rebuild the library"):
         _lib.load()
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    from cudnn_frontend_b200 import ops
+
+    class Stream:
+        device = torch.device("cuda", 1)
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    with pytest.raises(ValueError, match="stream belongs to cuda:1, the tensors live on cuda:0"):
+        ops.call_on(torch.device("cuda", 0), Stream(), lambda s: s)
