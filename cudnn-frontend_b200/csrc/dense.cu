@@ -1428,9 +1428,28 @@ struct TileShape {
   int64_t tiles;
   double time;
 };
-// SMs that clusters of this size can occupy at once: a cluster lies within one of the chip's groups of SMs, whose sizes are no
-// multiple of 4 or 8 (of 148 SMs: 33 clusters of 4, 15 of 8)
-static int cluster_slots(int split, const DeviceInfo* di) { return split <= 2 ? di->sm_count / 2 * 2 : (split == 4 ? di->sm_count * 33 / 148 * 4 : di->sm_count * 15 / 148 * 8); }
+// SMs that clusters of this size can occupy at once with a CTA of the tile kernel to an SM: a cluster lies within one of the chip's groups
+// of SMs, whose sizes are no multiple of 4 or 8 and differ between parts (here, of 148 SMs: 33 clusters of 4, 15 of 8), so each device is
+// asked once.  0: clusters of this size do not run.
+static int cluster_slots(int split, const DeviceInfo* di) {
+  if (split <= 2) return std::max(2, di->sm_count / 2 * 2);
+  static std::atomic<int> known[64][2];
+  int dev = 0, clusters = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::atomic<int>& slots = known[dev & 63][split == 8];
+  if (slots.load(std::memory_order_relaxed) == 0) {
+    auto kern = dense_tile_kernel<true, DENSE_LINEAR, false>;
+    LaunchConfig c((unsigned)(split * di->sm_count), DENSE_THREADS, DENSE_SMEM_ALONE, split, nullptr);
+    c.cfg.numAttrs = 1;  // (the cluster's size alone)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DENSE_SMEM_ALONE) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kern, &c.cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      clusters = 0;
+    }
+    slots.store(clusters > 0 ? clusters * split : -1, std::memory_order_relaxed);
+  }
+  return std::max(0, slots.load(std::memory_order_relaxed));
+}
 static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
   const int64_t tile_rows = g.dual ? 64 : 128;
   const int64_t rows = (g.rows + tile_rows - 1) / tile_rows * (g.stacked ? 2 : 1);
@@ -1443,6 +1462,7 @@ static TileShape tile_shape(const DenseGemm& g, const DeviceInfo* di) {
     const double bytes = DENSE_A_BYTES + c * 128;
     for (int split = 1; split <= DENSE_MAX_SPLIT && split * 4 <= std::max<int64_t>(4, stages); split *= 2) {
       const int64_t ctas = tiles * split, slots = cluster_slots(split, di);
+      if (slots < split) continue;
       const int64_t per_sm = (ctas + slots - 1) / slots;
       const double together = per_sm > 1 ? 2.0 : 1.0, rounds = per_sm > 1 ? (double)((per_sm + 1) / 2) : 1.0;
       const double stage = std::max({190.0, together * bytes / 160.0, together * bytes * (double)std::min<int64_t>(ctas, di->sm_count) / 15800.0});
