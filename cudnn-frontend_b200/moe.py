@@ -18,7 +18,7 @@ _LOGIT_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, 
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
 
-def _check_logits(logits: torch.Tensor, score_func: str) -> int:
+def _check_logits(logits: torch.Tensor, score_func: str, topk: int) -> int:
     """Row pitch of the router's logits."""
     shape = logits.shape
     if len(shape) != 2 or not logits.is_cuda:
@@ -28,6 +28,8 @@ def _check_logits(logits: torch.Tensor, score_func: str) -> int:
     if score_func not in _SCORES:
         raise ValueError(f"score_func must be 'softmax' or 'sigmoid', got {score_func!r}")
     t, e = shape
+    if not 1 <= e <= 1024 or not 1 <= topk <= min(e, 32):  # (before anything is allocated, and before both become 32-bit numbers)
+        raise ValueError(f"experts must be 1 to 1024 and topk 1 to 32, at most the experts; got {e} experts and topk {topk}")
     pitch, step = logits.stride()
     if step != 1 and e > 1 and t > 0:
         raise ValueError("logits must have contiguous rows")
@@ -48,10 +50,8 @@ def router_topk(logits: torch.Tensor, topk: int, score_func: str = "softmax", no
         if stream is not None:
             raise NotImplementedError("stream is an eager-only launch option")
         return torch.ops.b200moe.router_topk(logits, topk, score_func, normalize, bias, scale)
-    ld = _check_logits(logits, score_func)
+    ld = _check_logits(logits, score_func, topk)
     t, e = logits.shape
-    if topk < 0:
-        raise ValueError(f"topk must be positive, got {topk}")
     if bias is not None and (tuple(bias.shape) != (e,) or bias.dtype != torch.float32 or bias.device != logits.device or (e > 1 and bias.stride(0) != 1)):
         raise ValueError(f"bias must be a contiguous float32 [{e}] tensor on {logits.device}")
 
@@ -72,7 +72,7 @@ def router_topk_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torc
     """Backward pass of :func:`router_topk`: ``dweights [T, topk]`` float32 (what the gated GEMMs return as the gradient of
     the gate probabilities) -> ``dlogits [T, E]`` of the logits' type.  Slots with id -1 have no part; the choice itself has no
     gradient."""
-    ld = _check_logits(logits, score_func)
+    ld = _check_logits(logits, score_func, ids.shape[-1] if ids.dim() else 0)
     t, e = logits.shape
     if ids.dim() != 2 or ids.shape[0] != t or ids.dtype != torch.int32 or ids.device != logits.device or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 [{t}, topk] tensor on {logits.device}")

@@ -262,3 +262,21 @@ def test_gate_feeds_the_expert_path():
 
 def rel(got, want):
     return float((got.double() - want).norm() / want.norm())
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    """2^32 + 2 choices are refused before anything of that size is allocated; the C entry point would see 2."""
+    import cudnn_frontend_b200 as cf
+
+    logits = torch.zeros((4, 8), device="cuda")
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    wide = torch.zeros((1, 1), device="cuda").as_strided((0, 2**32 + 8), (2**32 + 8, 1))  # (no rows: nothing to allocate)
+    for call in (
+        lambda: cf.router_topk(logits, 2**32 + 2),
+        lambda: cf.router_topk(wide, 2),
+        lambda: cf.router_topk_backward(logits[:0, :2], wide, torch.zeros((0, 2), dtype=torch.int32, device="cuda")),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.cuda.max_memory_allocated() <= held + 4096
