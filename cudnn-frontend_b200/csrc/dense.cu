@@ -517,32 +517,30 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
       }
     }
   };
-  // kTrans: kN values of feature `row` for the tokens col0 + c0 + j step, of which the first `count` exist; v = the accumulator
+  // kTrans: kN values of feature `row` for the tokens col0 + c0 + j, of which the first `count` exist; v = the accumulator
   // (GLU: the gate's), u = the up projection's.  Every choice is a branch around a whole loop.
   const float unscale = !kGlu && finisher ? grad_unscale(p.amax) : 1.0f;
   // residual values (raw) of the same elements; their loads are issued by `fetch`, ahead of whatever v waits for
-  auto fetch = [&](auto size, int row, int c0, int step, int count, uint16_t* raw) {
+  auto fetch = [&](auto size, int row, int c0, int count, uint16_t* raw) {
     constexpr int kN = decltype(size)::value;
     if (kEpi != DENSE_LINEAR || !p.residual) return;
     const uint16_t* r = reinterpret_cast<const uint16_t*>(p.residual) + (int64_t)(col0 + c0) * p.ld_res + row;
-    const int64_t hop = p.ld_res * step;
 #pragma unroll
-    for (int j = 0; j < kN; ++j, r += hop)
+    for (int j = 0; j < kN; ++j, r += p.ld_res)
       if (j < count) raw[j] = __ldg(r);
   };
-  auto finish = [&](auto size, int row, int c0, int step, int count, float bias, float* v, const float* u, const uint16_t* raw) {
+  auto finish = [&](auto size, int row, int c0, int count, float bias, float* v, const float* u, const uint16_t* raw) {
     constexpr int kN = decltype(size)::value;
     const int64_t t0 = col0 + c0;
     auto put = [&](void* base, int64_t ld, const float* w) {
       uint16_t* d = reinterpret_cast<uint16_t*>(base) + t0 * ld + row;
-      const int64_t hop = ld * step;
       if (f16) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j, d += hop)
+        for (int j = 0; j < kN; ++j, d += ld)
           if (j < count) *d = __half_as_ushort(__float2half_rn(w[j]));
       } else {
 #pragma unroll
-        for (int j = 0; j < kN; ++j, d += hop)
+        for (int j = 0; j < kN; ++j, d += ld)
           if (j < count) *d = __bfloat16_as_ushort(__float2bfloat16_rn(w[j]));
       }
     };
@@ -566,9 +564,8 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
     }
     if (p.out_f32) {
       float* d = reinterpret_cast<float*>(p.out[0]) + t0 * p.ld_out + row;
-      const int64_t hop = p.ld_out * step;
 #pragma unroll
-      for (int j = 0; j < kN; ++j, d += hop)
+      for (int j = 0; j < kN; ++j, d += p.ld_out)
         if (j < count) *d = v[j];
     } else {
       put(p.out[0], p.ld_out, v);
@@ -634,7 +631,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
           const int c = (rank * slice4 + g) * 4, count = min(4, valid - c);
           if (count <= 0) break;
           uint16_t raw[4];
-          if constexpr (kTrans) fetch(std::integral_constant<int, 4>(), row, c, 1, count, raw);
+          if constexpr (kTrans) fetch(std::integral_constant<int, 4>(), row, c, count, raw);
           float v[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           for (int q = 0; q < split; ++q) {
             const float4 w = part[(q * slice4 + g) * 128];
@@ -645,7 +642,7 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
             }
           }
           if constexpr (kTrans) {
-            finish(std::integral_constant<int, 4>(), row, c, 1, count, bias, v, u, raw);
+            finish(std::integral_constant<int, 4>(), row, c, count, bias, v, u, raw);
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -661,21 +658,21 @@ __global__ void __launch_bounds__(DENSE_BOUND, kSeg ? 1 : 2) dense_tile_kernel(c
     uint16_t raw[16];
     const std::integral_constant<int, 8> eight;
     const std::integral_constant<int, 16> sixteen;
-    if (kTrans && row_ok && half * 16 < valid) fetch(sixteen, row, half * 16, 1, valid - half * 16, raw);
+    if (kTrans && row_ok && half * 16 < valid) fetch(sixteen, row, half * 16, valid - half * 16, raw);
     each_chunk([&](int c0, const float* v) {
       if (!row_ok) return;
       if constexpr (kTrans) {
         uint16_t now[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) now[j] = raw[j];
-        if (c0 + 32 < valid) fetch(sixteen, row, c0 + 32, 1, valid - c0 - 32, raw);  // this warp's next chunk
+        if (c0 + 32 < valid) fetch(sixteen, row, c0 + 32, valid - c0 - 32, raw);  // this warp's next chunk
 #pragma unroll
         for (int h = 0; h < 16; h += 8) {
           if (c0 + h >= valid) break;
           float w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) w[j] = v[h + j];
-          finish(eight, row, c0 + h, 1, min(8, valid - c0 - h), bias, w, w, now + h);
+          finish(eight, row, c0 + h, min(8, valid - c0 - h), bias, w, w, now + h);
         }
       } else {
         const int64_t o = (int64_t)row * p.ld_out + col0 + c0;
@@ -756,7 +753,7 @@ struct PairParams {
   int jobs;
   int full_rounds, rest;      // job 0: every pair takes full_rounds tiles, the first `rest` pairs one more
   int early, early_tiles;     // rounds (and tiles) of job 1 that the other pairs take before all join
-  int act, f16, out_f32, bias_f32;
+  int act, f16, bias_f32;
   void* pre[2];
   int64_t ld_pre[2];
   const void* bias;
@@ -1240,15 +1237,15 @@ __global__ void __launch_bounds__(256)
     if constexpr (kFind) {
       find_max8(g, top);
       find_max8(u, top);
-      continue;
-    }
-    if constexpr (kF16) {
+    } else {
+      if constexpr (kF16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] *= scale, u[j] *= scale;
+        for (int j = 0; j < 8; ++j) g[j] *= scale, u[j] *= scale;
+      }
+      // (the padding columns of the last 8 are written too: they are part of the padded row)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = pack8<kF16>(g);
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = pack8<kF16>(u);
     }
-    // (the padding columns of the last 8 are written too: they are part of the padded row)
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dg) + r * ldo + c) = pack8<kF16>(g);
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(du) + r * ldo + c) = pack8<kF16>(u);
   }
   if constexpr (kFind) publish_max(top, amax);
 }
@@ -1295,15 +1292,15 @@ __global__ void __launch_bounds__(256)
         }
         if constexpr (kFind) {
           find_max8(d, top);
-          continue;
-        }
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += d[j];
-        if constexpr (kF16) {
+          for (int j = 0; j < 8; ++j) acc[j] += d[j];
+          if constexpr (kF16) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] *= scale;
+            for (int j = 0; j < 8; ++j) d[j] *= scale;
+          }
+          if (dz) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = pack8<kF16>(d);
         }
-        if (dz) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dz) + row * ldo + c) = pack8<kF16>(d);
       }
     }
   }
