@@ -173,7 +173,7 @@ __device__ __forceinline__ float2 unpack16x2(uint32_t w, bool f16) {
 // (the bits of a float32, kept on the device) into [2^14, 2^15).  fp16 holds 2^-24 to 65504, a gradient from float32 values or from
 // products with `up` may lie anywhere; so scaled, values down to 2^-28 of the largest keep all their bits and none
 // overflows.  The sums of the products are taken back by the inverse, in float32: both factors are exact.  Finding amax takes a pass of its own
-// over what dz is formed from (backward pass of the gated block, 1531 x 7168, 2048: 157 -> 161 to 166 us).
+// over what dz is formed from (backward pass of the gated block, 1531 x 7168, 2048: 157 -> 165 us).
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ int grad_exponent(uint32_t amax) { return amax ? min(14 - ((int)(amax >> 23) - 127), 126) : 0; }
 __device__ __forceinline__ float pow2_f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -182,7 +182,8 @@ __device__ __forceinline__ float grad_unscale(const uint32_t* amax) { return ama
 
 // ---------------------------------------------------------------------------------------
 // Activations.  sigmoid(v) = 1 / (1 + 2^(-v log2 e)) on the approximate exponential and reciprocal (about 2^-22
-// relative each): the results are rounded to 16 bits, where that is a 2^-10th of a step.
+// relative each, where the exponential's argument is small; its rounding costs 2^-24 of the argument, so 4e-6 at v = -80, and below
+// -87 the result is 0).  Of a 16-bit result that is a 2^-7th of a step or less; float32 results carry it as it is.
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.0f + ex2_approx(v * -1.4426950408889634f)); }
 
@@ -1420,6 +1421,8 @@ static double memory_ns(const DenseGemm& g) {
 // Columns of the tile kernel's tiles (as many as there are, up to 128; an MN-major B comes in slabs of 64) and the CTAs that
 // share a tile's reduction.  A stage takes a CTA 190 ns (the issuer's loop) or as long as its bytes take at 160 GB/s for the SM
 // and 15.8 TB/s for all of L2; two CTAs run on an SM at once; joining partial sums costs more the more columns and CTAs.
+// (Float32 outputs are taken for the same, but their registers leave one CTA to an SM: beyond one round of CTAs these times are
+// too short for them and the ring they get is half of what they could have.  The fit had no such case.)
 struct TileShape {
   int cols, split;
   int64_t tiles;

@@ -6,8 +6,9 @@ product in one kernel.  ``linear`` is the projection behind it or the router's, 
 residual in its epilogue.  Both have their backward pass.  The reference has no counterpart.
 
 All functions take bf16 or fp16 tensors ``[rows, cols]`` with contiguous rows (any pitch that is a multiple
-of 8 elements, 16-byte aligned, for what a tensor map reads: ``x`` and the weights), sum in float32 and round
-once.  They allocate their outputs and launch on ``stream`` (default: the current stream of the tensors' device); when
+of 8 elements, 16-byte aligned, for what a tensor map reads: ``x`` and the weights) and sum in float32.  The forward
+functions round their results once; the backward functions round twice, the gradient operand that both products share and
+the results.  They allocate their outputs and launch on ``stream`` (default: the current stream of the tensors' device); when
 another stream is passed, outputs and workspace belong to that stream, and inputs must stay alive until it has passed the
 call.  They are not recorded by autograd: the backward functions are called explicitly, as with the grouped GEMMs.
 While ``torch.compile`` traces, the forward functions go through custom ops (``torch.ops.b200moe.gated_ffn`` and ``linear``),
@@ -146,8 +147,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, return_preact: bool = False, stream=None):  # fmt: skip
     """``act(x weight^T + bias) + residual``: ``x [tokens, k]``, ``weight [n, k]``, ``bias [n]`` (x's type or float32),
     ``residual [tokens, n]`` (x's type; a pitch of 0, one row for every token, included) -> ``[tokens, n]`` of
-    ``out_dtype`` (x's type, or float32, which is then exact to float32 rounding).  ``act_func``: ``None``, ``"relu"``,
-    ``"silu"`` or ``"gelu"`` (the error-function form).  With ``return_preact`` the result is ``(y, x weight^T + bias)``,
+    ``out_dtype`` (x's type, or float32).  ``act_func``: ``None``, ``"relu"``, ``"silu"`` or ``"gelu"`` (the error-function form).
+    A float32 result is not exact to its rounding: the tensor cores truncate within 512 elements of k (4e-7 of the terms' size
+    at most in the mean), SiLU and GELU are good to about 1e-6 and in their negative tails to 8e-6 relative, and SiLU is 0 below -87.  With ``return_preact`` the result is ``(y, x weight^T + bias)``,
     the second in x's type, for :func:`linear_backward`."""
     if torch.compiler.is_compiling():
         _eager_stream_only(stream)
