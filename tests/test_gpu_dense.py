@@ -712,3 +712,24 @@ def test_expired_waits_store_nothing(m, k, n, form):
     torch.cuda.synchronize()
     assert ops.device_status(clear=True) == 0
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_float16_gated_workspace_without_the_scale_is_refused():
+    """The size that bf16 needs is 256 bytes short in fp16: refused with the size, nothing written."""
+    import ctypes
+
+    from cudnn_frontend_b200 import _lib
+
+    lib, (m, k, n) = _lib.load(), (16, 64, 32)
+    gen = torch.Generator(device="cuda").manual_seed(26)
+    x, w, t = rows(gen, m, k, FP16), rows(gen, n, k, FP16), rows(gen, m, n, FP16)
+    dx = torch.full_like(x, 3.0)
+    need = lib.b200moe_dense_workspace_bytes(m, n, 1 | _lib.DENSE_WORKSPACE_F16)
+    work = torch.empty((need,), dtype=torch.uint8, device="cuda")
+    for size, code in ((lib.b200moe_dense_workspace_bytes(m, n, 1), _lib.E_WORKSPACE), (need, 0)):
+        args = _lib.DenseArgs(x=x.data_ptr(), w0=w.data_ptr(), w1=w.data_ptr(), dy=t.data_ptr(), pre0=t.data_ptr(), pre1=t.data_ptr(), dx=dx.data_ptr(),
+                              workspace=work.data_ptr(), workspace_bytes=size, m=m, n=n, k=k, ld_x=k, ld_w0=k, ld_w1=k, ld_dy=n, ld_pre0=n, ld_pre1=n,
+                              dtype=_lib.DTYPE_F16, act=_lib.ACT_SWIGLU)  # fmt: skip
+        assert lib.b200moe_gated_ffn_backward(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == code
+        assert str(need) in _lib.last_error() if code else True
+        assert bool((dx == 3.0).all()) == (code != 0)
